@@ -214,7 +214,7 @@ def _own(s):
     q = paged.append(kv, batch, s["qkv"], s["inv_freq"], **kw)
     if case["op"] == "append":
         return q, s["k"], s["v"]
-    return (q,) + paged.read(kv, batch, dtype=s["qkv"].dtype)
+    return (q,) + paged.read(kv, batch, s["rows"], dtype=s["qkv"].dtype)
 
 
 def _plain_places(s):
