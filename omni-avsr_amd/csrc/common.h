@@ -69,8 +69,8 @@ __device__ __forceinline__ float gelu_erf(float x) { return 0.5f * x * (1.0f + e
 //         has the same bits whichever kernel produced it.
 template <typename T> __device__ __forceinline__ float gelu_act(float x);
 template <> __device__ __forceinline__ float gelu_act<float>(float x) { return gelu_erf(x); }
-// Written for two elements at a time in packed fp32 math (v_pk_mul / v_pk_fma / v_pk_add; only the rcp / exp2 stay scalar):
-// that halves the VALU issue slots of the fc1 epilogues.  The scalar entry point is the same code on a duplicated lane.
+// Written for two elements at a time; the library is built without packed fp32 instructions, so each operation is two scalar ones.  The scalar
+// entry point is the same code on a duplicated lane.
 __device__ __forceinline__ f32x2 gelu_act2_bf16(f32x2 x) {
   const f32x2 ax = f32x2{fabsf(x[0]), fabsf(x[1])};
   const f32x2 z = ax * 0.70710678118654752440f;
