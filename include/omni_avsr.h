@@ -25,7 +25,8 @@ extern "C" {
  * 3 (round 5): oavsr_gemm_desc follows the single decode regime (weight-streaming decode kernels removed: no `skinny` / norm_gain / rn_* /
  * shared_chip; `kernel`, decode_tiled, sync, row_scale, ng_* added); oavsr_generate / _submit take optional per-utterance digest buffers.
  * 4 (round 6): oavsr_gemm_desc gained rowsq_strips / row_sumsq_form (the <= 32-row strip kernels' layout of the deferred RMSNorm's sums of
- * squares); oavsr_get_launch_objective added.
+ * squares); oavsr_get_launch_objective added.  The paged-cache entry points (oavsr_op_qk_norm_rope, oavsr_op_paged_*) are additions to 4: nothing
+ * that was there changed.
  * A binding built against an older version must not load. */
 #define OAVSR_ABI_VERSION 4
 #define OAVSR_DT_F32 0  /* parity mode: exact-f32 MFMA */
@@ -323,6 +324,91 @@ typedef struct oavsr_decode_attn_desc {
   const int32_t *pos, *cpos;
 } oavsr_decode_attn_desc;
 int oavsr_op_decode_attention(const oavsr_decode_attn_desc* d, oavsr_stream stream);
+
+/* ---- paged key / value cache ------------------------------------------------------------------------------
+ * The cache of a decoder layer as a pool of pages of page_size tokens, given to sequences one page at a time, so that contexts of any length share one
+ * pool without a maximum each.  Four operators work on it: norm + rotation of the fused [q | k | v] rows (oavsr_op_qk_norm_rope, also of use without
+ * a cache), the same pass writing keys and values into the pages (oavsr_op_paged_append), reading rows back (oavsr_op_paged_read), and attention of a
+ * batch's new tokens over their cached context (oavsr_op_paged_attention).  A decoder layer calls append, then attention, for a prompt, a chunk of
+ * one, a single token, or all of these in one batch.  omni_avsr_amd/paged.py binds them to tensors. */
+#define OAVSR_KV_SAME 0 /* keys and values in `dtype` */
+#define OAVSR_KV_E4M3 1 /* 8 bits: e4m3 bytes and one f32 scale per (token, kv head) for the key and one for the value */
+
+typedef struct oavsr_paged_kv {
+  int32_t dtype;      /* OAVSR_DT_*: of the rows that are written, read back, or attend */
+  int32_t format;     /* OAVSR_KV_* */
+  int32_t n_kv_heads, head_dim, page_size, n_pages; /* head_dim 64 or 128; page_size a power of two, 16 .. 256 */
+  void *K, *V;                                      /* [n_pages][n_kv_heads][page_size][head_dim], 16-byte aligned */
+  int64_t page_stride;                              /* elements from one page to the next (>= n_kv_heads * page_size * head_dim, whole 16 bytes) */
+  float *k_scale, *v_scale;                         /* E4M3: [n_pages][n_kv_heads][page_size], 16-byte aligned; else NULL */
+  int64_t scale_stride;                             /* floats from one page's scales to the next (>= n_kv_heads * page_size, a multiple of 4) */
+  /* Optional device word.  The lengths and page numbers of a batch live on the device and are checked there: whatever they hold, nothing outside the
+     given buffers is touched.  A launch that meets a bad one ORs its bit into *status and goes on. */
+  int32_t* status;
+} oavsr_paged_kv;
+#define OAVSR_PAGED_BAD_PAGE 1 /* a page number outside [0, n_pages) inside a context: its tokens are not written, and read and attend as zeros */
+#define OAVSR_PAGED_BAD_LENGTH 2 /* a context longer than max_ctx (its tokens from max_ctx on are not written and not seen), more new tokens than max_q, a
+                                    negative length, or cu_q that falls or passes `rows` (such a sequence is skipped) */
+
+/* Sequence s brings the new tokens of rows cu_q[s] .. cu_q[s + 1] - 1; row i of them is token p = ctx_len[s] - (cu_q[s + 1] - cu_q[s]) + i of its
+ * sequence (ctx_len counts them), which lies in page table[s * ld_table + p / page_size] at place p % page_size.  Rows behind cu_q[n_seqs], and rows
+ * with p < 0 in append and read, are left as they were.  Two sequences may share pages that a call only reads; a call must not write one place twice. */
+typedef struct oavsr_paged_batch {
+  int32_t n_seqs, rows;   /* rows: of the row buffers (>= cu_q[n_seqs]) */
+  int32_t max_q, max_ctx; /* host bounds of a sequence's new tokens and of ctx_len; max_ctx <= ld_table * page_size */
+  const int32_t *cu_q, *ctx_len, *table; /* device: [n_seqs + 1], [n_seqs], [n_seqs][ld_table] */
+  int64_t ld_table;
+} oavsr_paged_batch;
+
+/* For a program that builds its tables on the host: the bits (OAVSR_PAGED_BAD_*) that a launch over this batch would set, 0 for a sound one.  cu_q, ctx_len
+ * and table are HOST arrays here; no device is touched, and kv's pointers are not followed.  < 0: refused. */
+int oavsr_paged_check_host(const oavsr_paged_kv* kv, const oavsr_paged_batch* b);
+
+/* One pass over fused rows [n_heads q | n_kv_heads k | n_kv_heads v] x head_dim.  Per q and k head, in f32:  x = x * rsqrt(mean(x^2) + eps) * gain
+ * (q_gain / k_gain; NULL: no norm);  then, with inv_freq, the pairs of the first rot_dim dimensions turn by pos * inv_freq[i]:
+ * (a, b) -> rot_scale * (a cos - b sin, b cos + a sin), pair i being dimensions (i, i + rot_dim / 2), or (2i, 2i + 1) when interleaved.  The angle is formed
+ * in 64 bits (oavsr_op_rope_kv: in 32), so it holds at any position.  One rounding, at the end. */
+typedef struct oavsr_qk_rope_desc {
+  int32_t dtype, rows, n_heads, n_kv_heads, head_dim;
+  const void* qkv; int64_t ld;
+  void* q_out; int64_t ldq; /* [rows][n_heads * head_dim]; may be the q part of qkv itself */
+  void* k_out; int64_t ldk; /* [rows][n_kv_heads * head_dim]; may be the k part of qkv itself; append: unused */
+  const int32_t* pos;       /* [rows]; append: NULL = the token's place in its sequence */
+  const float* inv_freq;    /* [rot_dim / 2], with any long-context scaling in it; NULL: no rotation */
+  int32_t rot_dim;          /* multiple of 16, <= head_dim */
+  int32_t interleaved;
+  float rot_scale;          /* factor of the rotated dimensions (1: none) */
+  const float *q_gain, *k_gain; /* [head_dim] each; both or neither */
+  float eps;
+} oavsr_qk_rope_desc;
+int oavsr_op_qk_norm_rope(const oavsr_qk_rope_desc* d, oavsr_stream stream);
+/* The pass above, the keys (after norm and rotation) and the values going into the pages instead of k_out.  E4M3: scale = max(amax / 448, 2^-126) over the
+ * head's f32 values, byte = the e4m3 value nearest to x / scale (ties to even); a head that holds an infinity or a NaN reads back as NaN throughout.
+ * d->rows, n_kv_heads, head_dim and dtype must be the batch's and the cache's. */
+int oavsr_op_paged_append(const oavsr_paged_kv* kv, const oavsr_paged_batch* b, const oavsr_qk_rope_desc* d, oavsr_stream stream);
+/* k_out / v_out [rows][n_kv_heads * head_dim] (row strides ldk / ldv; either may be NULL) = the cached values of the batch's rows, in kv->dtype.  (A batch
+ * whose new tokens are whole contexts reads whole contexts.) */
+int oavsr_op_paged_read(const oavsr_paged_kv* kv, const oavsr_paged_batch* b, void* k_out, int64_t ldk, void* v_out, int64_t ldv, oavsr_stream stream);
+
+/* O[row][h] = softmax over the keys j <= p of the row's sequence of (scale q . k_j), times v_j;  kv head h / (n_heads / n_kv_heads).  Scores and softmax
+ * statistics in f32; keys a row does not see do not count, whatever their bytes hold.  A row that sees no key (p < 0): zeros, lse = -infinity. */
+typedef struct oavsr_paged_attn_desc {
+  int32_t n_heads;
+  float scale;         /* > 0 */
+  const void* Q; int64_t ldq; /* [rows][n_heads * head_dim], kv->dtype */
+  void* O; int64_t ldo;
+  float* lse;          /* optional [rows][n_heads]: natural logarithm of the sum of exponentials of a row's scores */
+  /* Long contexts of few rows are split: workgroups take split_keys keys each and a second launch joins their partial results.  0: the launcher's rule,
+     which follows the batch's bounds (so the last bits of a row may follow them); a multiple of 256: this split, the same bits for a row in any batch of
+     the same max_q. */
+  int32_t split_keys;
+  void* workspace;     /* device, oavsr_paged_attention_workspace() bytes, 16-byte aligned; free for anything once the launch has run; launches that may
+                          run at the same time need one each */
+  uint64_t workspace_bytes;
+} oavsr_paged_attn_desc;
+int oavsr_op_paged_attention(const oavsr_paged_kv* kv, const oavsr_paged_batch* b, const oavsr_paged_attn_desc* d, oavsr_stream stream);
+/* bytes of workspace the call needs (0: none; d's pointers are not looked at); < 0: the call would be refused */
+int64_t oavsr_paged_attention_workspace(const oavsr_paged_kv* kv, const oavsr_paged_batch* b, const oavsr_paged_attn_desc* d);
 
 /* mode: 0 LayerNorm, 1 RMSNorm, 2 LayerNorm over [zeros(D), x] */
 int oavsr_op_norm(int32_t mode, int32_t dtype, const void* x, int64_t ldx, void* y, int64_t ldy, const float* w, const float* b,

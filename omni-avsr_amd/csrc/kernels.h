@@ -158,6 +158,44 @@ struct DecodeAttnArgs {
 };
 int launch_decode_attention(const DecodeAttnArgs& a, hipStream_t st);
 
+// ---- paged key / value cache (paged.hip, paged_attn.hip; the fields are those of include/omni_avsr.h: oavsr_paged_*) ----
+enum KvFormat : int { KV_SAME = 0, KV_E4M3 = 1 };
+struct PagedKv {
+  int dtype = DT_BF16, format = KV_SAME;
+  int n_kv_heads = 0, head_dim = 64, page_size = 64, n_pages = 0;
+  void *K = nullptr, *V = nullptr; int64_t page_stride = 0;
+  float *k_scale = nullptr, *v_scale = nullptr; int64_t scale_stride = 0;
+  int* status = nullptr;
+};
+struct PagedBatch {
+  int n_seqs = 0, rows = 0, max_q = 0, max_ctx = 0;
+  const int *cu_q = nullptr, *ctx_len = nullptr, *table = nullptr; int64_t ld_table = 0;
+};
+struct QkRopeArgs {
+  int dtype = DT_BF16, rows = 0, n_heads = 0, n_kv_heads = 0, head_dim = 64;
+  const void* qkv = nullptr; int64_t ld = 0;
+  void* q_out = nullptr; int64_t ldq = 0;
+  void* k_out = nullptr; int64_t ldk = 0;
+  const int* pos = nullptr;
+  const float* inv_freq = nullptr; int rot_dim = 0, interleaved = 0; float rot_scale = 1.f;
+  const float *q_gain = nullptr, *k_gain = nullptr; float eps = 0.f;
+};
+struct PagedAttnArgs {
+  int n_heads = 0; float scale = 1.f;
+  const void* Q = nullptr; int64_t ldq = 0;
+  void* O = nullptr; int64_t ldo = 0;
+  float* lse = nullptr;
+  int split_keys = 0;
+  void* workspace = nullptr; uint64_t workspace_bytes = 0;
+};
+int launch_qk_norm_rope(const QkRopeArgs& a, hipStream_t st);
+int launch_paged_append(const PagedKv& kv, const PagedBatch& b, const QkRopeArgs& a, hipStream_t st);
+int launch_paged_read(const PagedKv& kv, const PagedBatch& b, void* k_out, int64_t ldk, void* v_out, int64_t ldv, hipStream_t st);
+int launch_paged_attention(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a, hipStream_t st);
+int64_t paged_attention_workspace(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a);      // < 0: refused
+int check_paged(const PagedKv& kv, const PagedBatch& b, const char* who);                              // what every paged launch asks of its cache and batch
+int check_paged_host(const PagedKv& kv, const PagedBatch& b);                                          // b's arrays on the host: the bits a launch would report
+
 // ---- normalisation / elementwise ----------------------------------------------------------------
 int launch_layernorm(int dtype, const void* x, int64_t ldx, void* y, int64_t ldy, const float* w, const float* b,
                      int rows, int D, float eps, hipStream_t st);

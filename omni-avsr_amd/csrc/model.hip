@@ -2225,6 +2225,53 @@ int oavsr_op_decode_attention(const oavsr_decode_attn_desc* d, oavsr_stream stre
   return launch_decode_attention(a, (hipStream_t)stream);
 }
 
+static PagedKv paged_kv_of(const oavsr_paged_kv* d) {
+  PagedKv k; k.dtype = d->dtype; k.format = d->format; k.n_kv_heads = d->n_kv_heads; k.head_dim = d->head_dim; k.page_size = d->page_size;
+  k.n_pages = d->n_pages; k.K = d->K; k.V = d->V; k.page_stride = d->page_stride; k.k_scale = d->k_scale; k.v_scale = d->v_scale;
+  k.scale_stride = d->scale_stride; k.status = d->status;
+  return k;
+}
+static PagedBatch paged_batch_of(const oavsr_paged_batch* d) {
+  PagedBatch b; b.n_seqs = d->n_seqs; b.rows = d->rows; b.max_q = d->max_q; b.max_ctx = d->max_ctx; b.cu_q = d->cu_q; b.ctx_len = d->ctx_len;
+  b.table = d->table; b.ld_table = d->ld_table;
+  return b;
+}
+static QkRopeArgs qk_rope_of(const oavsr_qk_rope_desc* d) {
+  QkRopeArgs a; a.dtype = d->dtype; a.rows = d->rows; a.n_heads = d->n_heads; a.n_kv_heads = d->n_kv_heads; a.head_dim = d->head_dim; a.qkv = d->qkv;
+  a.ld = d->ld; a.q_out = d->q_out; a.ldq = d->ldq; a.k_out = d->k_out; a.ldk = d->ldk; a.pos = d->pos; a.inv_freq = d->inv_freq;
+  a.rot_dim = d->rot_dim; a.interleaved = d->interleaved; a.rot_scale = d->rot_scale; a.q_gain = d->q_gain; a.k_gain = d->k_gain; a.eps = d->eps;
+  return a;
+}
+static PagedAttnArgs paged_attn_of(const oavsr_paged_attn_desc* d) {
+  PagedAttnArgs a; a.n_heads = d->n_heads; a.scale = d->scale; a.Q = d->Q; a.ldq = d->ldq; a.O = d->O; a.ldo = d->ldo; a.lse = d->lse;
+  a.split_keys = d->split_keys; a.workspace = d->workspace; a.workspace_bytes = d->workspace_bytes;
+  return a;
+}
+int oavsr_op_qk_norm_rope(const oavsr_qk_rope_desc* d, oavsr_stream stream) {
+  OAVSR_REQUIRE(d, "op_qk_norm_rope: null desc");
+  return launch_qk_norm_rope(qk_rope_of(d), (hipStream_t)stream);
+}
+int oavsr_paged_check_host(const oavsr_paged_kv* kv, const oavsr_paged_batch* b) {
+  OAVSR_REQUIRE(kv && b, "paged_check_host: null desc");
+  return check_paged_host(paged_kv_of(kv), paged_batch_of(b));
+}
+int oavsr_op_paged_append(const oavsr_paged_kv* kv, const oavsr_paged_batch* b, const oavsr_qk_rope_desc* d, oavsr_stream stream) {
+  OAVSR_REQUIRE(kv && b && d, "op_paged_append: null desc");
+  return launch_paged_append(paged_kv_of(kv), paged_batch_of(b), qk_rope_of(d), (hipStream_t)stream);
+}
+int oavsr_op_paged_read(const oavsr_paged_kv* kv, const oavsr_paged_batch* b, void* k_out, int64_t ldk, void* v_out, int64_t ldv, oavsr_stream stream) {
+  OAVSR_REQUIRE(kv && b, "op_paged_read: null desc");
+  return launch_paged_read(paged_kv_of(kv), paged_batch_of(b), k_out, ldk, v_out, ldv, (hipStream_t)stream);
+}
+int oavsr_op_paged_attention(const oavsr_paged_kv* kv, const oavsr_paged_batch* b, const oavsr_paged_attn_desc* d, oavsr_stream stream) {
+  OAVSR_REQUIRE(kv && b && d, "op_paged_attention: null desc");
+  return launch_paged_attention(paged_kv_of(kv), paged_batch_of(b), paged_attn_of(d), (hipStream_t)stream);
+}
+int64_t oavsr_paged_attention_workspace(const oavsr_paged_kv* kv, const oavsr_paged_batch* b, const oavsr_paged_attn_desc* d) {
+  OAVSR_REQUIRE(kv && b && d, "paged_attention_workspace: null desc");
+  return paged_attention_workspace(paged_kv_of(kv), paged_batch_of(b), paged_attn_of(d));
+}
+
 int oavsr_op_norm(int32_t mode, int32_t dtype, const void* x, int64_t ldx, void* y, int64_t ldy, const float* w, const float* b, int32_t rows,
                   int32_t D, float eps, oavsr_stream stream) {
   hipStream_t st = (hipStream_t)stream;

@@ -1,0 +1,339 @@
+// Rows into and out of a paged key / value cache, and the norm + rotation of queries and keys in the same pass.
+//
+// qk_rope_kernel: a fused row is [q heads | k heads | v heads] x head_dim.  Per q and k head, in f32,
+//     x <- x * rsqrt(mean x^2 + eps) * gain,     (a, b) <- m (a cos t - b sin t, b cos t + a sin t),  t = pos * f_i,
+// one rounding at the end; then q to its buffer, k to its buffer or (CACHE) its page, v to its page, in 8 bits (F8) with one scale per head.
+//   * HBM bound: a row is read once and written once.  head_dim / 16 lanes own a head, a lane two 16-byte pieces of it (bf16): the two that turn with
+//     each other, so a rotation needs no exchange between lanes; the norm's and the scale's reductions are butterflies over those 4 or 8 lanes.
+//   * The angle of a far position does not fit 32 bits (pos = 10^5, f = 1: spacing 0.008): it is formed in f64 as a number of quarter turns, whose
+//     fraction is exact to 2^-25 of a turn after the integer part is dropped.  A wave computes the row's <= 64 angles once, one per lane, and every head
+//     it handles reads them from LDS.
+#include "paged.h"
+
+namespace oavsr {
+namespace {
+
+constexpr int kThreads = 256, kWaves = 4;
+
+template <typename T> __device__ __forceinline__ void load8(const T* p, float* x);
+template <> __device__ __forceinline__ void load8<bf16_t>(const bf16_t* p, float* x) { chunk_to_f32<bf16_t>(*reinterpret_cast<const Chunk16*>(p), x); }
+template <> __device__ __forceinline__ void load8<float>(const float* p, float* x) {
+  chunk_to_f32<float>(*reinterpret_cast<const Chunk16*>(p), x);
+  chunk_to_f32<float>(*reinterpret_cast<const Chunk16*>(p + 4), x + 4);
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const float* x);
+template <> __device__ __forceinline__ void store8<bf16_t>(bf16_t* p, const float* x) { *reinterpret_cast<Chunk16*>(p) = chunk_from_f32<bf16_t>(x); }
+template <> __device__ __forceinline__ void store8<float>(float* p, const float* x) {
+  *reinterpret_cast<Chunk16*>(p) = chunk_from_f32<float>(x);
+  *reinterpret_cast<Chunk16*>(p + 4) = chunk_from_f32<float>(x + 4);
+}
+
+// cos and sin of pos * f
+__device__ __forceinline__ float2 turn_of(int pos, float f) {
+  const double quarters = (double)pos * (double)f * 0.63661977236758134308;      // 2 / pi
+  const double whole = __builtin_rint(quarters);
+  float s, c;
+  sincospif(0.5f * (float)(quarters - whole), &s, &c);                           // within an eighth of a turn of 0
+  const int k = (int)((long long)whole & 3);
+  const float c1 = (k & 1) ? s : c, s1 = (k & 1) ? c : s;
+  return make_float2((k == 1 || k == 2) ? -c1 : c1, (k & 2) ? -s1 : s1);
+}
+
+// x / scale as an f32 that rounds to e4m3 as the exact quotient does: cut off towards zero, the lowest bit set where anything was cut (round to odd).
+// Plain f32 division lands on the middle between two e4m3 values too often (bf16 inputs: 8-bit numerators) and then picks the even one on no ground.
+__device__ __forceinline__ float quotient_odd(float x, float scale, float inv) {
+  const float y0 = x * inv, y = fmaf(fmaf(-y0, scale, x), inv, y0);
+  const float r = fmaf(-y, scale, x);                                            // x - y * scale, exact
+  const bool unlike = (__builtin_bit_cast(int, r) ^ __builtin_bit_cast(int, y)) < 0;
+  const int over = (r != 0.f && unlike) ? 1 : 0;                                 // |y| > |x / scale|
+  const int bits = (__builtin_bit_cast(int, y) - over) | (r != 0.f ? 1 : 0);
+  return __builtin_bit_cast(float, bits);
+}
+
+template <typename T, int HD, bool CACHE, bool F8>
+__global__ __launch_bounds__(kThreads) void qk_rope_kernel(const QkRopeArgs p, const PagedKv kv, const PagedBatch b, int parts) {
+  constexpr int LPH = HD / 16, HPW = 64 / LPH;       // lanes per head, heads per wave
+  __shared__ float2 turns[kWaves][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t task = (int64_t)blockIdx.x * kWaves + wave;
+  const int row = (int)(task / parts), part = (int)(task - (int64_t)row * parts);
+  if (row >= p.rows) return;
+
+  int pos = 0, page = -1, off = 0;
+  if constexpr (CACHE) {
+    const int s = wave_find_seq(b.cu_q, b.n_seqs, row, lane);
+    const SeqInfo q = paged_seq(b, s);
+    if (q.bad && lane == 0 && part == 0) paged_report(kv.status, kBadLength);
+    if (row < q.q0 || row >= q.q0 + q.nq) return;    // behind the last sequence, or of a skipped one
+    pos = q.ctx - (q.nq - (row - q.q0));
+    if (pos < 0) return;
+    if (pos < b.max_ctx) {
+      page = paged_page(kv, b, s, pos, page_shift_of(kv));
+      off = pos & (kv.page_size - 1);
+      if (page < 0 && lane == 0 && part == 0) paged_report(kv.status, kBadPage);
+    }
+    if (p.pos) pos = p.pos[row];
+  } else if (p.inv_freq) pos = p.pos[row];
+
+  const int rl = p.inv_freq ? p.rot_dim / 16 : 0;    // lanes of a head that rotate
+  const int c = lane % LPH;
+  float cs[8], sn[8];
+  if (p.inv_freq) {
+    if (lane < p.rot_dim / 2) {
+      const float2 t = turn_of(pos, p.inv_freq[lane]);
+      turns[wave][lane] = make_float2(t.x * p.rot_scale, t.y * p.rot_scale);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int i0 = c < rl ? 8 * c : 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { const float2 t = turns[wave][i0 + i]; cs[i] = t.x; sn[i] = t.y; }
+  }
+  // the lane's two pieces of a head: the halves' partners where they turn, neighbours elsewhere
+  const bool halves = c < rl && !p.interleaved;
+  const int e0 = 8 * (halves ? c : 2 * c), e1 = 8 * (halves ? c + rl : 2 * c + 1);
+
+  const int heads = p.n_heads + p.n_kv_heads + (CACHE ? p.n_kv_heads : 0);
+  for (int h0 = part * HPW; h0 < heads; h0 += parts * HPW) {
+    const int h = h0 + lane / LPH;
+    if (h >= heads) continue;                        // (whole heads: the lanes of a butterfly stay or leave together)
+    const bool is_q = h < p.n_heads, is_v = h >= p.n_heads + p.n_kv_heads;
+    if (CACHE && !is_q && page < 0) continue;
+    const T* src = reinterpret_cast<const T*>(p.qkv) + (int64_t)row * p.ld + (int64_t)h * HD;
+    float x[16];
+    load8<T>(src + e0, x);
+    load8<T>(src + e1, x + 8);
+    if (!is_v) {
+      if (p.q_gain) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+        for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor(ss, o, 64);
+        const float r = 1.f / sqrtf(ss * (1.f / HD) + p.eps);
+        const float* gain = is_q ? p.q_gain : p.k_gain;
+        float g[16];
+        load8<float>(gain + e0, g);
+        load8<float>(gain + e1, g + 8);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = x[i] * r * g[i];
+      }
+      if (c < rl) {
+        if (p.interleaved) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float a = x[2 * i], bb = x[2 * i + 1];
+            x[2 * i] = a * cs[i] - bb * sn[i];
+            x[2 * i + 1] = bb * cs[i] + a * sn[i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float a = x[i], bb = x[8 + i];
+            x[i] = a * cs[i] - bb * sn[i];
+            x[8 + i] = bb * cs[i] + a * sn[i];
+          }
+        }
+      }
+    }
+    if (is_q || !CACHE) {
+      T* dst = is_q ? reinterpret_cast<T*>(p.q_out) + (int64_t)row * p.ldq + (int64_t)h * HD
+                    : reinterpret_cast<T*>(p.k_out) + (int64_t)row * p.ldk + (int64_t)(h - p.n_heads) * HD;
+      store8<T>(dst + e0, x);
+      store8<T>(dst + e1, x + 8);
+    } else {
+      const int kh = is_v ? h - p.n_heads - p.n_kv_heads : h - p.n_heads;
+      const int64_t tok = (int64_t)kh * kv.page_size + off;
+      void* base = is_v ? kv.V : kv.K;
+      if constexpr (F8) {
+        float m = 0.f;
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { m = fmaxf(m, fabsf(x[i])); odd |= !(fabsf(x[i]) <= 3.402823466e38f); }
+        if (odd) m = INFINITY;
+#pragma unroll
+        for (int o = 1; o < LPH; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        const float scale = m == INFINITY ? NAN : fmaxf(m / 448.f, 1.17549435e-38f);
+        const float inv = 1.f / scale;
+        char* dst = reinterpret_cast<char*>(base) + (int64_t)page * kv.page_stride + tok * HD;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          unsigned w[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float* y = x + 8 * half + 4 * j;
+            int pk = 0;
+            pk = __builtin_amdgcn_cvt_pk_fp8_f32(quotient_odd(y[0], scale, inv), quotient_odd(y[1], scale, inv), pk, false);
+            pk = __builtin_amdgcn_cvt_pk_fp8_f32(quotient_odd(y[2], scale, inv), quotient_odd(y[3], scale, inv), pk, true);
+            w[j] = (unsigned)pk;
+          }
+          *reinterpret_cast<uint2*>(dst + (half ? e1 : e0)) = make_uint2(w[0], w[1]);
+        }
+        if (c == 0) (is_v ? kv.v_scale : kv.k_scale)[(int64_t)page * kv.scale_stride + tok] = scale;
+      } else {
+        T* dst = reinterpret_cast<T*>(base) + (int64_t)page * kv.page_stride + tok * HD;
+        store8<T>(dst + e0, x);
+        store8<T>(dst + e1, x + 8);
+      }
+    }
+  }
+}
+
+// Cached rows back as values: a wave per row, head_dim / 16 lanes per head, keys' heads then values' heads.  HBM bound.
+template <typename T, int HD, bool F8>
+__global__ __launch_bounds__(kThreads) void paged_read_kernel(const PagedKv kv, const PagedBatch b, T* __restrict__ k_out, int64_t ldk, T* __restrict__ v_out, int64_t ldv) {
+  constexpr int LPH = HD / 16, HPW = 64 / LPH;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t task = (int64_t)blockIdx.x * kWaves + wave;
+  if (task >= b.rows) return;
+  const int row = (int)task;
+  const int s = wave_find_seq(b.cu_q, b.n_seqs, row, lane);
+  const SeqInfo q = paged_seq(b, s);
+  if (q.bad && lane == 0) paged_report(kv.status, kBadLength);
+  if (row < q.q0 || row >= q.q0 + q.nq) return;
+  const int pos = q.ctx - (q.nq - (row - q.q0));
+  if (pos < 0) return;
+  int page = -1;
+  if (pos < b.max_ctx) {
+    page = paged_page(kv, b, s, pos, page_shift_of(kv));
+    if (page < 0 && lane == 0) paged_report(kv.status, kBadPage);
+  }
+  const int off = pos & (kv.page_size - 1), c = lane % LPH;
+  for (int h0 = 0; h0 < 2 * kv.n_kv_heads; h0 += HPW) {
+    const int h = h0 + lane / LPH;
+    if (h >= 2 * kv.n_kv_heads) continue;
+    const bool is_v = h >= kv.n_kv_heads;
+    const int kh = is_v ? h - kv.n_kv_heads : h;
+    T* dst = is_v ? v_out : k_out;
+    if (!dst) continue;
+    dst += (int64_t)row * (is_v ? ldv : ldk) + (int64_t)kh * HD + 16 * c;
+    float x[16];
+    if (page < 0) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = 0.f;
+    } else {
+      const int64_t tok = (int64_t)kh * kv.page_size + off;
+      const void* base = is_v ? kv.V : kv.K;
+      if constexpr (F8) {
+        const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(base) + (int64_t)page * kv.page_stride + tok * HD + 16 * c);
+        const float scale = (is_v ? kv.v_scale : kv.k_scale)[(int64_t)page * kv.scale_stride + tok];
+        e4m3_to_f32(w.x, x); e4m3_to_f32(w.y, x + 4); e4m3_to_f32(w.z, x + 8); e4m3_to_f32(w.w, x + 12);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] *= scale;
+      } else {
+        const T* src = reinterpret_cast<const T*>(base) + (int64_t)page * kv.page_stride + tok * HD + 16 * c;
+        load8<T>(src, x);
+        load8<T>(src + 8, x + 8);
+      }
+    }
+    store8<T>(dst, x);
+    store8<T>(dst + 8, x + 8);
+  }
+}
+
+int check_rope(const QkRopeArgs& a, const char* who) {
+  OAVSR_REQUIRE(a.dtype == DT_F32 || a.dtype == DT_BF16, "%s: unknown dtype %d", who, a.dtype);
+  OAVSR_REQUIRE(a.rows >= 0 && a.n_heads > 0 && a.n_kv_heads > 0, "%s: bad sizes (rows %d, heads %d / %d)", who, a.rows, a.n_heads, a.n_kv_heads);
+  OAVSR_REQUIRE(a.head_dim == 64 || a.head_dim == 128, "%s: head_dim %d unsupported", who, a.head_dim);
+  const int vec = a.dtype == DT_F32 ? 4 : 8;
+  OAVSR_REQUIRE(a.ld >= (int64_t)(a.n_heads + 2 * a.n_kv_heads) * a.head_dim && a.ldq >= (int64_t)a.n_heads * a.head_dim, "%s: row strides shorter than the rows", who);
+  OAVSR_REQUIRE(a.ld % vec == 0 && a.ldq % vec == 0 && a.ldk % vec == 0, "%s: rows must be 16-byte aligned", who);
+  OAVSR_REQUIRE(a.rows == 0 || (a.qkv && a.q_out), "%s: null rows", who);
+  OAVSR_REQUIRE((((uintptr_t)a.qkv | (uintptr_t)a.q_out | (uintptr_t)a.k_out | (uintptr_t)a.q_gain | (uintptr_t)a.k_gain) & 15) == 0, "%s: pointers must be 16-byte aligned", who);
+  OAVSR_REQUIRE(!a.q_gain == !a.k_gain, "%s: gains for both queries and keys, or for neither", who);
+  OAVSR_REQUIRE(!a.q_gain || a.eps >= 0.f, "%s: eps %g", who, a.eps);
+  OAVSR_REQUIRE(!a.inv_freq || (a.rot_dim > 0 && a.rot_dim <= a.head_dim && a.rot_dim % 16 == 0), "%s: %d rotated dimensions (a multiple of 16 up to head_dim)", who, a.rot_dim);
+  return 0;
+}
+
+// Waves per row.  One wave per row and pass of heads gives every head its own wave (few rows: a decode step's latency); from kManyRows rows on a wave takes
+// all heads of its row and forms the row's angles once.
+constexpr int kManyRows = 2048;
+template <typename T, bool CACHE, bool F8>
+int launch_rope_t(const QkRopeArgs& a, const PagedKv& kv, const PagedBatch& b, hipStream_t st) {
+  const int hpw = 64 / (a.head_dim / 16), heads = a.n_heads + (CACHE ? 2 : 1) * a.n_kv_heads;
+  const int parts = a.rows >= kManyRows ? 1 : ceil_div(heads, hpw);
+  const int64_t blocks = ceil_div64((int64_t)a.rows * parts, kWaves);
+  OAVSR_REQUIRE(blocks < (1ll << 31), "paged: %d rows are too many for one launch", a.rows);
+  if (a.head_dim == 64) hipLaunchKernelGGL((qk_rope_kernel<T, 64, CACHE, F8>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a, kv, b, parts);
+  else hipLaunchKernelGGL((qk_rope_kernel<T, 128, CACHE, F8>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a, kv, b, parts);
+  OAVSR_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
+template <typename T, bool F8>
+int launch_read_t(const PagedKv& kv, const PagedBatch& b, void* k_out, int64_t ldk, void* v_out, int64_t ldv, hipStream_t st) {
+  const dim3 grid(ceil_div(b.rows, kWaves));
+  if (kv.head_dim == 64) hipLaunchKernelGGL((paged_read_kernel<T, 64, F8>), grid, dim3(kThreads), 0, st, kv, b, (T*)k_out, ldk, (T*)v_out, ldv);
+  else hipLaunchKernelGGL((paged_read_kernel<T, 128, F8>), grid, dim3(kThreads), 0, st, kv, b, (T*)k_out, ldk, (T*)v_out, ldv);
+  OAVSR_CHECK_HIP(hipGetLastError());
+  return 0;
+}
+
+}  // namespace
+
+int check_paged(const PagedKv& kv, const PagedBatch& b, const char* who) {
+  OAVSR_REQUIRE(kv.dtype == DT_F32 || kv.dtype == DT_BF16, "%s: unknown dtype %d", who, kv.dtype);
+  OAVSR_REQUIRE(kv.format == KV_SAME || kv.format == KV_E4M3, "%s: unknown cache format %d", who, kv.format);
+  OAVSR_REQUIRE(kv.head_dim == 64 || kv.head_dim == 128, "%s: head_dim %d unsupported", who, kv.head_dim);
+  OAVSR_REQUIRE(kv.page_size >= 16 && kv.page_size <= 256 && (kv.page_size & (kv.page_size - 1)) == 0, "%s: page_size %d (a power of two, 16 .. 256)", who, kv.page_size);
+  OAVSR_REQUIRE(kv.n_kv_heads > 0 && kv.n_kv_heads <= 65535 && kv.n_pages >= 0, "%s: bad cache sizes (kv heads %d, pages %d)", who, kv.n_kv_heads, kv.n_pages);
+  const int vec = kv.format == KV_E4M3 ? 16 : kv.dtype == DT_F32 ? 4 : 8;
+  OAVSR_REQUIRE(kv.page_stride >= (int64_t)kv.n_kv_heads * kv.page_size * kv.head_dim && kv.page_stride % vec == 0, "%s: page stride %lld", who, (long long)kv.page_stride);
+  OAVSR_REQUIRE(kv.n_pages == 0 || (kv.K && kv.V), "%s: null cache", who);
+  OAVSR_REQUIRE((((uintptr_t)kv.K | (uintptr_t)kv.V | (uintptr_t)kv.k_scale | (uintptr_t)kv.v_scale) & 15) == 0, "%s: pointers must be 16-byte aligned", who);
+  if (kv.format == KV_E4M3) {
+    OAVSR_REQUIRE(kv.n_pages == 0 || (kv.k_scale && kv.v_scale), "%s: an 8-bit cache needs its scales", who);
+    OAVSR_REQUIRE(kv.scale_stride >= (int64_t)kv.n_kv_heads * kv.page_size && kv.scale_stride % 4 == 0, "%s: scale stride %lld", who, (long long)kv.scale_stride);
+  }
+  OAVSR_REQUIRE(b.n_seqs >= 0 && b.rows >= 0 && b.max_q >= 0 && b.max_ctx >= 0, "%s: bad batch sizes (sequences %d, rows %d, max_q %d, max_ctx %d)", who, b.n_seqs, b.rows, b.max_q, b.max_ctx);
+  OAVSR_REQUIRE(b.max_ctx <= (1 << 30), "%s: max_ctx %d", who, b.max_ctx);
+  OAVSR_REQUIRE(b.n_seqs == 0 || (b.cu_q && b.ctx_len && (b.table || b.max_ctx == 0)), "%s: null batch", who);
+  OAVSR_REQUIRE(b.ld_table >= 0 && b.ld_table <= (1ll << 31) && b.max_ctx <= b.ld_table * kv.page_size, "%s: a table of %lld pages does not hold max_ctx %d", who, (long long)b.ld_table, b.max_ctx);
+  return 0;
+}
+
+int check_paged_host(const PagedKv& kv, const PagedBatch& b) {
+  OAVSR_TRY(check_paged(kv, b, "paged_check_host"));
+  int bits = 0;
+  for (int s = 0; s < b.n_seqs; ++s) {
+    const SeqInfo q = paged_seq(b, s);
+    if (q.bad) bits |= kBadLength;
+    const int n = q.ctx < b.max_ctx ? q.ctx : b.max_ctx;
+    for (int pos = 0; pos < n; pos += kv.page_size)
+      if (paged_page(kv, b, s, pos, page_shift_of(kv)) < 0) bits |= kBadPage;
+  }
+  return bits;
+}
+
+int launch_qk_norm_rope(const QkRopeArgs& a, hipStream_t st) {
+  OAVSR_TRY(check_rope(a, "qk_norm_rope"));
+  OAVSR_REQUIRE(a.ldk >= (int64_t)a.n_kv_heads * a.head_dim, "qk_norm_rope: row strides shorter than the rows");
+  OAVSR_REQUIRE(a.rows == 0 || (a.k_out && (a.pos || !a.inv_freq)), "qk_norm_rope: null rows or positions");
+  if (a.rows == 0) return 0;
+  const PagedKv kv; const PagedBatch b;
+  return a.dtype == DT_F32 ? launch_rope_t<float, false, false>(a, kv, b, st) : launch_rope_t<bf16_t, false, false>(a, kv, b, st);
+}
+
+int launch_paged_append(const PagedKv& kv, const PagedBatch& b, const QkRopeArgs& a, hipStream_t st) {
+  OAVSR_TRY(check_paged(kv, b, "paged_append"));
+  OAVSR_TRY(check_rope(a, "paged_append"));
+  OAVSR_REQUIRE(a.rows == b.rows && a.dtype == kv.dtype && a.n_kv_heads == kv.n_kv_heads && a.head_dim == kv.head_dim,
+                "paged_append: rows (%d, dtype %d, %d kv heads of %d) are not the batch's and the cache's (%d, dtype %d, %d of %d)", a.rows, a.dtype, a.n_kv_heads,
+                a.head_dim, b.rows, kv.dtype, kv.n_kv_heads, kv.head_dim);
+  if (a.rows == 0 || b.n_seqs == 0) return 0;
+  if (kv.format == KV_E4M3) return a.dtype == DT_F32 ? launch_rope_t<float, true, true>(a, kv, b, st) : launch_rope_t<bf16_t, true, true>(a, kv, b, st);
+  return a.dtype == DT_F32 ? launch_rope_t<float, true, false>(a, kv, b, st) : launch_rope_t<bf16_t, true, false>(a, kv, b, st);
+}
+
+int launch_paged_read(const PagedKv& kv, const PagedBatch& b, void* k_out, int64_t ldk, void* v_out, int64_t ldv, hipStream_t st) {
+  OAVSR_TRY(check_paged(kv, b, "paged_read"));
+  const int vec = kv.dtype == DT_F32 ? 4 : 8;
+  const int64_t width = (int64_t)kv.n_kv_heads * kv.head_dim;
+  OAVSR_REQUIRE((!k_out || (ldk >= width && ldk % vec == 0)) && (!v_out || (ldv >= width && ldv % vec == 0)), "paged_read: row strides %lld / %lld", (long long)ldk, (long long)ldv);
+  OAVSR_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, "paged_read: pointers must be 16-byte aligned");
+  if (b.rows == 0 || b.n_seqs == 0 || (!k_out && !v_out)) return 0;
+  if (kv.format == KV_E4M3) return kv.dtype == DT_F32 ? launch_read_t<float, true>(kv, b, k_out, ldk, v_out, ldv, st) : launch_read_t<bf16_t, true>(kv, b, k_out, ldk, v_out, ldv, st);
+  return kv.dtype == DT_F32 ? launch_read_t<float, false>(kv, b, k_out, ldk, v_out, ldv, st) : launch_read_t<bf16_t, false>(kv, b, k_out, ldk, v_out, ldv, st);
+}
+
+}  // namespace oavsr

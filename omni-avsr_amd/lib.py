@@ -90,6 +90,41 @@ class DecodeAttnDesc(C.Structure):
     ]
 
 
+KV_SAME, KV_E4M3 = 0, 1
+PAGED_BAD_PAGE, PAGED_BAD_LENGTH = 1, 2
+
+
+class PagedKvDesc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("format", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int32),
+        ("K", C.c_void_p), ("V", C.c_void_p), ("page_stride", C.c_int64), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("scale_stride", C.c_int64),
+        ("status", C.c_void_p),
+    ]
+
+
+class PagedBatchDesc(C.Structure):
+    _fields_ = [
+        ("n_seqs", C.c_int32), ("rows", C.c_int32), ("max_q", C.c_int32), ("max_ctx", C.c_int32),
+        ("cu_q", C.c_void_p), ("ctx_len", C.c_void_p), ("table", C.c_void_p), ("ld_table", C.c_int64),
+    ]
+
+
+class QkRopeDesc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("rows", C.c_int32), ("n_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("qkv", C.c_void_p), ("ld", C.c_int64), ("q_out", C.c_void_p), ("ldq", C.c_int64), ("k_out", C.c_void_p), ("ldk", C.c_int64),
+        ("pos", C.c_void_p), ("inv_freq", C.c_void_p), ("rot_dim", C.c_int32), ("interleaved", C.c_int32), ("rot_scale", C.c_float),
+        ("q_gain", C.c_void_p), ("k_gain", C.c_void_p), ("eps", C.c_float),
+    ]
+
+
+class PagedAttnDesc(C.Structure):
+    _fields_ = [
+        ("n_heads", C.c_int32), ("scale", C.c_float), ("Q", C.c_void_p), ("ldq", C.c_int64), ("O", C.c_void_p), ("ldo", C.c_int64),
+        ("lse", C.c_void_p), ("split_keys", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+    ]
+
+
 # every symbol include/omni_avsr.h declares: (name, restype, argtypes)
 _P, _I, _L, _F = C.c_void_p, C.c_int32, C.c_int64, C.c_float
 SYMBOLS = {
@@ -133,6 +168,12 @@ SYMBOLS = {
     "oavsr_op_gemm_chain": (C.c_int, [C.POINTER(GemmDesc), C.c_int32, _P, _P]),
     "oavsr_op_attention": (C.c_int, [C.POINTER(AttnDesc), _P]),
     "oavsr_op_decode_attention": (C.c_int, [C.POINTER(DecodeAttnDesc), _P]),
+    "oavsr_paged_check_host": (C.c_int, [C.POINTER(PagedKvDesc), C.POINTER(PagedBatchDesc)]),
+    "oavsr_op_qk_norm_rope": (C.c_int, [C.POINTER(QkRopeDesc), _P]),
+    "oavsr_op_paged_append": (C.c_int, [C.POINTER(PagedKvDesc), C.POINTER(PagedBatchDesc), C.POINTER(QkRopeDesc), _P]),
+    "oavsr_op_paged_read": (C.c_int, [C.POINTER(PagedKvDesc), C.POINTER(PagedBatchDesc), _P, _L, _P, _L, _P]),
+    "oavsr_op_paged_attention": (C.c_int, [C.POINTER(PagedKvDesc), C.POINTER(PagedBatchDesc), C.POINTER(PagedAttnDesc), _P]),
+    "oavsr_paged_attention_workspace": (C.c_int64, [C.POINTER(PagedKvDesc), C.POINTER(PagedBatchDesc), C.POINTER(PagedAttnDesc)]),
     "oavsr_op_norm": (C.c_int, [_I, _I, _P, _L, _P, _L, _P, _P, _I, _I, _F, _P]),
     "oavsr_op_rms_prep": (C.c_int, [_I, _P, _L, _P, _L, _P, _P, _I, _I, _P]),
     "oavsr_op_stem_pool": (C.c_int, [_I, _P, _I, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P]),
