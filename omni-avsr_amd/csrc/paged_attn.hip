@@ -10,6 +10,7 @@
 // Keys behind a sequence's context are never fetched.  A tile that some of the workgroup's rows see only in part (an edge tile) is masked; P = 0 there
 // does not suffice, since 0 * NaN and 0 * infinity are NaN: where such a tile's values hold one (rare), its second product runs without those values, and
 // they are then added for the rows that see them.
+#include <algorithm>
 #include "paged.h"
 
 namespace oavsr {
@@ -105,6 +106,380 @@ __device__ __forceinline__ Chunk16 cache_chunk(const void* base, int64_t at) {
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i) e4m3_to_f32(w[i], x + 4 * i);
     return chunk_from_f32<T>(x);                     // exact: three bits of mantissa
+  }
+}
+
+// ---- pieces of the streaming kernels -----------------------------------------------------------------------------------------------------------
+typedef __attribute__((ext_vector_type(2))) int i32x2;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef const __attribute__((address_space(1))) void* global_ptr;
+
+// max over lanes l, l ^ 16, l ^ 32, l ^ 48 / l, l ^ 32 by exchanges of the register file (no LDS round trip).  The second operand is kept apart from the
+// first: the instruction swaps two registers.
+__device__ __forceinline__ float max_xor32(float x) {
+  float y = x;
+  asm volatile("" : "+v"(y));
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
+  return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+}
+__device__ __forceinline__ float max_xor16_32(float x) {
+  float y = x;
+  asm volatile("" : "+v"(y));
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
+  return max_xor32(fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1])));
+}
+
+// Where 16-byte piece c of row r lies in an image of rows of RB bytes: c ^ swizzle.  Rows that one LDS access reads together fall into different banks.
+template <int RB> __device__ __forceinline__ constexpr int swizzle(int row) {
+  return RB >= 256 ? (row & 7) << 1 : RB == 128 ? row & 7 : (row >> 2) & 3;
+}
+
+// A page's number by scalar load (the table is the kernel's to read only), checked.
+__device__ __forceinline__ int uniform_page(const PagedAttnKArgs& p, int seq, int key, int shift) {
+  const int* t = p.b.table + (int64_t)seq * p.b.ld_table + (key >> shift);
+  const int page = *reinterpret_cast<const __attribute__((address_space(4))) int*>((uintptr_t)t);
+  return (unsigned)page < (unsigned)p.kv.n_pages ? page : -1;
+}
+
+// what a key row that is no key (behind the context, or of a page that is none) is fetched from: 16 rows
+__device__ const Chunk16 kZeroRows[16 * 512 / 16] = {};
+
+__device__ __forceinline__ bf16x4 e4m3_to_bf16(unsigned w) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true);
+  return bf16x4{a[0], a[1], b[0], b[1]};                // exact
+}
+// Transposing reads of four 16-column blocks, waited for where they are made (the builtin makes the compiler wait for every LDS-DMA on its way first):
+// lane 4 q + p of 16 gives the address of columns 4 p .. of row q and gets rows 0 .. 3 of its own column.  b16: two row blocks, OFF bytes apart; b8: eight rows,
+// lane 2 q + h giving bytes 8 h .. of row q.
+template <int OFF>
+__device__ __forceinline__ void read_tr16_x4(const unsigned (&at)[4], u32x4 (&out)[4]) {
+  i32x2 a[4], b[4];
+  asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\tds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+               "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\tds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1]), "=&v"(a[2]), "=&v"(b[2]), "=&v"(a[3]), "=&v"(b[3])
+               : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(OFF)
+               : "memory");
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = u32x4{(unsigned)a[i][0], (unsigned)a[i][1], (unsigned)b[i][0], (unsigned)b[i][1]};
+}
+__device__ __forceinline__ void read_tr8_x4(const unsigned (&at)[4], i32x2 (&out)[4]) {
+  asm volatile("ds_read_b64_tr_b8 %0, %4\n\tds_read_b64_tr_b8 %1, %5\n\tds_read_b64_tr_b8 %2, %6\n\tds_read_b64_tr_b8 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(out[0]), "=&v"(out[1]), "=&v"(out[2]), "=&v"(out[3])
+               : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3])
+               : "memory");
+}
+__device__ __forceinline__ unsigned lds_address(const void* p) { return (unsigned)(uintptr_t)(lds_ptr)(void*)p; }
+
+__device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) { return bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}; }
+
+// ---- few rows per sequence: single tokens ------------------------------------------------------------------------------------------------------
+//
+// A workgroup per (sequence, kv head, split of its keys) whose packed rows are the <= 16 columns of the matrix instructions.  HBM bound: 2 G flop per byte
+// of a bf16 cache.  Each wave streams its own tiles of KT keys (wave, wave + NW, ...) through a private ring of NS tiles in LDS, fetched by LDS-DMA and
+// awaited by counted vmcnt, so there is no barrier in the loop and (NS - 1) tiles are on their way while one is computed.  16 keys lie in one page, so
+// an instruction's page is uniform: scalar loads, one page base per 16 keys.  The waves' (m, l, O) meet in LDS in wave order.
+template <typename T, bool F8, int HD> struct DecodeShape {
+  static constexpr int KT = sizeof(T) == 4 ? 16 : 32;                        // keys per wave tile
+  static constexpr int RB = HD * (F8 ? 1 : (int)sizeof(T));                  // bytes of a cached row
+  static constexpr int IMG = KT * RB, STAGE = 2 * IMG + (F8 ? 256 : 0);      // K image, V image, scales
+};
+
+template <typename T, bool F8, int HD, int NW, int NS>
+__global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAttnKArgs p) {
+  using Sh = DecodeShape<T, F8, HD>;
+  constexpr int KT = Sh::KT, RB = Sh::RB, IMG = Sh::IMG, STAGE = Sh::STAGE, NCH = RB / 16;
+  constexpr int RPI = 1024 / RB, NI = IMG / 1024;      // rows per DMA instruction, instructions per image
+  constexpr int NSUB = KT / 16, NDT = HD / 16, NOFF = RPI >= 8 ? 1 : 8 / RPI;
+  constexpr int VM = 2 * NI + (F8 ? 1 : 0);
+  constexpr int RING = STAGE * NS > HD * 64 + 128 ? STAGE * NS : HD * 64 + 128;      // the ring, afterwards (m, l, O) of the wave
+  static_assert(VM * (NS - 1) <= 63, "vmcnt");
+  __shared__ __attribute__((aligned(1024))) char smem[NW * RING];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), qi = lane & 15, g = lane >> 4;
+  const int seq = blockIdx.x, kvh = blockIdx.y, G = p.group;
+  const SeqInfo sq = paged_seq(p.b, seq);
+  if (sq.bad && tid == 0) paged_report(p.kv.status, kBadLength);
+  const int packed = sq.nq * G;
+  if (packed == 0) return;
+  const int first_pos = sq.ctx - sq.nq, kmax = min(sq.ctx, p.b.max_ctx);
+  const int kend_all = max(0, min(first_pos + sq.nq, kmax));
+  const int kbeg = p.split ? (int)blockIdx.z * p.split : 0;
+  if (blockIdx.z > 0 && kbeg >= kend_all) return;
+  const int kend = p.split ? min(kend_all, kbeg + p.split) : kend_all;
+  char* ring = smem + wave * RING;
+
+  // ---- the ring
+  const int shift = page_shift_of(p.kv);
+  int loff[NOFF];                                      // byte offset of this lane's piece inside the rows of an instruction
+#pragma unroll
+  for (int j = 0; j < NOFF; ++j) {
+    const int r = j * RPI + lane / NCH;
+    loff[j] = (lane / NCH) * RB + (((lane % NCH) ^ swizzle<RB>(r)) << 4);
+  }
+  const char* Kb = reinterpret_cast<const char*>(p.kv.K);
+  const char* Vb = reinterpret_cast<const char*>(p.kv.V);
+  const int64_t page_bytes = p.kv.page_stride * (F8 ? 1 : (int64_t)sizeof(T));
+  bool bad_page = false;
+  auto issue = [&](int kt0, int slot) __attribute__((always_inline)) {
+    char* dst = ring + slot * STAGE;
+    int page[NSUB];
+#pragma unroll
+    for (int j = 0; j < NSUB; ++j) {
+      const int key = kt0 + 16 * j;
+      page[j] = -1;
+      if (key < kend) { page[j] = uniform_page(p, seq, key, shift); bad_page |= page[j] < 0; }
+    }
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int j = i * RPI / 16, key = kt0 + 16 * j;
+      const int64_t at = (int64_t)page[j] * page_bytes + ((int64_t)kvh * p.kv.page_size + (key & (p.kv.page_size - 1)) + (i * RPI) % 16) * RB;
+      const char* k = page[j] < 0 ? reinterpret_cast<const char*>(kZeroRows) : Kb + at;
+      const char* v = page[j] < 0 ? reinterpret_cast<const char*>(kZeroRows) : Vb + at;
+      __builtin_amdgcn_global_load_lds((global_ptr)(k + loff[i % NOFF]), (lds_ptr)(dst + i * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((global_ptr)(v + loff[i % NOFF]), (lds_ptr)(dst + IMG + i * 1024), 16, 0, 0);
+    }
+    if constexpr (F8) {                                // lanes 0 .. KT - 1: the keys' scales, then the values'
+      const int l = lane & (2 * KT - 1), key = kt0 + (l & (KT - 1));
+      const int pg = NSUB == 1 || (l & 16) == 0 ? page[0] : page[NSUB - 1];
+      const float* base = l < KT ? p.kv.k_scale : p.kv.v_scale;
+      const float* src = pg < 0 ? reinterpret_cast<const float*>(kZeroRows)
+                                : base + (int64_t)pg * p.kv.scale_stride + (int64_t)kvh * p.kv.page_size + (key & (p.kv.page_size - 1));
+      __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(dst + 2 * IMG), 4, 0, 0);
+    }
+  };
+  const int first = kbeg + wave * KT, step = NW * KT;
+  const int ntile = first < kend ? (kend - first + step - 1) / step : 0;
+
+  // ---- queries: lane = packed row qi, in the element order of the K fragments
+  const int r = min(qi, packed - 1), tok = r / G, head = kvh * G + (r - tok * G);
+  const int64_t row = sq.q0 + tok;
+  const int see = min(first_pos + tok + 1, kmax), see_min = min(first_pos + 1, kmax);
+  const T* qp = reinterpret_cast<const T*>(p.Q) + row * p.ldq + (int64_t)head * HD;
+  constexpr int NQ = F8 ? HD / 64 : RB / 64;           // 16-byte pieces of a cached row per lane
+  constexpr int QE = F8 ? 16 : 16 / (int)sizeof(T);    // elements of a piece
+  constexpr int QC = QE * (int)sizeof(T) / 16;
+  Chunk16 qf[NQ][QC];
+#pragma unroll
+  for (int b = 0; b < NQ; ++b)
+#pragma unroll
+    for (int e = 0; e < QC; ++e) qf[b][e] = reinterpret_cast<const Chunk16*>(qp + (b * 4 + g) * QE)[e];
+#pragma unroll
+  for (int i = 0; i < NS; ++i)
+    if (i < ntile) issue(first + i * step, i);
+  // (waited for here, once: inside the loop the wait for them would be one for the ring too)
+#pragma unroll
+  for (int b = 0; b < NQ; ++b)
+#pragma unroll
+    for (int e = 0; e < QC; ++e) asm volatile("" : "+v"(qf[b][e].v));
+
+  f32x4 o[NDT];
+#pragma unroll
+  for (int i = 0; i < NDT; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m_run = -INFINITY, l_run = 0.f;
+
+  for (int t = 0; t < ntile; ++t) {
+    const int kt0 = first + t * step;
+    if (ntile - t >= NS) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(VM * (NS - 1)) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    char* sK = ring + (NS == 1 ? 0 : t % NS) * STAGE;
+    char* sV = sK + IMG;
+    const float* sc = reinterpret_cast<const float*>(sK + 2 * IMG);
+    if (kt0 + KT > kend) {                             // rows behind the context: whatever the page holds there must not meet a zero
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        if (kt0 + i * RPI + lane / NCH >= kend) reinterpret_cast<Chunk16*>(sV + i * 1024)[lane].v = u32x4{0u, 0u, 0u, 0u};
+    }
+    const bool edge = kt0 + KT > see_min;              // some row does not see the whole tile
+
+    f32x4 s[NSUB];
+    float mt = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < NSUB; ++kt) {
+      s[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const int krow = kt * 16 + qi;
+#pragma unroll
+      for (int b = 0; b < NQ; ++b) {
+        const Chunk16 kc = *reinterpret_cast<const Chunk16*>(sK + krow * RB + (((b * 4 + g) ^ swizzle<RB>(krow)) << 4));
+        if constexpr (!F8) Mma16<T>::run(kc, qf[b][0], s[kt]);
+        else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf)
+            s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join(e4m3_to_bf16(kc.v[2 * hf]), e4m3_to_bf16(kc.v[2 * hf + 1])), __builtin_bit_cast(bf16x8, qf[b][hf].v), s[kt], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            float x[4];
+            e4m3_to_f32(kc.v[w], x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], __builtin_bit_cast(f32x4, qf[b][w].v)[e], s[kt], 0, 0, 0);
+          }
+        }
+      }
+      f32x4 ks = f32x4{p.scale2, p.scale2, p.scale2, p.scale2};
+      if constexpr (F8) ks *= *reinterpret_cast<const f32x4*>(sc + kt * 16 + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float v = s[kt][i] * ks[i];
+        if (edge && kt0 + kt * 16 + 4 * g + i >= see) v = -INFINITY;
+        s[kt][i] = v;
+        mt = fmaxf(mt, v);
+      }
+    }
+    mt = max_xor16_32(mt);
+    const float m_new = fmaxf(m_run, mt), m_use = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+    float sum = 0.f;
+#pragma unroll
+    for (int kt = 0; kt < NSUB; ++kt) {
+      f32x4 vs = f32x4{1.f, 1.f, 1.f, 1.f};
+      if constexpr (F8) vs = *reinterpret_cast<const f32x4*>(sc + KT + kt * 16 + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float e = __builtin_amdgcn_exp2f(s[kt][i] - m_use);
+        sum += e;
+        if constexpr (F8) e *= vs[i];
+        if (edge && kt0 + kt * 16 + 4 * g + i >= see) e = 0.f;
+        s[kt][i] = e;
+      }
+    }
+    l_run = l_run * alpha + sum;
+    m_run = m_new;
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0ull) {
+#pragma unroll
+      for (int i = 0; i < NDT; ++i) o[i] *= alpha;
+    }
+
+    // infinities and NaN among the values of an edge tile (of several new tokens: a later one's)
+    bool odd = false;
+    auto v_at = [&](int krow, int d) -> float {
+      const int byte = d * (F8 ? 1 : (int)sizeof(T));
+      const char* at = sV + krow * RB + (((byte >> 4) ^ swizzle<RB>(krow)) << 4) + (byte & 15);
+      if constexpr (F8) { float x[4]; e4m3_to_f32(*reinterpret_cast<const unsigned char*>(at), x); return x[0]; }
+      else return to_f32(*reinterpret_cast<const T*>(at));
+    };
+    if (edge) {
+      bool ok = true;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const Chunk16 c = reinterpret_cast<const Chunk16*>(sV + i * 1024)[lane];
+        if constexpr (F8) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) ok = ok && (((c.v[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) == 0;
+        } else ok = ok && chunk_finite(c, T());
+      }
+      odd = __builtin_amdgcn_ballot_w64(!ok) != 0ull;
+    }
+
+    if constexpr (sizeof(T) == 2) {
+      bf16x8 pf;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { pf[i] = (bf16_t)s[0][i]; pf[4 + i] = (bf16_t)s[1][i]; }
+      const unsigned vb = lds_address(sV);
+#pragma unroll
+      for (int d4 = 0; d4 < NDT; d4 += 4) {
+        unsigned at[4];
+        bf16x8 vf[4];
+        if constexpr (F8) {
+          const int rr = qi >> 1, krow = rr < 4 ? 4 * g + rr : 12 + 4 * g + rr;
+          i32x2 w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) at[j] = vb + krow * RB + (((d4 + j) ^ swizzle<RB>(krow)) << 4) + (qi & 1) * 8;
+          read_tr8_x4(at, w);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) vf[j] = join(e4m3_to_bf16((unsigned)w[j][0]), e4m3_to_bf16((unsigned)w[j][1]));
+        } else {
+          const int qq = qi >> 2, pp = qi & 3, krow = 4 * g + qq;
+          u32x4 w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) at[j] = vb + krow * RB + ((((d4 + j) * 2 + (pp >> 1)) ^ swizzle<RB>(krow)) << 4) + (pp & 1) * 8;
+          read_tr16_x4<16 * RB>(at, w);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) vf[j] = __builtin_bit_cast(bf16x8, w[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (odd) vf[j] = finite_part(vf[j]);
+          o[d4 + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[j], pf, o[d4 + j], 0, 0, 0);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float vv = v_at(4 * g + i, dt * 16 + qi);
+          if (odd && !is_finite(vv)) vv = 0.f;
+          o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv, s[0][i], o[dt], 0, 0, 0);
+        }
+    }
+    if (odd) {
+      for (int k = 0; k < KT; ++k) {
+        float e = 0.f;
+#pragma unroll
+        for (int kt = 0; kt < NSUB; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if ((k & 3) == i && (k >> 4) == kt) e = s[kt][i];
+        e = __shfl(e, ((k >> 2) & 3) * 16 + qi, 64);
+        if (kt0 + k < see)
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const float vv = v_at(k, dt * 16 + 4 * g + q);
+              if (!is_finite(vv)) o[dt][q] += e * vv;
+            }
+      }
+    }
+    if (t + NS < ntile) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // this tile has been read
+      issue(kt0 + NS * step, NS == 1 ? 0 : t % NS);
+    }
+  }
+  if (bad_page && lane == 0) paged_report(p.kv.status, kBadPage);
+
+  l_run += __shfl_xor(l_run, 16, 64);
+  l_run += __shfl_xor(l_run, 32, 64);
+  // ---- the waves' partial results, joined in wave order
+  float* so = reinterpret_cast<float*>(ring);          // [HD][16] O^T, then [16] m, [16] l
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) so[(dt * 16 + 4 * g + i) * 16 + qi] = o[dt][i];
+  if (g == 0) { so[HD * 16 + qi] = m_run; so[HD * 16 + 16 + qi] = l_run; }
+  __syncthreads();
+  for (int i = tid; i < packed * (HD / 4); i += NW * 64) {
+    const int pr = i / (HD / 4), d0 = (i - pr * (HD / 4)) * 4, ptok = pr / G, phead = kvh * G + (pr - ptok * G);
+    float m = -INFINITY, l = 0.f;
+    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float* x = reinterpret_cast<const float*>(smem + w * RING);
+      m = fmaxf(m, x[HD * 16 + pr]);
+    }
+    const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float* x = reinterpret_cast<const float*>(smem + w * RING);
+      const float f = __builtin_amdgcn_exp2f(x[HD * 16 + pr] - mu);
+      l = fmaf(f, x[HD * 16 + 16 + pr], l);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] = fmaf(f, x[(d0 + j) * 16 + pr], acc[j]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t prow = sq.q0 + ptok;
+    if (p.split) {
+      const int64_t at = ((int64_t)blockIdx.z * p.b.rows + prow) * p.n_heads + phead;
+      if (d0 == 0) p.part_ml[at] = make_float2(m, l);
+      *reinterpret_cast<f32x4*>(p.part + at * HD + d0) = acc * inv;
+    } else {
+      if (p.lse && d0 == 0) p.lse[prow * p.n_heads + phead] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+      T* O = reinterpret_cast<T*>(p.O) + prow * p.ldo + (int64_t)phead * HD + d0;
+      if constexpr (sizeof(T) == 2) *reinterpret_cast<bf16x4*>(O) = bf16x4{(bf16_t)(acc[0] * inv), (bf16_t)(acc[1] * inv), (bf16_t)(acc[2] * inv), (bf16_t)(acc[3] * inv)};
+      else *reinterpret_cast<f32x4*>(O) = acc * inv;
+    }
   }
 }
 
@@ -301,37 +676,57 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(const PagedAttnKAr
   }
 }
 
-// Joins the splits of a row's keys: a wave per (row, head), the splits in order.  out = sum_z w_z O_z / sum_z w_z,  w_z = l_z 2^(m_z - max m).
+// Joins the splits of a row's keys: a workgroup per (row, head).  out = sum_z w_z O_z / sum_z w_z,  w_z = l_z 2^(m_z - max m).  Its threads are groups of
+// HD / 4 that take every NG-th split, joined in LDS in a fixed order: the time is one or two loads' latency, not the number of splits.
 template <typename T, int HD>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnKArgs p) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t i = (int64_t)blockIdx.x * 4 + wave;
-  if (i >= (int64_t)p.b.rows * p.n_heads) return;
+  constexpr int TPG = HD / 4, NG = kThreads / TPG;
+  __shared__ __attribute__((aligned(16))) float acc_s[NG][HD];
+  __shared__ float m_s[NG], l_s[NG];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int64_t i = blockIdx.x;
   const int row = (int)(i / p.n_heads), head = (int)(i - (int64_t)row * p.n_heads);
   const int seq = wave_find_seq(p.b.cu_q, p.b.n_seqs, row, lane);
   const SeqInfo sq = paged_seq(p.b, seq);
   if (row < sq.q0 || row >= sq.q0 + sq.nq) return;
   const int see = min(sq.ctx - sq.nq + (row - sq.q0) + 1, min(sq.ctx, p.b.max_ctx));
   const int n = see > 0 ? (see - 1) / p.split + 1 : 0;
-  constexpr int E = HD / 64;
-  float acc[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int z = 0; z < n; ++z) {
+  const int grp = tid / TPG, d0 = (tid - grp * TPG) * 4;
+  float m = -INFINITY, l = 0.f;
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int z = grp; z < n; z += NG) {
     const int64_t at = ((int64_t)z * p.b.rows + row) * p.n_heads + head;
     const float2 ml = p.part_ml[at];
+    const f32x4 x = *reinterpret_cast<const f32x4*>(p.part + at * HD + d0);
     const float mn = fmaxf(m, ml.x), mu = mn == -INFINITY ? 0.f : mn;
-    const float w0 = exp2f(m - mu), w1 = exp2f(ml.x - mu) * ml.y;
+    const float w0 = __builtin_amdgcn_exp2f(m - mu), w1 = __builtin_amdgcn_exp2f(ml.x - mu) * ml.y;
     l = l * w0 + w1;
     m = mn;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = acc[e] * w0 + w1 * p.part[at * HD + lane * E + e];
+    for (int e = 0; e < 4; ++e) acc[e] = acc[e] * w0 + w1 * x[e];
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (p.lse && lane == 0) p.lse[i] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
-  T* O = reinterpret_cast<T*>(p.O) + row * p.ldo + (int64_t)head * HD;
+  if (d0 == 0) { m_s[grp] = m; l_s[grp] = l; }
+  *reinterpret_cast<f32x4*>(&acc_s[grp][d0]) = acc;
+  __syncthreads();
+  if (grp > 0) return;
+  float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) O[lane * E + e] = from_f32<T>(acc[e] * inv);
+  for (int j = 0; j < NG; ++j) mm = fmaxf(mm, m_s[j]);
+  const float mu = mm == -INFINITY ? 0.f : mm;
+  acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < NG; ++j) {
+    const float w = __builtin_amdgcn_exp2f(m_s[j] - mu);
+    ll = fmaf(w, l_s[j], ll);
+    const f32x4 x = *reinterpret_cast<const f32x4*>(&acc_s[j][d0]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, x[e], acc[e]);
+  }
+  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  if (p.lse && d0 == 0) p.lse[i] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994530942f;
+  T* O = reinterpret_cast<T*>(p.O) + row * p.ldo + (int64_t)head * HD + d0;
+  if constexpr (sizeof(T) == 2) *reinterpret_cast<bf16x4*>(O) = bf16x4{(bf16_t)(acc[0] * inv), (bf16_t)(acc[1] * inv), (bf16_t)(acc[2] * inv), (bf16_t)(acc[3] * inv)};
+  else *reinterpret_cast<f32x4*>(O) = acc * inv;
 }
 
 int cu_count() {
@@ -339,23 +734,28 @@ int cu_count() {
   return n;
 }
 
-// How a call is laid out: tiles of packed rows, keys per workgroup.
-struct Plan { int64_t tiles; int split, splits, tile_is_seq; };
+// How a call is laid out.
+struct Plan { int64_t tiles; int split, splits, tile_is_seq; bool decode, narrow; };
 Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
   Plan pl;
   const int G = a.n_heads / kv.n_kv_heads;
+  pl.decode = (int64_t)b.max_q * G <= 16;
   pl.tile_is_seq = (int64_t)b.max_q * G <= 64;
   pl.tiles = pl.tile_is_seq ? b.n_seqs : (int64_t)b.rows * G / 64 + b.n_seqs;
   pl.split = a.split_keys;
+  const int64_t wgs = pl.tiles * kv.n_kv_heads;
+  pl.narrow = false;
   if (!pl.split) {
-    const int64_t wgs = pl.tiles * kv.n_kv_heads, want = 4 * cu_count();
-    int64_t n = want / (wgs > 0 ? wgs : 1);
-    int64_t k = n > 1 ? ceil_div64(b.max_ctx, n) : b.max_ctx;
-    k = (k + 255) / 256 * 256;
-    pl.split = (int)(k < 256 ? 256 : k);
+    if (pl.decode && wgs <= cu_count() && b.max_ctx <= 1024) pl.split = 1024;
+    else {
+      const int64_t want = 4 * cu_count(), n = want / (wgs > 0 ? wgs : 1);
+      const int64_t k = n > 1 ? ceil_div64(b.max_ctx, n) : b.max_ctx;
+      pl.split = (int)std::max<int64_t>(256, (k + 255) / 256 * 256);
+    }
   }
   pl.splits = b.max_ctx > 0 ? ceil_div(b.max_ctx, pl.split) : 1;
   if (pl.splits <= 1) pl.split = 0, pl.splits = 1;
+  pl.narrow = wgs * pl.splits > cu_count();      // more workgroups than CUs: two waves each, several side by side; else eight for one
   return pl;
 }
 uint64_t workspace_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a, const Plan& pl) {
@@ -373,10 +773,15 @@ int check_attn(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
 
 template <typename T, bool F8, int HD>
 int launch_t(const PagedAttnKArgs& k, const Plan& pl, hipStream_t st) {
-  hipLaunchKernelGGL((paged_attn_kernel<T, F8, HD>), dim3((unsigned)pl.tiles, k.kv.n_kv_heads, pl.splits), dim3(kThreads), 0, st, k);
+  const dim3 grid((unsigned)pl.tiles, k.kv.n_kv_heads, pl.splits);
+  if (pl.decode) {
+    constexpr int STAGE = DecodeShape<T, F8, HD>::STAGE, NS = 33 * 1024 / STAGE > 4 ? 4 : 33 * 1024 / STAGE, NS8 = 17 * 1024 / STAGE > 2 ? 2 : 17 * 1024 / STAGE;
+    if (pl.narrow) hipLaunchKernelGGL((paged_decode_kernel<T, F8, HD, 2, NS>), grid, dim3(128), 0, st, k);
+    else hipLaunchKernelGGL((paged_decode_kernel<T, F8, HD, 8, NS8>), grid, dim3(512), 0, st, k);
+  } else hipLaunchKernelGGL((paged_attn_kernel<T, F8, HD>), grid, dim3(kThreads), 0, st, k);
   OAVSR_CHECK_HIP(hipGetLastError());
   if (pl.split) {
-    hipLaunchKernelGGL((paged_merge_kernel<T, HD>), dim3((unsigned)ceil_div64((int64_t)k.b.rows * k.n_heads, 4)), dim3(kThreads), 0, st, k);
+    hipLaunchKernelGGL((paged_merge_kernel<T, HD>), dim3((unsigned)((int64_t)k.b.rows * k.n_heads)), dim3(kThreads), 0, st, k);
     OAVSR_CHECK_HIP(hipGetLastError());
   }
   return 0;
