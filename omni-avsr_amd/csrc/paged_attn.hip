@@ -26,7 +26,7 @@ struct PagedAttnKArgs {
   void* O; int64_t ldo;
   float* lse;
   float scale2;                                      // scale * log2 e
-  int n_heads, group, split, tile_is_seq;            // split: keys per workgroup (0: all); tile_is_seq: every sequence fits one tile
+  int n_heads, group, split, tile_is_seq, tiles;     // split: keys per workgroup (0: all); tile_is_seq: every sequence fits one tile; tiles: of all sequences (bound)
   float* part;                                       // split: [splits][rows][n_heads][head_dim] O / l, then [splits][rows][n_heads] (m, l)
   float2* part_ml;
 };
@@ -163,6 +163,17 @@ __device__ __forceinline__ void read_tr16_x4(const unsigned (&at)[4], u32x4 (&ou
                : "memory");
 #pragma unroll
   for (int i = 0; i < 4; ++i) out[i] = u32x4{(unsigned)a[i][0], (unsigned)a[i][1], (unsigned)b[i][0], (unsigned)b[i][1]};
+}
+template <int OFF>
+__device__ __forceinline__ void read_tr16_x2(const unsigned (&at)[2], u32x4 (&out)[2]) {
+  i32x2 a[2], b[2];
+  asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\tds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1])
+               : "v"(at[0]), "v"(at[1]), "n"(OFF)
+               : "memory");
+#pragma unroll
+  for (int i = 0; i < 2; ++i) out[i] = u32x4{(unsigned)a[i][0], (unsigned)a[i][1], (unsigned)b[i][0], (unsigned)b[i][1]};
 }
 __device__ __forceinline__ void read_tr8_x4(const unsigned (&at)[4], i32x2 (&out)[4]) {
   asm volatile("ds_read_b64_tr_b8 %0, %4\n\tds_read_b64_tr_b8 %1, %5\n\tds_read_b64_tr_b8 %2, %6\n\tds_read_b64_tr_b8 %3, %7\n\ts_waitcnt lgkmcnt(0)"
@@ -483,6 +494,321 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
   }
 }
 
+// ---- many rows per sequence: chunks and whole prompts, bf16 ------------------------------------------------------------------------------------
+//
+// A workgroup of 8 waves takes 256 packed rows of a (sequence, kv head), 32 per wave, on 32x32x16 matrix instructions; tiles of 64 keys are shared by the
+// waves.  Bound by the matrix pipe and the vector issue of the softmax together (per tile and wave at head_dim 128: 32 products of 32 cycles, about 200 vector
+// instructions of 4).  A bf16 cache goes to a ring of three tiles in LDS by LDS-DMA, two tiles ahead, one barrier per tile; an 8-bit one through
+// registers, each thread widening its 16 bytes once per tile for all waves, into a ring of two.  The kv head is the fastest part of a workgroup's number:
+// workgroups of one kv head then share an XCD (8 of them take the numbers in turn), and its L2 serves their common keys.
+// A wave skips the tiles none of its rows sees, and masks only those that some row sees in part.
+template <bool F8, int HD>
+__global__ __launch_bounds__(512, 2) void paged_chunk_kernel(const PagedAttnKArgs p) {
+  constexpr int NW = 8, ROWS = NW * 32, RB = HD * 2, IMG = KT * RB, NSTAGE = F8 ? 2 : 3, STAGE = 2 * IMG + (F8 ? 2 * KT * 4 : 0);
+  constexpr int NCH = RB / 16, RPI = 1024 / RB, NSEG = IMG / 1024 / NW, NDS = HD / 16, NDT = HD / 32, VM = 2 * NSEG;
+  constexpr int FB = HD / 8;                           // 8 bits: bytes per thread, image and tile
+  __shared__ __attribute__((aligned(1024))) char smem[NSTAGE * STAGE];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ql = lane & 31, h = lane >> 5;
+  const int G = p.group, KV = p.kv.n_kv_heads;
+  const int kvh = blockIdx.x % KV, unit = blockIdx.x / KV, split = unit / p.tiles;
+  const TileAt at = wave_find_tile<ROWS>(p.b, G, unit - split * p.tiles, lane);
+  if (at.seq < 0) return;
+  const int seq = __builtin_amdgcn_readfirstlane(at.seq), r0 = __builtin_amdgcn_readfirstlane(at.r0);
+  const SeqInfo sq = paged_seq(p.b, seq);
+  if (sq.bad && tid == 0) paged_report(p.kv.status, kBadLength);
+  const int packed = sq.nq * G;
+  const int first_pos = sq.ctx - sq.nq, kmax = min(sq.ctx, p.b.max_ctx);
+  const int kend_all = max(0, min(first_pos + (min(r0 + ROWS, packed) - 1) / G + 1, kmax));
+  const int kbeg = p.split ? split * p.split : 0;
+  if (split > 0 && kbeg >= kend_all) return;
+  const int kend = p.split ? min(kend_all, kbeg + p.split) : kend_all;
+  const int ntile = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
+
+  // ---- this wave's rows
+  const int w0 = r0 + wave * 32;                       // first packed row
+  const bool rows_here = w0 < packed;
+  const int r = w0 + ql, rc = min(r, packed - 1), tok = rc / G, head = kvh * G + (rc - tok * G);
+  const int64_t row = sq.q0 + tok;
+  const int see = min(first_pos + tok + 1, kmax);
+  const int see_min = min(first_pos + min(w0, packed - 1) / G + 1, kmax), see_max = rows_here ? min(first_pos + min(w0 + 31, packed - 1) / G + 1, kmax) : 0;
+
+  // ---- tiles
+  const int shift = page_shift_of(p.kv), pmask = p.kv.page_size - 1;
+  const char* Kb = reinterpret_cast<const char*>(p.kv.K);
+  const char* Vb = reinterpret_cast<const char*>(p.kv.V);
+  const int64_t page_bytes = p.kv.page_stride * (F8 ? 1 : 2);
+  bool bad_page = false;
+  int page[NSEG];                                      // of the next tile to fetch
+  auto next_pages = [&](int kt0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NSEG; ++j) {
+      const int key = kt0 + (F8 ? wave * 8 : (wave + NW * j) * RPI);
+      page[j] = -1;
+      if (key < kend) { page[j] = uniform_page(p, seq, key, shift); bad_page |= page[j] < 0; }
+    }
+  };
+  const char* zero = reinterpret_cast<const char*>(kZeroRows);
+  // bf16: instruction (wave + 8 j) fills 1 KiB = RPI rows of an image
+  auto issue = [&](int kt0, int slot) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NSEG; ++j) {
+      const int key = kt0 + (wave + NW * j) * RPI, lrow = (wave + NW * j) * RPI + lane / NCH;
+      const int off = (lane / NCH) * RB + (((lane % NCH) ^ swizzle<RB>(lrow)) << 4);
+      const int64_t at = (int64_t)page[j] * page_bytes + ((int64_t)kvh * p.kv.page_size + (key & pmask)) * RB;
+      const char *k = page[j] < 0 ? zero : Kb + at, *v = page[j] < 0 ? zero : Vb + at;
+      char* dst = smem + slot * STAGE + (wave + NW * j) * 1024;
+      if (kt0 + KT > kend && kt0 + lrow >= kend) { k = zero; v = zero; }      // behind the context: whatever the page holds must not meet a zero
+      __builtin_amdgcn_global_load_lds((global_ptr)(k + off), (lds_ptr)dst, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((global_ptr)(v + off), (lds_ptr)(dst + IMG), 16, 0, 0);
+    }
+  };
+  // 8 bits: thread = FB bytes of row tid / 8 of both images; lanes 0 .. 15 of a wave the scales of its 8 rows
+  struct Raw { unsigned k[FB / 4], v[FB / 4]; float scale; };
+  auto fetch = [&](int kt0, Raw& x) __attribute__((always_inline)) {
+    const int key = kt0 + wave * 8 + (lane >> 3);
+    const bool ok = page[0] >= 0 && key < kend;
+    const int64_t tok_at = (int64_t)kvh * p.kv.page_size + (key & pmask);
+    const int64_t at = (int64_t)page[0] * page_bytes + tok_at * HD + (lane & 7) * FB;
+    const char *k = ok ? Kb + at : zero, *v = ok ? Vb + at : zero;
+    __builtin_memcpy(x.k, __builtin_assume_aligned(k, FB), FB);
+    __builtin_memcpy(x.v, __builtin_assume_aligned(v, FB), FB);
+    const int skey = kt0 + wave * 8 + (lane & 7);
+    const int64_t sat = (int64_t)page[0] * p.kv.scale_stride + (int64_t)kvh * p.kv.page_size + (skey & pmask);
+    const float* sp = page[0] >= 0 && skey < kend ? ((lane & 8) ? p.kv.v_scale : p.kv.k_scale) + sat : reinterpret_cast<const float*>(zero);
+    x.scale = *sp;
+  };
+  auto widen = [&](const Raw& x, int slot) __attribute__((always_inline)) {
+    char* dst = smem + slot * STAGE;
+    const int lrow = wave * 8 + (lane >> 3);
+#pragma unroll
+    for (int c = 0; c < FB / 8; ++c) {
+      const int at = lrow * RB + ((((lane & 7) * (FB / 8) + c) ^ swizzle<RB>(lrow)) << 4);
+      *reinterpret_cast<bf16x8*>(dst + at) = join(e4m3_to_bf16(x.k[2 * c]), e4m3_to_bf16(x.k[2 * c + 1]));
+      *reinterpret_cast<bf16x8*>(dst + IMG + at) = join(e4m3_to_bf16(x.v[2 * c]), e4m3_to_bf16(x.v[2 * c + 1]));
+    }
+    if (lane < 16) reinterpret_cast<float*>(dst + 2 * IMG)[(lane & 8) * 8 + wave * 8 + (lane & 7)] = (lane & 8) ? x.scale : x.scale * p.scale2;
+  };
+
+  // Q^T fragments (B operand: lane = row ql, k-group h): step ds covers d = 16 ds + 8 h .. + 7
+  Chunk16 qf[NDS];
+  {
+    const char* qp = reinterpret_cast<const char*>(reinterpret_cast<const bf16_t*>(p.Q) + row * p.ldq + (int64_t)head * HD);
+#pragma unroll
+    for (int ds = 0; ds < NDS; ++ds) qf[ds] = *reinterpret_cast<const Chunk16*>(qp + ds * 32 + h * 16);
+  }
+  Raw raw;
+  next_pages(kbeg);
+  if constexpr (F8) {
+    if (ntile > 0) { fetch(kbeg, raw); next_pages(kbeg + KT); widen(raw, 0); }
+    if (ntile > 1) { fetch(kbeg + KT, raw); next_pages(kbeg + 2 * KT); }
+  } else {
+    if (ntile > 0) { issue(kbeg, 0); next_pages(kbeg + KT); }
+    if (ntile > 1) { issue(kbeg + KT, 1); next_pages(kbeg + 2 * KT); }
+  }
+#pragma unroll
+  for (int ds = 0; ds < NDS; ++ds) asm volatile("" : "+v"(qf[ds].v));      // waited for here, not in the loop
+
+  // LDS offsets inside a stage.  K (A operand): row ql (+ 32), piece 2 ds + h.  V^T (transposing reads: 16 lanes fetch 4 rows x 16 columns): row 4 h + qq
+  // (+ 16 per step, + 8), piece 4 dt + 2 d16 + (pp >> 1); the row offsets are multiples of 8, which the swizzle does not see.
+  unsigned kbase[NDS], vbase[NDT];
+  {
+    const unsigned s0 = lds_address(smem);
+    const int qi = lane & 15, d16 = (lane >> 4) & 1, qq = qi >> 2, pp = qi & 3, vrow = 4 * h + qq;
+#pragma unroll
+    for (int ds = 0; ds < NDS; ++ds) kbase[ds] = ql * RB + (((ds * 2 + h) ^ swizzle<RB>(ql)) << 4);
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) vbase[dt] = s0 + IMG + vrow * RB + (((dt * 4 + d16 * 2 + (pp >> 1)) ^ swizzle<RB>(vrow)) << 4) + (pp & 1) * 8;
+  }
+
+  f32x16 o[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;
+
+  auto compute = [&](int kt0, unsigned so, auto masked_tag) __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(masked_tag)::value;
+    const float* sc = reinterpret_cast<const float*>(smem + so + 2 * IMG);
+    f32x16 s[2];
+#pragma unroll
+    for (int t2 = 0; t2 < 2; ++t2) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[t2][e] = 0.f;
+#pragma unroll
+      for (int ds = 0; ds < NDS; ++ds) {
+        const Chunk16 kf = *reinterpret_cast<const Chunk16*>(smem + so + kbase[ds] + t2 * 32 * RB);
+        s[t2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf.v), __builtin_bit_cast(bf16x8, qf[ds].v), s[t2], 0, 0, 0);
+      }
+    }
+    // softmax: the lane's keys are 32 t2 + 8 i + 4 h + r
+    if constexpr (F8) {
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 ks = *reinterpret_cast<const f32x4*>(sc + 32 * t2 + 8 * i + 4 * h);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) s[t2][4 * i + q] *= ks[q];
+        }
+    }
+    int key0 = kt0 + 4 * h;
+    if constexpr (MASKED) {
+      asm volatile("" : "+v"(key0));
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (key0 + 32 * t2 + 8 * (e >> 2) + (e & 3) >= see) s[t2][e] = -INFINITY;
+    }
+    float mt = -INFINITY;
+#pragma unroll
+    for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[t2][e]);
+    mt = max_xor32(mt);
+    if constexpr (!F8) mt *= p.scale2;                 // scale > 0
+    const float m_new = fmaxf(m_run, mt), m_use = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m_run - m_use), nm = -m_use;
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0ull) {
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+    }
+    bool odd = false;                                  // infinities or NaN among the values of a masked tile
+    if constexpr (MASKED) {
+      bool ok = true;
+#pragma unroll
+      for (int i = 0; i < IMG / 1024; ++i) ok = ok && chunk_finite(reinterpret_cast<const Chunk16*>(smem + so + IMG + i * 1024)[lane], bf16_t());
+      odd = __builtin_amdgcn_ballot_w64(!ok) != 0ull;
+    }
+    float sum[2] = {0.f, 0.f};
+    auto weights = [&](auto T2) __attribute__((always_inline)) {
+      constexpr int t2 = decltype(T2)::value;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float ev = __builtin_amdgcn_exp2f(F8 ? s[t2][e] + nm : fmaf(s[t2][e], p.scale2, nm));
+        s[t2][e] = ev;
+        sum[e & 1] += ev;
+      }
+      if constexpr (F8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 vs = *reinterpret_cast<const f32x4*>(sc + KT + 32 * t2 + 8 * i + 4 * h);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            s[t2][4 * i + q] *= vs[q];
+            if (MASKED && key0 + 32 * t2 + 8 * i + q >= see) s[t2][4 * i + q] = 0.f;
+          }
+        }
+      }
+    };
+    if constexpr (MASKED) {
+      static_for<0, 2>(weights);
+      if (__builtin_expect(odd, 0)) {
+        const char* sV = smem + so + IMG;
+        for (int k = 0; k < KT; ++k) {
+          float pe = 0.f;
+#pragma unroll
+          for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (k >> 5 == t2 && ((k >> 3) & 3) == e >> 2 && (k & 3) == (e & 3)) pe = s[t2][e];
+          pe = __shfl(pe, ((k >> 2) & 1) * 32 + ql, 64);
+          if (kt0 + k < see)
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+              for (int q = 0; q < 16; ++q) {
+                const int byte = (32 * dt + 8 * (q >> 2) + 4 * h + (q & 3)) * 2;
+                const float vv = (float)*reinterpret_cast<const bf16_t*>(sV + k * RB + (((byte >> 4) ^ swizzle<RB>(k)) << 4) + (byte & 15));
+                if (!is_finite(vv)) o[dt][q] += pe * vv;
+                if (q & 1) asm volatile("" ::: "memory");      // few of these reads at a time: this code must not cost the common path registers
+              }
+        }
+      }
+    }
+    static_for<0, 2>([&](auto T2) __attribute__((always_inline)) {
+      constexpr int t2 = decltype(T2)::value;
+      if constexpr (!MASKED) weights(T2);
+#pragma unroll
+      for (int sl = 0; sl < 2; ++sl) {
+        bf16x8 pf;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) pf[q] = (bf16_t)s[t2][8 * sl + q];
+        const unsigned step = so + (2 * t2 + sl) * 16 * RB;
+        unsigned at[NDT];
+        u32x4 w[NDT];
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) at[dt] = vbase[dt] + step;
+        if constexpr (NDT == 4) read_tr16_x4<8 * RB>(at, w);
+        else read_tr16_x2<8 * RB>(at, w);
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) {
+          bf16x8 vf = __builtin_bit_cast(bf16x8, w[dt]);
+          if (MASKED && odd) vf = finite_part(vf);
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o[dt], 0, 0, 0);
+        }
+      }
+    });
+    l_run = l_run * alpha + (sum[0] + sum[1]);
+    m_run = m_new;
+  };
+
+  auto tile = [&](int t, auto masked_tag) __attribute__((always_inline)) {
+    const int kt0 = kbeg + t * KT;
+    if constexpr (F8) {
+      __syncthreads();
+      if (t + 1 < ntile) widen(raw, (t + 1) & 1);      // (its slot held tile t - 1: every wave is past it)
+      if (t + 2 < ntile) { fetch(kt0 + 2 * KT, raw); next_pages(kt0 + 3 * KT); }
+    } else {
+      // tile t has landed once only tile t + 1's instructions of this wave are on their way
+      if (t + 1 < ntile) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(VM) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (t + 2 < ntile) { issue(kt0 + 2 * KT, (t + 2) % 3); next_pages(kt0 + 3 * KT); }      // (its slot held tile t - 1)
+    }
+    if (!decltype(masked_tag)::value || kt0 < see_max) compute(kt0, (F8 ? (t & 1) : t % 3) * STAGE, masked_tag);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // this wave has read the tile when it meets the next barrier
+  };
+  // two loops, each with one body: as two branches of one loop the bodies' accumulators met in copies of all of them
+  const int t_full = rows_here ? min(ntile, max(0, see_min - kbeg) / KT) : 0;
+  int t = 0;
+  for (; t < t_full; ++t) tile(t, std::false_type{});
+  for (; t < ntile; ++t) tile(t, std::true_type{});
+  if (bad_page && lane == 0) paged_report(p.kv.status, kBadPage);
+
+  if (r >= packed) return;
+  float l = l_run;
+  l += __shfl_xor(l, 32, 64);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (p.split) {
+    const int64_t at_row = ((int64_t)split * p.b.rows + row) * p.n_heads + head;
+    if (h == 0) p.part_ml[at_row] = make_float2(m_run, l);
+    float* P = p.part + at_row * HD;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4*>(P + 32 * dt + 8 * i + 4 * h) = f32x4{o[dt][4 * i] * inv, o[dt][4 * i + 1] * inv, o[dt][4 * i + 2] * inv, o[dt][4 * i + 3] * inv};
+    return;
+  }
+  if (p.lse && h == 0) p.lse[row * p.n_heads + head] = l == 0.f ? -INFINITY : (m_run + log2f(l)) * 0.69314718055994530942f;
+  bf16_t* O = reinterpret_cast<bf16_t*>(p.O) + row * p.ldo + (int64_t)head * HD;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      bf16x4 w;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) w[q] = (bf16_t)(o[dt][4 * i + q] * inv);
+      *reinterpret_cast<bf16x4*>(O + 32 * dt + 8 * i + 4 * h) = w;
+    }
+}
+
 template <typename T, bool F8, int HD>
 __global__ __launch_bounds__(kThreads) void paged_attn_kernel(const PagedAttnKArgs p) {
   constexpr int RB = HD * (int)sizeof(T), NCH = RB / 16, SWZ = RB == 128 ? 7 : 15, NBLK = RB / 64, NDT = HD / 16, NLD = KT * NCH / kThreads;
@@ -735,13 +1061,15 @@ int cu_count() {
 }
 
 // How a call is laid out.
-struct Plan { int64_t tiles; int split, splits, tile_is_seq; bool decode, narrow; };
+struct Plan { int64_t tiles; int split, splits, tile_is_seq; bool decode, chunk, narrow; };
 Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
   Plan pl;
   const int G = a.n_heads / kv.n_kv_heads;
   pl.decode = (int64_t)b.max_q * G <= 16;
-  pl.tile_is_seq = (int64_t)b.max_q * G <= 64;
-  pl.tiles = pl.tile_is_seq ? b.n_seqs : (int64_t)b.rows * G / 64 + b.n_seqs;
+  pl.chunk = !pl.decode && kv.dtype == DT_BF16;
+  const int rows = pl.chunk ? 256 : 64;
+  pl.tile_is_seq = !pl.chunk && (int64_t)b.max_q * G <= rows;
+  pl.tiles = pl.tile_is_seq ? b.n_seqs : (int64_t)b.rows * G / rows + b.n_seqs;
   pl.split = a.split_keys;
   const int64_t wgs = pl.tiles * kv.n_kv_heads;
   pl.narrow = false;
@@ -778,7 +1106,9 @@ int launch_t(const PagedAttnKArgs& k, const Plan& pl, hipStream_t st) {
     constexpr int STAGE = DecodeShape<T, F8, HD>::STAGE, NS = 33 * 1024 / STAGE > 4 ? 4 : 33 * 1024 / STAGE, NS8 = 17 * 1024 / STAGE > 2 ? 2 : 17 * 1024 / STAGE;
     if (pl.narrow) hipLaunchKernelGGL((paged_decode_kernel<T, F8, HD, 2, NS>), grid, dim3(128), 0, st, k);
     else hipLaunchKernelGGL((paged_decode_kernel<T, F8, HD, 8, NS8>), grid, dim3(512), 0, st, k);
-  } else hipLaunchKernelGGL((paged_attn_kernel<T, F8, HD>), grid, dim3(kThreads), 0, st, k);
+  } else if (pl.chunk) {
+    if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((paged_chunk_kernel<F8, HD>), dim3((unsigned)(pl.tiles * k.kv.n_kv_heads * pl.splits)), dim3(512), 0, st, k);
+  } else if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((paged_attn_kernel<T, F8, HD>), grid, dim3(kThreads), 0, st, k);
   OAVSR_CHECK_HIP(hipGetLastError());
   if (pl.split) {
     hipLaunchKernelGGL((paged_merge_kernel<T, HD>), dim3((unsigned)((int64_t)k.b.rows * k.n_heads)), dim3(kThreads), 0, st, k);
@@ -806,10 +1136,10 @@ int launch_paged_attention(const PagedKv& kv, const PagedBatch& b, const PagedAt
   const uint64_t need = workspace_of(kv, b, a, pl);
   OAVSR_REQUIRE(need == 0 || (a.workspace && a.workspace_bytes >= need), "paged_attention: a workspace of %llu bytes is needed, %llu given", (unsigned long long)need,
                 (unsigned long long)(a.workspace ? a.workspace_bytes : 0));
-  OAVSR_REQUIRE(pl.tiles < (1ll << 31) && pl.splits <= 65535, "paged_attention: too many workgroups (%lld tiles, %d splits)", (long long)pl.tiles, pl.splits);
+  OAVSR_REQUIRE(pl.tiles * kv.n_kv_heads * pl.splits < (1ll << 31) && pl.splits <= 65535, "paged_attention: too many workgroups (%lld tiles, %d splits)", (long long)pl.tiles, pl.splits);
   PagedAttnKArgs k;
   k.kv = kv; k.b = b; k.Q = a.Q; k.ldq = a.ldq; k.O = a.O; k.ldo = a.ldo; k.lse = a.lse; k.scale2 = a.scale * 1.44269504088896340736f;
-  k.n_heads = a.n_heads; k.group = a.n_heads / kv.n_kv_heads; k.split = pl.split; k.tile_is_seq = pl.tile_is_seq;
+  k.n_heads = a.n_heads; k.group = a.n_heads / kv.n_kv_heads; k.split = pl.split; k.tile_is_seq = pl.tile_is_seq; k.tiles = (int)pl.tiles;
   k.part = reinterpret_cast<float*>(a.workspace);
   k.part_ml = reinterpret_cast<float2*>(k.part + (size_t)pl.splits * b.rows * a.n_heads * kv.head_dim);
   const bool f8 = kv.format == KV_E4M3;
