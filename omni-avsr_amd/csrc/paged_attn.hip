@@ -109,6 +109,9 @@ __device__ __forceinline__ Chunk16 cache_chunk(const void* base, int64_t at) {
   }
 }
 
+// Splits that hold keys of a row that sees `see` of them.  A row of one split (or none) is finished by that split's workgroup; the others leave partial results.
+__device__ __forceinline__ int splits_of(const PagedAttnKArgs& p, int see) { return p.split && see > p.split ? (see - 1) / p.split + 1 : 1; }
+
 // ---- pieces of the streaming kernels -----------------------------------------------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(2))) int i32x2;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
@@ -481,7 +484,9 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int64_t prow = sq.q0 + ptok;
-    if (p.split) {
+    const int n = splits_of(p, min(first_pos + ptok + 1, kmax));
+    if ((int)blockIdx.z >= n) continue;
+    if (n > 1) {
       const int64_t at = ((int64_t)blockIdx.z * p.b.rows + prow) * p.n_heads + phead;
       if (d0 == 0) p.part_ml[at] = make_float2(m, l);
       *reinterpret_cast<f32x4*>(p.part + at * HD + d0) = acc * inv;
@@ -502,11 +507,11 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
 // registers, each thread widening its 16 bytes once per tile for all waves, into a ring of two.  The kv head is the fastest part of a workgroup's number:
 // workgroups of one kv head then share an XCD (8 of them take the numbers in turn), and its L2 serves their common keys.
 // A wave skips the tiles none of its rows sees, and masks only those that some row sees in part.
-template <bool F8, int HD>
-__global__ __launch_bounds__(512, 2) void paged_chunk_kernel(const PagedAttnKArgs p) {
-  constexpr int NW = 8, ROWS = NW * 32, RB = HD * 2, IMG = KT * RB, NSTAGE = F8 ? 2 : 3, STAGE = 2 * IMG + (F8 ? 2 * KT * 4 : 0);
+template <bool F8, int HD, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttnKArgs p) {
+  constexpr int ROWS = NW * 32, RB = HD * 2, IMG = KT * RB, NSTAGE = F8 || (HD == 128 && NW == 4) ? 2 : 3, STAGE = 2 * IMG + (F8 ? 2 * KT * 4 : 0);
   constexpr int NCH = RB / 16, RPI = 1024 / RB, NSEG = IMG / 1024 / NW, NDS = HD / 16, NDT = HD / 32, VM = 2 * NSEG;
-  constexpr int FB = HD / 8;                           // 8 bits: bytes per thread, image and tile
+  constexpr int FB = HD / NW, RW = KT / NW;            // 8 bits: bytes per thread, image and tile; rows per wave
   __shared__ __attribute__((aligned(1024))) char smem[NSTAGE * STAGE];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ql = lane & 31, h = lane >> 5;
@@ -543,7 +548,7 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_kernel(const PagedAttnKArg
   auto next_pages = [&](int kt0) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < NSEG; ++j) {
-      const int key = kt0 + (F8 ? wave * 8 : (wave + NW * j) * RPI);
+      const int key = kt0 + (F8 ? wave * RW : (wave + NW * j) * RPI);
       page[j] = -1;
       if (key < kend) { page[j] = uniform_page(p, seq, key, shift); bad_page |= page[j] < 0; }
     }
@@ -563,31 +568,31 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_kernel(const PagedAttnKArg
       __builtin_amdgcn_global_load_lds((global_ptr)(v + off), (lds_ptr)(dst + IMG), 16, 0, 0);
     }
   };
-  // 8 bits: thread = FB bytes of row tid / 8 of both images; lanes 0 .. 15 of a wave the scales of its 8 rows
+  // 8 bits: thread = FB bytes of a row of both images, NW threads a row; the first 2 RW lanes of a wave the scales of its rows
   struct Raw { unsigned k[FB / 4], v[FB / 4]; float scale; };
   auto fetch = [&](int kt0, Raw& x) __attribute__((always_inline)) {
-    const int key = kt0 + wave * 8 + (lane >> 3);
+    const int key = kt0 + wave * RW + lane / NW;
     const bool ok = page[0] >= 0 && key < kend;
     const int64_t tok_at = (int64_t)kvh * p.kv.page_size + (key & pmask);
-    const int64_t at = (int64_t)page[0] * page_bytes + tok_at * HD + (lane & 7) * FB;
+    const int64_t at = (int64_t)page[0] * page_bytes + tok_at * HD + (lane % NW) * FB;
     const char *k = ok ? Kb + at : zero, *v = ok ? Vb + at : zero;
-    __builtin_memcpy(x.k, __builtin_assume_aligned(k, FB), FB);
-    __builtin_memcpy(x.v, __builtin_assume_aligned(v, FB), FB);
-    const int skey = kt0 + wave * 8 + (lane & 7);
+    __builtin_memcpy(x.k, __builtin_assume_aligned(k, FB < 16 ? FB : 16), FB);
+    __builtin_memcpy(x.v, __builtin_assume_aligned(v, FB < 16 ? FB : 16), FB);
+    const int skey = kt0 + wave * RW + lane % RW;
     const int64_t sat = (int64_t)page[0] * p.kv.scale_stride + (int64_t)kvh * p.kv.page_size + (skey & pmask);
-    const float* sp = page[0] >= 0 && skey < kend ? ((lane & 8) ? p.kv.v_scale : p.kv.k_scale) + sat : reinterpret_cast<const float*>(zero);
+    const float* sp = page[0] >= 0 && skey < kend ? ((lane & RW) ? p.kv.v_scale : p.kv.k_scale) + sat : reinterpret_cast<const float*>(zero);
     x.scale = *sp;
   };
   auto widen = [&](const Raw& x, int slot) __attribute__((always_inline)) {
     char* dst = smem + slot * STAGE;
-    const int lrow = wave * 8 + (lane >> 3);
+    const int lrow = wave * RW + lane / NW;
 #pragma unroll
     for (int c = 0; c < FB / 8; ++c) {
-      const int at = lrow * RB + ((((lane & 7) * (FB / 8) + c) ^ swizzle<RB>(lrow)) << 4);
+      const int at = lrow * RB + ((((lane % NW) * (FB / 8) + c) ^ swizzle<RB>(lrow)) << 4);
       *reinterpret_cast<bf16x8*>(dst + at) = join(e4m3_to_bf16(x.k[2 * c]), e4m3_to_bf16(x.k[2 * c + 1]));
       *reinterpret_cast<bf16x8*>(dst + IMG + at) = join(e4m3_to_bf16(x.v[2 * c]), e4m3_to_bf16(x.v[2 * c + 1]));
     }
-    if (lane < 16) reinterpret_cast<float*>(dst + 2 * IMG)[(lane & 8) * 8 + wave * 8 + (lane & 7)] = (lane & 8) ? x.scale : x.scale * p.scale2;
+    if (lane < 2 * RW) reinterpret_cast<float*>(dst + 2 * IMG)[((lane & RW) ? KT : 0) + wave * RW + lane % RW] = (lane & RW) ? x.scale : x.scale * p.scale2;
   };
 
   // Q^T fragments (B operand: lane = row ql, k-group h): step ds covers d = 16 ds + 8 h .. + 7
@@ -604,7 +609,7 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_kernel(const PagedAttnKArg
     if (ntile > 1) { fetch(kbeg + KT, raw); next_pages(kbeg + 2 * KT); }
   } else {
     if (ntile > 0) { issue(kbeg, 0); next_pages(kbeg + KT); }
-    if (ntile > 1) { issue(kbeg + KT, 1); next_pages(kbeg + 2 * KT); }
+    if (NSTAGE == 3 && ntile > 1) { issue(kbeg + KT, 1); next_pages(kbeg + 2 * KT); }
   }
 #pragma unroll
   for (int ds = 0; ds < NDS; ++ds) asm volatile("" : "+v"(qf[ds].v));      // waited for here, not in the loop
@@ -765,13 +770,14 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_kernel(const PagedAttnKArg
       if (t + 2 < ntile) { fetch(kt0 + 2 * KT, raw); next_pages(kt0 + 3 * KT); }
     } else {
       // tile t has landed once only tile t + 1's instructions of this wave are on their way
-      if (t + 1 < ntile) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(VM) : "memory");
+      if (NSTAGE == 3 && t + 1 < ntile) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(VM) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (t + 2 < ntile) { issue(kt0 + 2 * KT, (t + 2) % 3); next_pages(kt0 + 3 * KT); }      // (its slot held tile t - 1)
+      constexpr int AHEAD = NSTAGE - 1;
+      if (t + AHEAD < ntile) { issue(kt0 + AHEAD * KT, (t + AHEAD) % NSTAGE); next_pages(kt0 + (AHEAD + 1) * KT); }      // (its slot held tile t - 1)
     }
-    if (!decltype(masked_tag)::value || kt0 < see_max) compute(kt0, (F8 ? (t & 1) : t % 3) * STAGE, masked_tag);
+    if (!decltype(masked_tag)::value || kt0 < see_max) compute(kt0, (t % NSTAGE) * STAGE, masked_tag);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // this wave has read the tile when it meets the next barrier
   };
   // two loops, each with one body: as two branches of one loop the bodies' accumulators met in copies of all of them
@@ -785,7 +791,9 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_kernel(const PagedAttnKArg
   float l = l_run;
   l += __shfl_xor(l, 32, 64);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (p.split) {
+  const int n = splits_of(p, see);
+  if (split >= n) return;
+  if (n > 1) {
     const int64_t at_row = ((int64_t)split * p.b.rows + row) * p.n_heads + head;
     if (h == 0) p.part_ml[at_row] = make_float2(m_run, l);
     float* P = p.part + at_row * HD;
@@ -981,7 +989,9 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(const PagedAttnKAr
   l_run += __shfl_xor(l_run, 32, 64);
   if (r >= packed) return;
   const float inv = l_run == 0.f ? 0.f : 1.f / l_run;  // (a NaN sum stays one)
-  if (p.split) {
+  const int n = splits_of(p, see);
+  if ((int)blockIdx.z >= n) return;
+  if (n > 1) {
     const int64_t at_row = ((int64_t)blockIdx.z * p.b.rows + row) * p.n_heads + head;
     if (g == 0) p.part_ml[at_row] = make_float2(m_run, l_run);
     float* P = p.part + at_row * HD;
@@ -1002,55 +1012,62 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(const PagedAttnKAr
   }
 }
 
-// Joins the splits of a row's keys: a workgroup per (row, head).  out = sum_z w_z O_z / sum_z w_z,  w_z = l_z 2^(m_z - max m).  Its threads are groups of
-// HD / 4 that take every NG-th split, joined in LDS in a fixed order: the time is one or two loads' latency, not the number of splits.
-template <typename T, int HD>
+// Joins the splits of the rows whose keys lie in more than one:  out = sum_z w_z O_z / sum_z w_z,  w_z = l_z 2^(m_z - max m).  NG groups of HD / 4 threads share
+// a (row, head), each taking every NG-th split, joined in LDS in a fixed order: one group where the splits are few and the rows many, all of a
+// workgroup's where it is the other way round.
+template <typename T, int HD, int NG>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnKArgs p) {
-  constexpr int TPG = HD / 4, NG = kThreads / TPG;
-  __shared__ __attribute__((aligned(16))) float acc_s[NG][HD];
-  __shared__ float m_s[NG], l_s[NG];
+  constexpr int TPG = HD / 4, PER = kThreads / (TPG * NG);      // (row, head) pairs per workgroup: heads of one row
+  __shared__ __attribute__((aligned(16))) float acc_s[NG == 1 ? 1 : kThreads / TPG][HD];
+  __shared__ float m_s[kThreads / TPG], l_s[kThreads / TPG];
   const int tid = threadIdx.x, lane = tid & 63;
-  const int64_t i = blockIdx.x;
-  const int row = (int)(i / p.n_heads), head = (int)(i - (int64_t)row * p.n_heads);
+  const int hb = (p.n_heads + PER - 1) / PER, row = blockIdx.x / hb;
+  const int sub = tid / TPG, grp = sub % NG, head = (blockIdx.x - row * hb) * PER + sub / NG, d0 = (tid % TPG) * 4;
   const int seq = wave_find_seq(p.b.cu_q, p.b.n_seqs, row, lane);
   const SeqInfo sq = paged_seq(p.b, seq);
   if (row < sq.q0 || row >= sq.q0 + sq.nq) return;
-  const int see = min(sq.ctx - sq.nq + (row - sq.q0) + 1, min(sq.ctx, p.b.max_ctx));
-  const int n = see > 0 ? (see - 1) / p.split + 1 : 0;
-  const int grp = tid / TPG, d0 = (tid - grp * TPG) * 4;
+  const int n = splits_of(p, min(sq.ctx - sq.nq + (row - sq.q0) + 1, min(sq.ctx, p.b.max_ctx)));
+  if (n <= 1) return;
   float m = -INFINITY, l = 0.f;
   f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int z = grp; z < n; z += NG) {
-    const int64_t at = ((int64_t)z * p.b.rows + row) * p.n_heads + head;
-    const float2 ml = p.part_ml[at];
-    const f32x4 x = *reinterpret_cast<const f32x4*>(p.part + at * HD + d0);
-    const float mn = fmaxf(m, ml.x), mu = mn == -INFINITY ? 0.f : mn;
-    const float w0 = __builtin_amdgcn_exp2f(m - mu), w1 = __builtin_amdgcn_exp2f(ml.x - mu) * ml.y;
-    l = l * w0 + w1;
-    m = mn;
+  if (head < p.n_heads) {
+#pragma unroll 2
+    for (int z = grp; z < n; z += NG) {
+      const int64_t at = ((int64_t)z * p.b.rows + row) * p.n_heads + head;
+      const float2 ml = p.part_ml[at];
+      const f32x4 x = *reinterpret_cast<const f32x4*>(p.part + at * HD + d0);
+      const float mn = fmaxf(m, ml.x), mu = mn == -INFINITY ? 0.f : mn;
+      const float w0 = __builtin_amdgcn_exp2f(m - mu), w1 = __builtin_amdgcn_exp2f(ml.x - mu) * ml.y;
+      l = l * w0 + w1;
+      m = mn;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = acc[e] * w0 + w1 * x[e];
+      for (int e = 0; e < 4; ++e) acc[e] = acc[e] * w0 + w1 * x[e];
+    }
   }
-  if (d0 == 0) { m_s[grp] = m; l_s[grp] = l; }
-  *reinterpret_cast<f32x4*>(&acc_s[grp][d0]) = acc;
-  __syncthreads();
-  if (grp > 0) return;
-  float mm = -INFINITY, ll = 0.f;
+  if constexpr (NG > 1) {
+    if (d0 == 0) { m_s[sub] = m; l_s[sub] = l; }
+    *reinterpret_cast<f32x4*>(&acc_s[sub][d0]) = acc;
+    __syncthreads();
+    if (grp > 0) return;
+    m = -INFINITY;
+    l = 0.f;
 #pragma unroll
-  for (int j = 0; j < NG; ++j) mm = fmaxf(mm, m_s[j]);
-  const float mu = mm == -INFINITY ? 0.f : mm;
-  acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < NG; ++j) m = fmaxf(m, m_s[sub + j]);
+    const float mu = m == -INFINITY ? 0.f : m;
+    acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int j = 0; j < NG; ++j) {
-    const float w = __builtin_amdgcn_exp2f(m_s[j] - mu);
-    ll = fmaf(w, l_s[j], ll);
-    const f32x4 x = *reinterpret_cast<const f32x4*>(&acc_s[j][d0]);
+    for (int j = 0; j < NG; ++j) {
+      const float w = __builtin_amdgcn_exp2f(m_s[sub + j] - mu);
+      l = fmaf(w, l_s[sub + j], l);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(&acc_s[sub + j][d0]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, x[e], acc[e]);
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, x[e], acc[e]);
+    }
   }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
-  if (p.lse && d0 == 0) p.lse[i] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994530942f;
-  T* O = reinterpret_cast<T*>(p.O) + row * p.ldo + (int64_t)head * HD + d0;
+  if (head >= p.n_heads) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (p.lse && d0 == 0) p.lse[(int64_t)row * p.n_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+  T* O = reinterpret_cast<T*>(p.O) + (int64_t)row * p.ldo + (int64_t)head * HD + d0;
   if constexpr (sizeof(T) == 2) *reinterpret_cast<bf16x4*>(O) = bf16x4{(bf16_t)(acc[0] * inv), (bf16_t)(acc[1] * inv), (bf16_t)(acc[2] * inv), (bf16_t)(acc[3] * inv)};
   else *reinterpret_cast<f32x4*>(O) = acc * inv;
 }
@@ -1060,30 +1077,41 @@ int cu_count() {
   return n;
 }
 
-// How a call is laid out.
-struct Plan { int64_t tiles; int split, splits, tile_is_seq; bool decode, chunk, narrow; };
+// How a call is laid out: by its sizes' bounds alone, since the lengths are on the device.
+//   decode  up to 16 packed rows per sequence: the streaming kernel.  Eight waves a workgroup where that gives every one of few workgroups a CU, two where
+//           there are more (two workgroups side by side: 97 rows of 6000 keys 145 us, eight waves 160).
+//   chunk   more, bf16: 128 packed rows a workgroup, two side by side; 256 at head_dim 128 for even batches whose context is long against the new
+//           tokens, where keys are fetched once per 256 rows and few tiles are cut by the diagonal (2048 new tokens over 16384, 32 / 8 heads: 582 us against
+//           628; a prompt of 8192 alone: 746 against 734).
+//   split   keys per workgroup.  Single tokens: as many splits as give two rounds of workgroups, rounded down where there are many (131072 keys of 3
+//           sequences: 40 splits fill 1.9 rounds, 161 us; 43 begin a third, 193) and up where there are few.  Chunks: an even batch only up to
+//           one round, a ragged one two, since its longest sequence else runs on alone (24 sequences, 5 of them chunks of up to 701: 87 us, unsplit 145).
+struct Plan { int64_t tiles; int split, splits, nw; bool decode, chunk, tile_is_seq; };
 Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
   Plan pl;
-  const int G = a.n_heads / kv.n_kv_heads;
+  const int G = a.n_heads / kv.n_kv_heads, cus = cu_count();
+  const int64_t packed = (int64_t)b.rows * G;
+  const bool even = b.rows >= (int64_t)b.n_seqs * b.max_q;      // all sequences bring max_q tokens
   pl.decode = (int64_t)b.max_q * G <= 16;
   pl.chunk = !pl.decode && kv.dtype == DT_BF16;
-  const int rows = pl.chunk ? 256 : 64;
+  pl.nw = pl.chunk && kv.head_dim == 128 && even && b.max_ctx >= 4ll * b.max_q ? 8 : 4;
+  const int rows = pl.chunk ? 32 * pl.nw : 64;
   pl.tile_is_seq = !pl.chunk && (int64_t)b.max_q * G <= rows;
-  pl.tiles = pl.tile_is_seq ? b.n_seqs : (int64_t)b.rows * G / rows + b.n_seqs;
+  pl.tiles = pl.tile_is_seq ? b.n_seqs : packed / rows + b.n_seqs;
+  const int64_t wgs = std::max<int64_t>(1, pl.tiles * kv.n_kv_heads);
+  const int64_t slots = (int64_t)cus * (pl.nw == 8 ? 1 : 2);      // workgroups side by side
   pl.split = a.split_keys;
-  const int64_t wgs = pl.tiles * kv.n_kv_heads;
-  pl.narrow = false;
   if (!pl.split) {
-    if (pl.decode && wgs <= cu_count() && b.max_ctx <= 1024) pl.split = 1024;
+    if (pl.decode && wgs <= cus && b.max_ctx <= 1024) pl.split = 1024;
     else {
-      const int64_t want = 4 * cu_count(), n = want / (wgs > 0 ? wgs : 1);
-      const int64_t k = n > 1 ? ceil_div64(b.max_ctx, n) : b.max_ctx;
-      pl.split = (int)std::max<int64_t>(256, (k + 255) / 256 * 256);
+      const int64_t down = 2 * slots / wgs, up = ceil_div64(2 * slots, wgs);
+      const int64_t n = pl.decode ? (down >= 8 ? down : up) : even ? slots / wgs : up;
+      pl.split = (int)std::max<int64_t>(512, ceil_div64(ceil_div64(b.max_ctx, std::max<int64_t>(1, n)), 256) * 256);
     }
   }
-  pl.splits = b.max_ctx > 0 ? ceil_div(b.max_ctx, pl.split) : 1;
+  pl.splits = ceil_div(b.max_ctx, pl.split);
   if (pl.splits <= 1) pl.split = 0, pl.splits = 1;
-  pl.narrow = wgs * pl.splits > cu_count();      // more workgroups than CUs: two waves each, several side by side; else eight for one
+  if (pl.decode) pl.nw = wgs * pl.splits > cus ? 2 : 8;
   return pl;
 }
 uint64_t workspace_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a, const Plan& pl) {
@@ -1104,14 +1132,20 @@ int launch_t(const PagedAttnKArgs& k, const Plan& pl, hipStream_t st) {
   const dim3 grid((unsigned)pl.tiles, k.kv.n_kv_heads, pl.splits);
   if (pl.decode) {
     constexpr int STAGE = DecodeShape<T, F8, HD>::STAGE, NS = 33 * 1024 / STAGE > 4 ? 4 : 33 * 1024 / STAGE, NS8 = 17 * 1024 / STAGE > 2 ? 2 : 17 * 1024 / STAGE;
-    if (pl.narrow) hipLaunchKernelGGL((paged_decode_kernel<T, F8, HD, 2, NS>), grid, dim3(128), 0, st, k);
+    if (pl.nw == 2) hipLaunchKernelGGL((paged_decode_kernel<T, F8, HD, 2, NS>), grid, dim3(128), 0, st, k);
     else hipLaunchKernelGGL((paged_decode_kernel<T, F8, HD, 8, NS8>), grid, dim3(512), 0, st, k);
-  } else if (pl.chunk) {
-    if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((paged_chunk_kernel<F8, HD>), dim3((unsigned)(pl.tiles * k.kv.n_kv_heads * pl.splits)), dim3(512), 0, st, k);
-  } else if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((paged_attn_kernel<T, F8, HD>), grid, dim3(kThreads), 0, st, k);
+  } else if constexpr (sizeof(T) == 2) {
+    const dim3 line((unsigned)(pl.tiles * k.kv.n_kv_heads * pl.splits));
+    if constexpr (HD == 128) {
+      if (pl.nw == 8) hipLaunchKernelGGL((paged_chunk_kernel<F8, HD, 8>), line, dim3(512), 0, st, k);
+    }
+    if (pl.nw == 4) hipLaunchKernelGGL((paged_chunk_kernel<F8, HD, 4>), line, dim3(256), 0, st, k);
+  } else hipLaunchKernelGGL((paged_attn_kernel<T, F8, HD>), grid, dim3(kThreads), 0, st, k);
   OAVSR_CHECK_HIP(hipGetLastError());
   if (pl.split) {
-    hipLaunchKernelGGL((paged_merge_kernel<T, HD>), dim3((unsigned)((int64_t)k.b.rows * k.n_heads)), dim3(kThreads), 0, st, k);
+    constexpr int ALL = kThreads / (HD / 4);
+    if (pl.splits > 8) hipLaunchKernelGGL((paged_merge_kernel<T, HD, ALL>), dim3((unsigned)((int64_t)k.b.rows * k.n_heads)), dim3(kThreads), 0, st, k);
+    else hipLaunchKernelGGL((paged_merge_kernel<T, HD, 1>), dim3((unsigned)((int64_t)k.b.rows * ceil_div(k.n_heads, ALL))), dim3(kThreads), 0, st, k);
     OAVSR_CHECK_HIP(hipGetLastError());
   }
   return 0;

@@ -487,13 +487,13 @@ def test_refusals():
         "float32, the cache": lambda: paged.attention(kv, b, q.float()), "float16": lambda: paged.attention(kv, b, q.half()),
         "heads have 64": lambda: paged.attention(kv, b, z(2, 4, 32)), "multiple of kv": lambda: paged.attention(kv, b, z(2, 3, d)),
         "one piece": lambda: paged.attention(kv, b, z(2, d, H).transpose(1, 2)), "aligned": lambda: paged.attention(kv, b, z(2, H * d + 8)[:, 4:-4]), "strides": lambda: paged.attention(kv, b, z(2, H * d + 4)[:, :-4]),
-        "rows, q": lambda: paged.attention(kv, b, q, out=z(3, H, d)), "scale": lambda: paged.attention(kv, b, q, scale=0.0), "scale nan": lambda: paged.attention(kv, b, q, scale=float("nan")),
+        "3 rows, 2 are": lambda: paged.attention(kv, b, q, out=z(3, H, d)), "scale": lambda: paged.attention(kv, b, q, scale=0.0), "scale nan": lambda: paged.attention(kv, b, q, scale=float("nan")),
         "split_keys": lambda: paged.attention(kv, b, q, split_keys=64), "lse": lambda: paged.attention(kv, b, q, lse=z(2, H)), "overlap": lambda: paged.attention(kv, b, q, out=z(1, H, d).expand(2, H, d)),
         "does not hold max_ctx": lambda: paged.attention(kv, paged.PagedBatch(i32(0, 2), i32(20), i32(1, 2)[None], max_q=2, max_ctx=33), q),
         "query heads": lambda: paged.append(kv, b, z(2, 2 * KV * d)), "gains": lambda: paged.append(kv, b, qkv, q_gain=z(d, dt=torch.float32)),
         "q_gain is": lambda: paged.append(kv, b, qkv, q_gain=z(d), k_gain=z(d)), "pos is": lambda: paged.append(kv, b, qkv, pos=i32(1)),
         "inv_freq is": lambda: paged.append(kv, b, qkv, z(32)), "rotated": lambda: paged.append(kv, b, qkv, z(12, dt=torch.float32)),
-        "rows or out": lambda: paged.read(kv, b), "out has": lambda: paged.read(kv, b, 2, out=(z(3, KV, d), None)),
+        "rows or out": lambda: paged.read(kv, b), "out\\[0\\] has 3": lambda: paged.read(kv, b, 2, out=(z(3, KV, d), None)),
         "head_dim": lambda: paged.attention(paged.PagedKV.empty(2, 16, KV, 32), b, z(2, H, 32)), "page_size": lambda: paged.attention(paged.PagedKV.empty(2, 24, KV, d), b, q),
         "positions": lambda: paged.qk_norm_rope(qkv, H, KV, None, z(32, dt=torch.float32)), "do not hold": lambda: paged.qk_norm_rope(qkv, 3, KV, None, None),
         "v \\(": lambda: paged.PagedKV(z(2, 2, 16, 64), z(2, 2, 16, 32)), "8-bit": lambda: paged.PagedKV(z(2, 2, 16, 64), z(2, 2, 16, 64), z(2, 2, 16, dt=torch.float32)),
