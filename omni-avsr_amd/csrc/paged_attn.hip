@@ -26,7 +26,7 @@ struct PagedAttnKArgs {
   void* O; int64_t ldo;
   float* lse;
   float scale2;                                      // scale * log2 e
-  int n_heads, group, split, tile_is_seq, tiles;     // split: keys per workgroup (0: all); tile_is_seq: every sequence fits one tile; tiles: of all sequences (bound)
+  int n_heads, group, split, tiles;                  // split: keys per workgroup (0: all); tiles: of all sequences (bound)
   float* part;                                       // split: [splits][rows][n_heads][head_dim] O / l, then [splits][rows][n_heads] (m, l)
   float2* part_ml;
 };
@@ -83,6 +83,12 @@ __device__ __forceinline__ bool chunk_finite(const Chunk16& c, float) {
   return ok;
 }
 
+__device__ __forceinline__ bool e4m3_finite(const Chunk16& c) {
+  unsigned bad = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= (c.v[i] & 0x7f7f7f7fu) + 0x01010101u;
+  return (bad & 0x80808080u) == 0;
+}
 __device__ __forceinline__ bool is_finite(float x) { return (__builtin_bit_cast(unsigned, x) & 0x7f800000u) != 0x7f800000u; }
 // zeros in the place of infinities and NaN
 __device__ __forceinline__ bf16x8 finite_part(bf16x8 x) {
@@ -93,20 +99,6 @@ __device__ __forceinline__ bf16x8 finite_part(bf16x8 x) {
     if ((v[i] & 0x7f800000u) == 0x7f800000u) v[i] &= 0x0000ffffu;
   }
   return __builtin_bit_cast(bf16x8, v);
-}
-
-// 16 bytes of T from the cache: element e of a token's row
-template <typename T, bool F8>
-__device__ __forceinline__ Chunk16 cache_chunk(const void* base, int64_t at) {
-  if constexpr (!F8) return *reinterpret_cast<const Chunk16*>(reinterpret_cast<const T*>(base) + at);
-  else {
-    constexpr int VEC = TypeInfo<T>::kVec;
-    float x[VEC];
-    const unsigned* w = reinterpret_cast<const unsigned*>(reinterpret_cast<const char*>(base) + at);
-#pragma unroll
-    for (int i = 0; i < VEC / 4; ++i) e4m3_to_f32(w[i], x + 4 * i);
-    return chunk_from_f32<T>(x);                     // exact: three bits of mantissa
-  }
 }
 
 // Splits that hold keys of a row that sees `see` of them.  A row of one split (or none) is finished by that split's workgroup; the others leave partial results.
@@ -378,10 +370,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const Chunk16 c = reinterpret_cast<const Chunk16*>(sV + i * 1024)[lane];
-        if constexpr (F8) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w) ok = ok && (((c.v[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) == 0;
-        } else ok = ok && chunk_finite(c, T());
+        if constexpr (F8) ok = ok && e4m3_finite(c);
+        else ok = ok && chunk_finite(c, T());
       }
       odd = __builtin_amdgcn_ballot_w64(!ok) != 0ull;
     }
@@ -817,198 +807,244 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttn
     }
 }
 
-template <typename T, bool F8, int HD>
-__global__ __launch_bounds__(kThreads) void paged_attn_kernel(const PagedAttnKArgs p) {
-  constexpr int RB = HD * (int)sizeof(T), NCH = RB / 16, SWZ = RB == 128 ? 7 : 15, NBLK = RB / 64, NDT = HD / 16, NLD = KT * NCH / kThreads;
-  __shared__ __attribute__((aligned(16))) char sK[KT * RB];
-  __shared__ __attribute__((aligned(16))) char sV[KT * RB];
-  __shared__ float s_ks[KT], s_vs[KT];
-  __shared__ int s_odd;                                // the V tile holds an infinity or a NaN
+#ifndef F32_NC
+#define F32_NC 1
+#endif
+// ---- many rows per sequence, f32 ---------------------------------------------------------------------------------------------------------------
+//
+// The exact-f32 mode: a workgroup of 4 waves takes 64 packed rows, 16 per wave, on 16x16x4 matrix instructions, which bound it (32 cycles for 2048 flop;
+// reading the fragments from LDS takes a quarter of that).  Tiles of 32 keys through a ring that the waves share, as
+// cached bytes: 8-bit ones are widened where they are read.
+template <bool F8, int HD>
+__global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnKArgs p) {
+  constexpr int NW = 4, NC = F32_NC, ROWS = NW * 16 * NC, KT = 32, RB = HD * (F8 ? 1 : 4), IMG = KT * RB, STAGE = 2 * IMG + (F8 ? 256 : 0), NSTAGE = STAGE > 16 * 1024 ? 2 : 4;
+  constexpr int NCH = RB / 16, RPI = 1024 / RB, NI = IMG / 1024, NSEG = 2 * NI / NW, VM = NSEG + (F8 ? 1 : 0), NDT = HD / 16, NQ = HD / (F8 ? 64 : 16);
+  __shared__ __attribute__((aligned(1024))) char smem[NSTAGE * STAGE];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, qi = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.y, G = p.group;
-  const TileAt at = p.tile_is_seq ? TileAt{(int)blockIdx.x, 0} : wave_find_tile<64>(p.b, G, blockIdx.x, lane);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), qi = lane & 15, g = lane >> 4;
+  const int G = p.group, KV = p.kv.n_kv_heads;
+  const int kvh = blockIdx.x % KV, unit = blockIdx.x / KV, split = unit / p.tiles;
+  const TileAt at = wave_find_tile<ROWS>(p.b, G, unit - split * p.tiles, lane);
   if (at.seq < 0) return;
-  const SeqInfo sq = paged_seq(p.b, at.seq);
+  const int seq = __builtin_amdgcn_readfirstlane(at.seq), r0 = __builtin_amdgcn_readfirstlane(at.r0);
+  const SeqInfo sq = paged_seq(p.b, seq);
   if (sq.bad && tid == 0) paged_report(p.kv.status, kBadLength);
   const int packed = sq.nq * G;
-  if (at.r0 >= packed) return;
-  const int last_tok = (min(at.r0 + 64, packed) - 1) / G;
-  const int first_pos = sq.ctx - sq.nq;                // place of the sequence's first new token
-  const int kmax = min(sq.ctx, p.b.max_ctx);
-  const int kend_all = max(0, min(first_pos + last_tok + 1, kmax));
-  const int kbeg = p.split ? min(kend_all, (int)blockIdx.z * p.split) : 0;
-  if (p.split && blockIdx.z > 0 && kbeg >= kend_all) return;
+  const int first_pos = sq.ctx - sq.nq, kmax = min(sq.ctx, p.b.max_ctx);
+  const int kend_all = max(0, min(first_pos + (min(r0 + ROWS, packed) - 1) / G + 1, kmax));
+  const int kbeg = p.split ? split * p.split : 0;
+  if (split > 0 && kbeg >= kend_all) return;
   const int kend = p.split ? min(kend_all, kbeg + p.split) : kend_all;
+  const int ntile = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
 
-  const int r = at.r0 + wave * 16 + qi, rc = min(r, packed - 1), tok = rc / G, head = kvh * G + (rc - tok * G);
-  const int64_t row = sq.q0 + tok;
-  const int see = min(first_pos + tok + 1, kmax);      // keys this row sees
-  const int tok0 = min(at.r0 + wave * 16, packed - 1) / G, see0 = min(first_pos + tok0 + 1, kmax);      // ... and the wave's first row
-
-  Chunk16 qf[NBLK];
-  {
-    const char* qp = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.Q) + row * p.ldq + (int64_t)head * HD);
+  const int w0 = r0 + wave * 16 * NC;
+  const bool rows_here = w0 < packed;
+  const int see_min = min(first_pos + min(w0, packed - 1) / G + 1, kmax), see_max = rows_here ? min(first_pos + min(w0 + 16 * NC - 1, packed - 1) / G + 1, kmax) : 0;
+  int see[NC], head[NC];
+  int64_t row[NC];
+  Chunk16 qf[NC][NQ][F8 ? 4 : 1];
 #pragma unroll
-    for (int b = 0; b < NBLK; ++b) qf[b] = *reinterpret_cast<const Chunk16*>(qp + b * 64 + g * 16);
+  for (int c = 0; c < NC; ++c) {
+    const int rc = min(w0 + c * 16 + qi, packed - 1), tok = rc / G;
+    head[c] = kvh * G + (rc - tok * G);
+    row[c] = sq.q0 + tok;
+    see[c] = min(first_pos + tok + 1, kmax);
+    const float* qp = reinterpret_cast<const float*>(p.Q) + row[c] * p.ldq + (int64_t)head[c] * HD;
+#pragma unroll
+    for (int b = 0; b < NQ; ++b)
+#pragma unroll
+      for (int e = 0; e < (F8 ? 4 : 1); ++e) qf[c][b][e] = reinterpret_cast<const Chunk16*>(qp)[(b * 4 + g) * (F8 ? 4 : 1) + e];
   }
-  f32x4 o[NDT];
-#pragma unroll
-  for (int i = 0; i < NDT; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m_run = -INFINITY, l_run = 0.f;
-  const int shift = page_shift_of(p.kv);
 
-  for (int kt0 = kbeg; kt0 < kend; kt0 += KT) {
-    __syncthreads();
-    if (tid == 0) s_odd = 0;
-    __syncthreads();
+  const int shift = page_shift_of(p.kv), pmask = p.kv.page_size - 1;
+  const int64_t page_bytes = p.kv.page_stride * (F8 ? 1 : 4);
+  const char* zero = reinterpret_cast<const char*>(kZeroRows);
+  bool bad_page = false;
+  auto page_at = [&](int key) __attribute__((always_inline)) {
+    if (key >= kend) return -1;
+    const int page = uniform_page(p, seq, key, shift);
+    bad_page |= page < 0;
+    return page;
+  };
+  auto issue = [&](int kt0, int slot) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < NLD; ++j) {
-      const int id = tid + j * kThreads, krow = id / NCH, c = id - krow * NCH, key = kt0 + krow;
-      Chunk16 ck, cv;
-      ck.v = cv.v = u32x4{0u, 0u, 0u, 0u};
-      float ks = 0.f, vs = 0.f;
-      if (key < kend) {
-        const int page = paged_page(p.kv, p.b, at.seq, key, shift);
-        if (page >= 0) {
-          const int64_t t = (int64_t)kvh * p.kv.page_size + (key & (p.kv.page_size - 1));
-          const int64_t e = (int64_t)page * p.kv.page_stride + t * HD + c * TypeInfo<T>::kVec;
-          ck = cache_chunk<T, F8>(p.kv.K, e);
-          cv = cache_chunk<T, F8>(p.kv.V, e);
-          if constexpr (F8) {
-            ks = p.kv.k_scale[(int64_t)page * p.kv.scale_stride + t];
-            vs = p.kv.v_scale[(int64_t)page * p.kv.scale_stride + t];
-          }
-        } else if (c == 0) paged_report(p.kv.status, kBadPage);
-      }
-      const int off = krow * RB + ((c ^ (krow & SWZ)) << 4);
-      *reinterpret_cast<Chunk16*>(sK + off) = ck;
-      *reinterpret_cast<Chunk16*>(sV + off) = cv;
-      if (!chunk_finite(cv, T())) s_odd = 1;
-      if (F8 && c == 0) { s_ks[krow] = ks; s_vs[krow] = vs; }
+    for (int j = 0; j < NSEG; ++j) {
+      const int u = wave + NW * j, i = u % NI, key = kt0 + i * RPI, lrow = i * RPI + lane / NCH, page = page_at(key);
+      const char* base = reinterpret_cast<const char*>(u < NI ? p.kv.K : p.kv.V);
+      const char* src = page < 0 || kt0 + lrow >= kend ? zero : base + (int64_t)page * page_bytes + ((int64_t)kvh * p.kv.page_size + (key & pmask)) * RB;
+      src += (lane / NCH) * RB + (((lane % NCH) ^ swizzle<RB>(lrow)) << 4);
+      __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(smem + slot * STAGE + u * 1024), 16, 0, 0);
     }
-    __syncthreads();
-
-    const bool edge = kt0 + KT > see0;                 // some row of the wave does not see the whole tile
-    f32x4 s[4];
-    float mt = -INFINITY;
+    if constexpr (F8) {                                // (every wave the same 64 scales: one instruction, and the same count of them in every wave)
+      const int key = kt0 + (lane & 31), p0 = page_at(kt0), p1 = page_at(kt0 + 16), page = (lane & 16) ? p1 : p0;
+      const float* base = lane < 32 ? p.kv.k_scale : p.kv.v_scale;
+      const float* src = page < 0 || key >= kend ? reinterpret_cast<const float*>(zero)
+                                                 : base + (int64_t)page * p.kv.scale_stride + (int64_t)kvh * p.kv.page_size + (key & pmask);
+      __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(smem + slot * STAGE + 2 * IMG), 4, 0, 0);
+    }
+  };
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      s[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < NSTAGE - 1; ++i)
+    if (i < ntile) issue(kbeg + i * KT, i);
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int b = 0; b < NQ; ++b)
+#pragma unroll
+      for (int e = 0; e < (F8 ? 4 : 1); ++e) asm volatile("" : "+v"(qf[c][b][e].v));      // waited for here, not in the loop
+
+  f32x4 o[NC][NDT];
+  float m_run[NC], l_run[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    m_run[c] = -INFINITY;
+    l_run[c] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NDT; ++i) o[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  for (int t = 0; t < ntile; ++t) {
+    const int kt0 = kbeg + t * KT;
+    if (t + NSTAGE - 1 <= ntile) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(VM * (NSTAGE - 2)) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (t + NSTAGE - 1 < ntile) issue(kt0 + (NSTAGE - 1) * KT, (t + NSTAGE - 1) % NSTAGE);      // (its slot held tile t - 1: every wave is past it)
+    if (kt0 >= see_max) continue;
+    const char* sK = smem + (t % NSTAGE) * STAGE;
+    const char* sV = sK + IMG;
+    const float* sc = reinterpret_cast<const float*>(sK + 2 * IMG);
+    const bool edge = kt0 + KT > see_min;
+
+    f32x4 s[NC][2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) s[c][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
       const int krow = kt * 16 + qi;
 #pragma unroll
-      for (int b = 0; b < NBLK; ++b) Mma16<T>::run(*reinterpret_cast<const Chunk16*>(sK + krow * RB + (((b * 4 + g) ^ (krow & SWZ)) << 4)), qf[b], s[kt]);
+      for (int b = 0; b < NQ; ++b) {
+        const Chunk16 kc = *reinterpret_cast<const Chunk16*>(sK + krow * RB + (((b * 4 + g) ^ swizzle<RB>(krow)) << 4));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = kt * 16 + 4 * g + i;
-        float v = s[kt][i] * p.scale2;
-        if (F8) v *= s_ks[k];
-        if (edge && kt0 + k >= see) v = -INFINITY;
-        s[kt][i] = v;
-        mt = fmaxf(mt, v);
-      }
-    }
-    mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-    const float m_new = fmaxf(m_run, mt), m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = exp2f(m_run - m_use);
-    float sum = 0.f;
+        for (int w = 0; w < (F8 ? 4 : 1); ++w) {
+          float x[4];
+          if constexpr (F8) e4m3_to_f32(kc.v[w], x);
+          else chunk_to_f32<float>(kc, x);
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
+          for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = kt * 16 + 4 * g + i;
-        float e = exp2f(s[kt][i] - m_use);
-        sum += e;
-        if (F8) e *= s_vs[k];
-        if (edge && kt0 + k >= see) e = 0.f;
-        s[kt][i] = e;
-      }
-    l_run = l_run * alpha + sum;
-    m_run = m_new;
-#pragma unroll
-    for (int i = 0; i < NDT; ++i) o[i] *= alpha;
-
-    const bool odd = edge && s_odd;
-    if constexpr (sizeof(T) == 2) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        bf16x8 pf;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { pf[i] = (bf16_t)s[2 * u][i]; pf[4 + i] = (bf16_t)s[2 * u + 1][i]; }
-        const int qq = qi >> 2, pp = qi & 3;
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) {
-          const int c = dt * 2 + (pp >> 1), row0 = 32 * u + 4 * g + qq, row1 = row0 + 16;
-          const bf16x4 v0 = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(sV + row0 * RB + ((c ^ (row0 & SWZ)) << 4) + (pp & 1) * 8)));
-          const bf16x4 v1 = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(sV + row1 * RB + ((c ^ (row1 & SWZ)) << 4) + (pp & 1) * 8)));
-          bf16x8 vf;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) { vf[i] = v0[i]; vf[4 + i] = v1[i]; }
-          if (odd) vf = finite_part(vf);
-          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf, o[dt], 0, 0, 0);
+            for (int c = 0; c < NC; ++c) s[c][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], __builtin_bit_cast(f32x4, qf[c][b][w].v)[e], s[c][kt], 0, 0, 0);
         }
       }
-    } else {
+    }
+    auto v_at = [&](int krow, int d) -> float {
+      const int byte = d * (F8 ? 1 : 4);
+      const char* a = sV + krow * RB + (((byte >> 4) ^ swizzle<RB>(krow)) << 4) + (byte & 15);
+      if constexpr (F8) { float x[4]; e4m3_to_f32(*reinterpret_cast<const unsigned char*>(a), x); return x[0]; }
+      else return *reinterpret_cast<const float*>(a);
+    };
+    bool odd = false;                                  // infinities or NaN among the values of a masked tile
+    if (edge) {
+      bool ok = true;
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
+      for (int i = 0; i < NI; ++i) {
+        const Chunk16 x = reinterpret_cast<const Chunk16*>(sV + i * 1024)[lane];
+        if constexpr (F8) ok = ok && e4m3_finite(x);
+        else ok = ok && chunk_finite(x, float());
+      }
+      odd = __builtin_amdgcn_ballot_w64(!ok) != 0ull;
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      float mt = -INFINITY;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        f32x4 ks = f32x4{p.scale2, p.scale2, p.scale2, p.scale2};
+        if constexpr (F8) ks *= *reinterpret_cast<const f32x4*>(sc + kt * 16 + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v = s[c][kt][i] * ks[i];
+          if (edge && kt0 + kt * 16 + 4 * g + i >= see[c]) v = -INFINITY;
+          s[c][kt][i] = v;
+          mt = fmaxf(mt, v);
+        }
+      }
+      mt = max_xor16_32(mt);
+      const float m_new = fmaxf(m_run[c], mt), m_use = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f(m_run[c] - m_use);
+      float sum = 0.f;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        f32x4 vs = f32x4{1.f, 1.f, 1.f, 1.f};
+        if constexpr (F8) vs = *reinterpret_cast<const f32x4*>(sc + 32 + kt * 16 + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float e = __builtin_amdgcn_exp2f(s[c][kt][i] - m_use);
+          sum += e;
+          if constexpr (F8) e *= vs[i];
+          if (edge && kt0 + kt * 16 + 4 * g + i >= see[c]) e = 0.f;
+          s[c][kt][i] = e;
+        }
+      }
+      l_run[c] = l_run[c] * alpha + sum;
+      m_run[c] = m_new;
+      if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0ull) {
+#pragma unroll
+        for (int i = 0; i < NDT; ++i) o[c][i] *= alpha;
+      }
+      if (__builtin_expect(odd, 0)) {
+        for (int k = 0; k < KT; ++k) {
+          float e = 0.f;
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if ((k & 3) == i && (k >> 4) == kt) e = s[c][kt][i];
+          e = __shfl(e, ((k >> 2) & 3) * 16 + qi, 64);
+          if (kt0 + k < see[c])
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const float vv = v_at(k, dt * 16 + 4 * g + q);
+                if (!is_finite(vv)) o[c][dt][q] += e * vv;
+                if (q & 1) asm volatile("" ::: "memory");
+              }
+        }
+      }
+    }
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
-          const int c = dt * 4 + (qi >> 2);
+          float vv = v_at(kt * 16 + 4 * g + i, dt * 16 + qi);
+          if (odd && !is_finite(vv)) vv = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int krow = kt * 16 + 4 * g + i;
-            float vv = *reinterpret_cast<const float*>(sV + krow * RB + ((c ^ (krow & SWZ)) << 4) + (qi & 3) * 4);
-            if (odd && !is_finite(vv)) vv = 0.f;
-            o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv, s[kt][i], o[dt], 0, 0, 0);
-          }
+          for (int c = 0; c < NC; ++c) o[c][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv, s[c][kt][i], o[c][dt], 0, 0, 0);
         }
-    }
-    if (odd) {
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          for (int gg = 0; gg < 4; ++gg) {
-            const float e = __shfl(s[kt][i], gg * 16 + qi, 64);
-            const int krow = kt * 16 + 4 * gg + i;
-            if (kt0 + krow < see)
-#pragma unroll
-              for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  const int byte = (dt * 16 + 4 * g + q) * (int)sizeof(T);
-                  const float vv = to_f32(*reinterpret_cast<const T*>(sV + krow * RB + (((byte >> 4) ^ (krow & SWZ)) << 4) + (byte & 15)));
-                  if (!is_finite(vv)) o[dt][q] += e * vv;
-                }
-          }
-    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // this wave has read the tile when it meets the next barrier
   }
+  if (bad_page && lane == 0) paged_report(p.kv.status, kBadPage);
 
-  l_run += __shfl_xor(l_run, 16, 64);
-  l_run += __shfl_xor(l_run, 32, 64);
-  if (r >= packed) return;
-  const float inv = l_run == 0.f ? 0.f : 1.f / l_run;  // (a NaN sum stays one)
-  const int n = splits_of(p, see);
-  if ((int)blockIdx.z >= n) return;
-  if (n > 1) {
-    const int64_t at_row = ((int64_t)blockIdx.z * p.b.rows + row) * p.n_heads + head;
-    if (g == 0) p.part_ml[at_row] = make_float2(m_run, l_run);
-    float* P = p.part + at_row * HD;
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4*>(P + dt * 16 + 4 * g) = o[dt] * inv;
-    return;
-  }
-  if (p.lse && g == 0) p.lse[row * p.n_heads + head] = l_run == 0.f ? -INFINITY : (m_run + log2f(l_run)) * 0.69314718055994530942f;
-  T* O = reinterpret_cast<T*>(p.O) + row * p.ldo + (int64_t)head * HD;
+  for (int c = 0; c < NC; ++c) {
+    if (w0 + c * 16 + qi >= packed) continue;
+    float l = l_run[c];
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int n = splits_of(p, see[c]);
+    if (split >= n) continue;
+    float* O = reinterpret_cast<float*>(p.O) + row[c] * p.ldo + (int64_t)head[c] * HD;
+    if (n > 1) {
+      const int64_t at_row = ((int64_t)split * p.b.rows + row[c]) * p.n_heads + head[c];
+      if (g == 0) p.part_ml[at_row] = make_float2(m_run[c], l);
+      O = p.part + at_row * HD;
+    } else if (p.lse && g == 0) p.lse[row[c] * p.n_heads + head[c]] = l == 0.f ? -INFINITY : (m_run[c] + log2f(l)) * 0.69314718055994530942f;
 #pragma unroll
-  for (int dt = 0; dt < NDT; ++dt) {
-    if constexpr (sizeof(T) == 2) {
-      bf16x4 w;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = (bf16_t)(o[dt][i] * inv);
-      *reinterpret_cast<bf16x4*>(O + dt * 16 + 4 * g) = w;
-    } else *reinterpret_cast<f32x4*>(O + dt * 16 + 4 * g) = o[dt] * inv;
+    for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4*>(O + dt * 16 + 4 * g) = o[c][dt] * inv;
   }
 }
 
@@ -1080,24 +1116,21 @@ int cu_count() {
 // How a call is laid out: by its sizes' bounds alone, since the lengths are on the device.
 //   decode  up to 16 packed rows per sequence: the streaming kernel.  Eight waves a workgroup where that gives every one of few workgroups a CU, two where
 //           there are more (two workgroups side by side: 97 rows of 6000 keys 145 us, eight waves 160).
-//   chunk   more, bf16: 128 packed rows a workgroup, two side by side; 256 at head_dim 128 for even batches whose context is long against the new
+//   chunk   more: 128 packed rows a workgroup, two side by side; in bf16 256 at head_dim 128 for even batches whose context is long against the new
 //           tokens, where keys are fetched once per 256 rows and few tiles are cut by the diagonal (2048 new tokens over 16384, 32 / 8 heads: 582 us against
 //           628; a prompt of 8192 alone: 746 against 734).
 //   split   keys per workgroup.  Single tokens: as many splits as give two rounds of workgroups, rounded down where there are many (131072 keys of 3
 //           sequences: 40 splits fill 1.9 rounds, 161 us; 43 begin a third, 193) and up where there are few.  Chunks: an even batch only up to
 //           one round, a ragged one two, since its longest sequence else runs on alone (24 sequences, 5 of them chunks of up to 701: 87 us, unsplit 145).
-struct Plan { int64_t tiles; int split, splits, nw; bool decode, chunk, tile_is_seq; };
+struct Plan { int64_t tiles; int split, splits, nw; bool decode; };
 Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
   Plan pl;
   const int G = a.n_heads / kv.n_kv_heads, cus = cu_count();
   const int64_t packed = (int64_t)b.rows * G;
   const bool even = b.rows >= (int64_t)b.n_seqs * b.max_q;      // all sequences bring max_q tokens
   pl.decode = (int64_t)b.max_q * G <= 16;
-  pl.chunk = !pl.decode && kv.dtype == DT_BF16;
-  pl.nw = pl.chunk && kv.head_dim == 128 && even && b.max_ctx >= 4ll * b.max_q ? 8 : 4;
-  const int rows = pl.chunk ? 32 * pl.nw : 64;
-  pl.tile_is_seq = !pl.chunk && (int64_t)b.max_q * G <= rows;
-  pl.tiles = pl.tile_is_seq ? b.n_seqs : packed / rows + b.n_seqs;
+  pl.nw = !pl.decode && kv.dtype == DT_BF16 && kv.head_dim == 128 && even && b.max_ctx >= 4ll * b.max_q ? 8 : 4;
+  pl.tiles = pl.decode ? b.n_seqs : packed / (kv.dtype == DT_F32 ? 64 * F32_NC : 32 * pl.nw) + b.n_seqs;
   const int64_t wgs = std::max<int64_t>(1, pl.tiles * kv.n_kv_heads);
   const int64_t slots = (int64_t)cus * (pl.nw == 8 ? 1 : 2);      // workgroups side by side
   pl.split = a.split_keys;
@@ -1129,18 +1162,19 @@ int check_attn(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
 
 template <typename T, bool F8, int HD>
 int launch_t(const PagedAttnKArgs& k, const Plan& pl, hipStream_t st) {
-  const dim3 grid((unsigned)pl.tiles, k.kv.n_kv_heads, pl.splits);
+  const dim3 line((unsigned)(pl.tiles * k.kv.n_kv_heads * pl.splits));
   if (pl.decode) {
+    const dim3 grid((unsigned)pl.tiles, k.kv.n_kv_heads, pl.splits);
     constexpr int STAGE = DecodeShape<T, F8, HD>::STAGE, NS = 33 * 1024 / STAGE > 4 ? 4 : 33 * 1024 / STAGE, NS8 = 17 * 1024 / STAGE > 2 ? 2 : 17 * 1024 / STAGE;
     if (pl.nw == 2) hipLaunchKernelGGL((paged_decode_kernel<T, F8, HD, 2, NS>), grid, dim3(128), 0, st, k);
     else hipLaunchKernelGGL((paged_decode_kernel<T, F8, HD, 8, NS8>), grid, dim3(512), 0, st, k);
-  } else if constexpr (sizeof(T) == 2) {
-    const dim3 line((unsigned)(pl.tiles * k.kv.n_kv_heads * pl.splits));
+  } else if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((paged_rows_f32_kernel<F8, HD>), line, dim3(256), 0, st, k);
+  else {
     if constexpr (HD == 128) {
       if (pl.nw == 8) hipLaunchKernelGGL((paged_chunk_kernel<F8, HD, 8>), line, dim3(512), 0, st, k);
     }
     if (pl.nw == 4) hipLaunchKernelGGL((paged_chunk_kernel<F8, HD, 4>), line, dim3(256), 0, st, k);
-  } else hipLaunchKernelGGL((paged_attn_kernel<T, F8, HD>), grid, dim3(kThreads), 0, st, k);
+  }
   OAVSR_CHECK_HIP(hipGetLastError());
   if (pl.split) {
     constexpr int ALL = kThreads / (HD / 4);
@@ -1173,7 +1207,7 @@ int launch_paged_attention(const PagedKv& kv, const PagedBatch& b, const PagedAt
   OAVSR_REQUIRE(pl.tiles * kv.n_kv_heads * pl.splits < (1ll << 31) && pl.splits <= 65535, "paged_attention: too many workgroups (%lld tiles, %d splits)", (long long)pl.tiles, pl.splits);
   PagedAttnKArgs k;
   k.kv = kv; k.b = b; k.Q = a.Q; k.ldq = a.ldq; k.O = a.O; k.ldo = a.ldo; k.lse = a.lse; k.scale2 = a.scale * 1.44269504088896340736f;
-  k.n_heads = a.n_heads; k.group = a.n_heads / kv.n_kv_heads; k.split = pl.split; k.tile_is_seq = pl.tile_is_seq; k.tiles = (int)pl.tiles;
+  k.n_heads = a.n_heads; k.group = a.n_heads / kv.n_kv_heads; k.split = pl.split; k.tiles = (int)pl.tiles;
   k.part = reinterpret_cast<float*>(a.workspace);
   k.part_ml = reinterpret_cast<float2*>(k.part + (size_t)pl.splits * b.rows * a.n_heads * kv.head_dim);
   const bool f8 = kv.format == KV_E4M3;
