@@ -140,32 +140,43 @@ __device__ __forceinline__ int uniform_page(const PagedAttnKArgs& p, int seq, in
 // what a key row that is no key (behind the context, or of a page that is none) is fetched from: 16 rows
 __device__ const Chunk16 kZeroRows[16 * 512 / 16] = {};
 
+// f32 values: a lane reads four neighbours of a row at a time, one for each of four products, so that product dt of the O^T tiles holds the dimensions
+// f32_dim(dt, 0 .. 15) in its rows.
+__device__ __forceinline__ constexpr int f32_dim(int dt, int m) { return (dt >> 2) * 64 + 4 * m + (dt & 3); }
+template <bool F8, int RB>
+__device__ __forceinline__ void read_values4(const char* sV, int krow, int d, float (&out)[4]) {
+  const int byte = d * (F8 ? 1 : 4);
+  const char* at = sV + krow * RB + (((byte >> 4) ^ swizzle<RB>(krow)) << 4) + (byte & 15);
+  if constexpr (F8) e4m3_to_f32(*reinterpret_cast<const unsigned*>(at), out);
+  else chunk_to_f32<float>(*reinterpret_cast<const Chunk16*>(at), out);
+}
+
 __device__ __forceinline__ bf16x4 e4m3_to_bf16(unsigned w) {
   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true);
   return bf16x4{a[0], a[1], b[0], b[1]};                // exact
 }
-// Transposing reads of four 16-column blocks, waited for where they are made (the builtin makes the compiler wait for every LDS-DMA on its way first):
+// Transposing reads of four (two) 16-column blocks, AT bytes behind the given addresses, waited for where they are made (the builtin makes the compiler wait for every LDS-DMA on its way first):
 // lane 4 q + p of 16 gives the address of columns 4 p .. of row q and gets rows 0 .. 3 of its own column.  b16: two row blocks, OFF bytes apart; b8: eight rows,
 // lane 2 q + h giving bytes 8 h .. of row q.
-template <int OFF>
+template <int AT, int OFF>
 __device__ __forceinline__ void read_tr16_x4(const unsigned (&at)[4], u32x4 (&out)[4]) {
   i32x2 a[4], b[4];
-  asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\tds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
-               "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\tds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+  asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\tds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+               "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\tds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
                "s_waitcnt lgkmcnt(0)"
                : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1]), "=&v"(a[2]), "=&v"(b[2]), "=&v"(a[3]), "=&v"(b[3])
-               : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(OFF)
+               : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(AT), "n"(AT + OFF)
                : "memory");
 #pragma unroll
   for (int i = 0; i < 4; ++i) out[i] = u32x4{(unsigned)a[i][0], (unsigned)a[i][1], (unsigned)b[i][0], (unsigned)b[i][1]};
 }
-template <int OFF>
+template <int AT, int OFF>
 __device__ __forceinline__ void read_tr16_x2(const unsigned (&at)[2], u32x4 (&out)[2]) {
   i32x2 a[2], b[2];
-  asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\tds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
+  asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %4 offset:%7\n\tds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
                "s_waitcnt lgkmcnt(0)"
                : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1])
-               : "v"(at[0]), "v"(at[1]), "n"(OFF)
+               : "v"(at[0]), "v"(at[1]), "n"(AT), "n"(AT + OFF)
                : "memory");
 #pragma unroll
   for (int i = 0; i < 2; ++i) out[i] = u32x4{(unsigned)a[i][0], (unsigned)a[i][1], (unsigned)b[i][0], (unsigned)b[i][1]};
@@ -280,24 +291,26 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
 #pragma unroll
     for (int e = 0; e < QC; ++e) asm volatile("" : "+v"(qf[b][e].v));
 
+  auto dim_of = [](int dt, int m) { return sizeof(T) == 4 ? f32_dim(dt, m) : dt * 16 + m; };      // of row m of O^T tile dt
   f32x4 o[NDT];
 #pragma unroll
   for (int i = 0; i < NDT; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m_run = -INFINITY, l_run = 0.f;
 
-  for (int t = 0; t < ntile; ++t) {
+  int slot = 0;                                        // of tile t
+  auto tile = [&](int t, auto masked_tag) __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(masked_tag)::value;      // some row does not see the whole tile, or it ends behind the context
     const int kt0 = first + t * step;
     if (ntile - t >= NS) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(VM * (NS - 1)) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    char* sK = ring + (NS == 1 ? 0 : t % NS) * STAGE;
+    char* sK = ring + slot * STAGE;
     char* sV = sK + IMG;
     const float* sc = reinterpret_cast<const float*>(sK + 2 * IMG);
-    if (kt0 + KT > kend) {                             // rows behind the context: whatever the page holds there must not meet a zero
+    if (MASKED && kt0 + KT > kend) {                   // rows behind the context: whatever the page holds there must not meet a zero
 #pragma unroll
       for (int i = 0; i < NI; ++i)
         if (kt0 + i * RPI + lane / NCH >= kend) reinterpret_cast<Chunk16*>(sV + i * 1024)[lane].v = u32x4{0u, 0u, 0u, 0u};
     }
-    const bool edge = kt0 + KT > see_min;              // some row does not see the whole tile
 
     f32x4 s[NSUB];
     float mt = -INFINITY;
@@ -328,7 +341,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float v = s[kt][i] * ks[i];
-        if (edge && kt0 + kt * 16 + 4 * g + i >= see) v = -INFINITY;
+        if (MASKED && kt0 + kt * 16 + 4 * g + i >= see) v = -INFINITY;
         s[kt][i] = v;
         mt = fmaxf(mt, v);
       }
@@ -346,7 +359,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
         float e = __builtin_amdgcn_exp2f(s[kt][i] - m_use);
         sum += e;
         if constexpr (F8) e *= vs[i];
-        if (edge && kt0 + kt * 16 + 4 * g + i >= see) e = 0.f;
+        if (MASKED && kt0 + kt * 16 + 4 * g + i >= see) e = 0.f;
         s[kt][i] = e;
       }
     }
@@ -365,7 +378,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
       if constexpr (F8) { float x[4]; e4m3_to_f32(*reinterpret_cast<const unsigned char*>(at), x); return x[0]; }
       else return to_f32(*reinterpret_cast<const T*>(at));
     };
-    if (edge) {
+    if constexpr (MASKED) {
       bool ok = true;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
@@ -398,27 +411,31 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
           u32x4 w[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) at[j] = vb + krow * RB + ((((d4 + j) * 2 + (pp >> 1)) ^ swizzle<RB>(krow)) << 4) + (pp & 1) * 8;
-          read_tr16_x4<16 * RB>(at, w);
+          read_tr16_x4<0, 16 * RB>(at, w);
 #pragma unroll
           for (int j = 0; j < 4; ++j) vf[j] = __builtin_bit_cast(bf16x8, w[j]);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (odd) vf[j] = finite_part(vf[j]);
+          if (MASKED && odd) vf[j] = finite_part(vf[j]);
           o[d4 + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[j], pf, o[d4 + j], 0, 0, 0);
         }
       }
     } else {
 #pragma unroll
-      for (int dt = 0; dt < NDT; ++dt)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float vv = v_at(4 * g + i, dt * 16 + qi);
-          if (odd && !is_finite(vv)) vv = 0.f;
-          o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv, s[0][i], o[dt], 0, 0, 0);
+        for (int j = 0; j < HD / 64; ++j) {
+          float vv[4];
+          read_values4<F8, RB>(sV, 4 * g + i, 64 * j + 4 * qi, vv);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            if (MASKED && odd && !is_finite(vv[w])) vv[w] = 0.f;
+            o[4 * j + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[w], s[0][i], o[4 * j + w], 0, 0, 0);
+          }
         }
     }
-    if (odd) {
+    if (MASKED && __builtin_expect(odd, 0)) {
       for (int k = 0; k < KT; ++k) {
         float e = 0.f;
 #pragma unroll
@@ -432,16 +449,21 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
           for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const float vv = v_at(k, dt * 16 + 4 * g + q);
+              const float vv = v_at(k, dim_of(dt, 4 * g + q));
               if (!is_finite(vv)) o[dt][q] += e * vv;
             }
       }
     }
     if (t + NS < ntile) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // this tile has been read
-      issue(kt0 + NS * step, NS == 1 ? 0 : t % NS);
+      issue(kt0 + NS * step, slot);
     }
-  }
+    slot = slot == NS - 1 ? 0 : slot + 1;
+  };
+  const int t_full = see_min >= first + KT ? min(ntile, (see_min - first - KT) / step + 1) : 0;
+  int t = 0;
+  for (; t < t_full; ++t) tile(t, std::false_type{});
+  for (; t < ntile; ++t) tile(t, std::true_type{});
   if (bad_page && lane == 0) paged_report(p.kv.status, kBadPage);
 
   l_run += __shfl_xor(l_run, 16, 64);
@@ -451,7 +473,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) so[(dt * 16 + 4 * g + i) * 16 + qi] = o[dt][i];
+    for (int i = 0; i < 4; ++i) so[dim_of(dt, 4 * g + i) * 16 + qi] = o[dt][i];
   if (g == 0) { so[HD * 16 + qi] = m_run; so[HD * 16 + 16 + qi] = l_run; }
   __syncthreads();
   for (int i = tid; i < packed * (HD / 4); i += NW * 64) {
@@ -626,6 +648,9 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttn
   auto compute = [&](int kt0, unsigned so, auto masked_tag) __attribute__((always_inline)) {
     constexpr bool MASKED = decltype(masked_tag)::value;
     const float* sc = reinterpret_cast<const float*>(smem + so + 2 * IMG);
+    unsigned kat[NDS];
+#pragma unroll
+    for (int ds = 0; ds < NDS; ++ds) kat[ds] = so + kbase[ds];
     f32x16 s[2];
 #pragma unroll
     for (int t2 = 0; t2 < 2; ++t2) {
@@ -633,7 +658,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttn
       for (int e = 0; e < 16; ++e) s[t2][e] = 0.f;
 #pragma unroll
       for (int ds = 0; ds < NDS; ++ds) {
-        const Chunk16 kf = *reinterpret_cast<const Chunk16*>(smem + so + kbase[ds] + t2 * 32 * RB);
+        const Chunk16 kf = *reinterpret_cast<const Chunk16*>(smem + kat[ds] + t2 * 32 * RB);
         s[t2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf.v), __builtin_bit_cast(bf16x8, qf[ds].v), s[t2], 0, 0, 0);
       }
     }
@@ -725,21 +750,19 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttn
         }
       }
     }
-    static_for<0, 2>([&](auto T2) __attribute__((always_inline)) {
-      constexpr int t2 = decltype(T2)::value;
-      if constexpr (!MASKED) weights(T2);
+    unsigned vat[NDT];
 #pragma unroll
-      for (int sl = 0; sl < 2; ++sl) {
+    for (int dt = 0; dt < NDT; ++dt) vat[dt] = vbase[dt] + so;
+    static_for<0, 4>([&](auto ST) __attribute__((always_inline)) {
+      constexpr int st = decltype(ST)::value, t2 = st / 2, sl = st & 1;      // 16 keys
+      {
+        if constexpr (!MASKED && sl == 0) weights(std::integral_constant<int, t2>{});
         bf16x8 pf;
 #pragma unroll
         for (int q = 0; q < 8; ++q) pf[q] = (bf16_t)s[t2][8 * sl + q];
-        const unsigned step = so + (2 * t2 + sl) * 16 * RB;
-        unsigned at[NDT];
         u32x4 w[NDT];
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) at[dt] = vbase[dt] + step;
-        if constexpr (NDT == 4) read_tr16_x4<8 * RB>(at, w);
-        else read_tr16_x2<8 * RB>(at, w);
+        if constexpr (NDT == 4) read_tr16_x4<st * 16 * RB, 8 * RB>(vat, w);
+        else read_tr16_x2<st * 16 * RB, 8 * RB>(vat, w);
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
           bf16x8 vf = __builtin_bit_cast(bf16x8, w[dt]);
@@ -752,11 +775,12 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttn
     m_run = m_new;
   };
 
+  int slot = 0;                                        // of tile t
   auto tile = [&](int t, auto masked_tag) __attribute__((always_inline)) {
     const int kt0 = kbeg + t * KT;
     if constexpr (F8) {
       __syncthreads();
-      if (t + 1 < ntile) widen(raw, (t + 1) & 1);      // (its slot held tile t - 1: every wave is past it)
+      if (t + 1 < ntile) widen(raw, 1 - slot);         // (that slot held tile t - 1: every wave is past it)
       if (t + 2 < ntile) { fetch(kt0 + 2 * KT, raw); next_pages(kt0 + 3 * KT); }
     } else {
       // tile t has landed once only tile t + 1's instructions of this wave are on their way
@@ -765,9 +789,10 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttn
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       constexpr int AHEAD = NSTAGE - 1;
-      if (t + AHEAD < ntile) { issue(kt0 + AHEAD * KT, (t + AHEAD) % NSTAGE); next_pages(kt0 + (AHEAD + 1) * KT); }      // (its slot held tile t - 1)
+      if (t + AHEAD < ntile) { issue(kt0 + AHEAD * KT, slot == 0 ? AHEAD : slot - 1); next_pages(kt0 + (AHEAD + 1) * KT); }      // (that slot held tile t - 1)
     }
-    if (!decltype(masked_tag)::value || kt0 < see_max) compute(kt0, (t % NSTAGE) * STAGE, masked_tag);
+    if (!decltype(masked_tag)::value || kt0 < see_max) compute(kt0, slot * STAGE, masked_tag);
+    slot = slot == NSTAGE - 1 ? 0 : slot + 1;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // this wave has read the tile when it meets the next barrier
   };
   // two loops, each with one body: as two branches of one loop the bodies' accumulators met in copies of all of them
@@ -860,29 +885,34 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
   const int64_t page_bytes = p.kv.page_stride * (F8 ? 1 : 4);
   const char* zero = reinterpret_cast<const char*>(kZeroRows);
   bool bad_page = false;
-  auto page_at = [&](int key) __attribute__((always_inline)) {
-    if (key >= kend) return -1;
-    const int page = uniform_page(p, seq, key, shift);
-    bad_page |= page < 0;
-    return page;
+  int page[2];                                         // of the two halves of the next tile to fetch
+  auto next_pages = [&](int kt0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      page[j] = -1;
+      if (kt0 + 16 * j < kend) { page[j] = uniform_page(p, seq, kt0 + 16 * j, shift); bad_page |= page[j] < 0; }
+    }
   };
   auto issue = [&](int kt0, int slot) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < NSEG; ++j) {
-      const int u = wave + NW * j, i = u % NI, key = kt0 + i * RPI, lrow = i * RPI + lane / NCH, page = page_at(key);
+      const int u = wave + NW * j, i = u % NI, key = kt0 + i * RPI, lrow = i * RPI + lane / NCH, pg = i * RPI < 16 ? page[0] : page[1];
       const char* base = reinterpret_cast<const char*>(u < NI ? p.kv.K : p.kv.V);
-      const char* src = page < 0 || kt0 + lrow >= kend ? zero : base + (int64_t)page * page_bytes + ((int64_t)kvh * p.kv.page_size + (key & pmask)) * RB;
+      const char* src = pg < 0 ? zero : base + (int64_t)pg * page_bytes + ((int64_t)kvh * p.kv.page_size + (key & pmask)) * RB;
+      if (kt0 + KT > kend && kt0 + lrow >= kend) src = zero;      // behind the context: whatever the page holds must not meet a zero
       src += (lane / NCH) * RB + (((lane % NCH) ^ swizzle<RB>(lrow)) << 4);
       __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(smem + slot * STAGE + u * 1024), 16, 0, 0);
     }
     if constexpr (F8) {                                // (every wave the same 64 scales: one instruction, and the same count of them in every wave)
-      const int key = kt0 + (lane & 31), p0 = page_at(kt0), p1 = page_at(kt0 + 16), page = (lane & 16) ? p1 : p0;
+      const int key = kt0 + (lane & 31), pg = (lane & 16) ? page[1] : page[0];
       const float* base = lane < 32 ? p.kv.k_scale : p.kv.v_scale;
-      const float* src = page < 0 || key >= kend ? reinterpret_cast<const float*>(zero)
-                                                 : base + (int64_t)page * p.kv.scale_stride + (int64_t)kvh * p.kv.page_size + (key & pmask);
+      const float* src = pg < 0 || key >= kend ? reinterpret_cast<const float*>(zero)
+                                               : base + (int64_t)pg * p.kv.scale_stride + (int64_t)kvh * p.kv.page_size + (key & pmask);
       __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(smem + slot * STAGE + 2 * IMG), 4, 0, 0);
     }
+    next_pages(kt0 + KT);
   };
+  next_pages(kbeg);
 #pragma unroll
   for (int i = 0; i < NSTAGE - 1; ++i)
     if (i < ntile) issue(kbeg + i * KT, i);
@@ -903,38 +933,33 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
     for (int i = 0; i < NDT; ++i) o[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  for (int t = 0; t < ntile; ++t) {
-    const int kt0 = kbeg + t * KT;
-    if (t + NSTAGE - 1 <= ntile) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(VM * (NSTAGE - 2)) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (t + NSTAGE - 1 < ntile) issue(kt0 + (NSTAGE - 1) * KT, (t + NSTAGE - 1) % NSTAGE);      // (its slot held tile t - 1: every wave is past it)
-    if (kt0 >= see_max) continue;
-    const char* sK = smem + (t % NSTAGE) * STAGE;
+  auto compute = [&](int kt0, const char* sK, auto masked_tag) __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(masked_tag)::value;
     const char* sV = sK + IMG;
     const float* sc = reinterpret_cast<const float*>(sK + 2 * IMG);
-    const bool edge = kt0 + KT > see_min;
 
     f32x4 s[NC][2];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
+    for (int c = 0; c < NC; ++c) s[c][0] = s[c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < NC; ++c) s[c][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const int krow = kt * 16 + qi;
+    for (int b = 0; b < NQ; ++b) {
+      Chunk16 kc[2];
 #pragma unroll
-      for (int b = 0; b < NQ; ++b) {
-        const Chunk16 kc = *reinterpret_cast<const Chunk16*>(sK + krow * RB + (((b * 4 + g) ^ swizzle<RB>(krow)) << 4));
+      for (int kt = 0; kt < 2; ++kt) kc[kt] = *reinterpret_cast<const Chunk16*>(sK + (kt * 16 + qi) * RB + (((b * 4 + g) ^ swizzle<RB>(qi)) << 4));      // (+ 16 rows: the same swizzle)
 #pragma unroll
-        for (int w = 0; w < (F8 ? 4 : 1); ++w) {
-          float x[4];
-          if constexpr (F8) e4m3_to_f32(kc.v[w], x);
-          else chunk_to_f32<float>(kc, x);
+      for (int w = 0; w < (F8 ? 4 : 1); ++w) {
+        float x[2][4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int c = 0; c < NC; ++c) s[c][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], __builtin_bit_cast(f32x4, qf[c][b][w].v)[e], s[c][kt], 0, 0, 0);
+        for (int kt = 0; kt < 2; ++kt) {
+          if constexpr (F8) e4m3_to_f32(kc[kt].v[w], x[kt]);
+          else chunk_to_f32<float>(kc[kt], x[kt]);
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)              // chains of products that do not wait for each other
+#pragma unroll
+            for (int c = 0; c < NC; ++c) s[c][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[kt][e], __builtin_bit_cast(f32x4, qf[c][b][w].v)[e], s[c][kt], 0, 0, 0);
       }
     }
     auto v_at = [&](int krow, int d) -> float {
@@ -944,7 +969,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
       else return *reinterpret_cast<const float*>(a);
     };
     bool odd = false;                                  // infinities or NaN among the values of a masked tile
-    if (edge) {
+    if constexpr (MASKED) {
       bool ok = true;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
@@ -964,7 +989,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float v = s[c][kt][i] * ks[i];
-          if (edge && kt0 + kt * 16 + 4 * g + i >= see[c]) v = -INFINITY;
+          if (MASKED && kt0 + kt * 16 + 4 * g + i >= see[c]) v = -INFINITY;
           s[c][kt][i] = v;
           mt = fmaxf(mt, v);
         }
@@ -982,7 +1007,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
           float e = __builtin_amdgcn_exp2f(s[c][kt][i] - m_use);
           sum += e;
           if constexpr (F8) e *= vs[i];
-          if (edge && kt0 + kt * 16 + 4 * g + i >= see[c]) e = 0.f;
+          if (MASKED && kt0 + kt * 16 + 4 * g + i >= see[c]) e = 0.f;
           s[c][kt][i] = e;
         }
       }
@@ -992,7 +1017,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
 #pragma unroll
         for (int i = 0; i < NDT; ++i) o[c][i] *= alpha;
       }
-      if (__builtin_expect(odd, 0)) {
+      if (MASKED && __builtin_expect(odd, 0)) {
         for (int k = 0; k < KT; ++k) {
           float e = 0.f;
 #pragma unroll
@@ -1006,7 +1031,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
             for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
-                const float vv = v_at(k, dt * 16 + 4 * g + q);
+                const float vv = v_at(k, f32_dim(dt, 4 * g + q));
                 if (!is_finite(vv)) o[c][dt][q] += e * vv;
                 if (q & 1) asm volatile("" ::: "memory");
               }
@@ -1018,14 +1043,33 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) {
-          float vv = v_at(kt * 16 + 4 * g + i, dt * 16 + qi);
-          if (odd && !is_finite(vv)) vv = 0.f;
+        for (int j = 0; j < HD / 64; ++j) {
+          float vv[4];
+          read_values4<F8, RB>(sV, kt * 16 + 4 * g + i, 64 * j + 4 * qi, vv);
 #pragma unroll
-          for (int c = 0; c < NC; ++c) o[c][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv, s[c][kt][i], o[c][dt], 0, 0, 0);
+          for (int w = 0; w < 4; ++w) {
+            if (MASKED && odd && !is_finite(vv[w])) vv[w] = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) o[c][4 * j + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[w], s[c][kt][i], o[c][4 * j + w], 0, 0, 0);
+          }
         }
+  };
+  int slot = 0;                                        // of tile t
+  auto tile = [&](int t, auto masked_tag) __attribute__((always_inline)) {
+    const int kt0 = kbeg + t * KT;
+    if (t + NSTAGE - 1 <= ntile) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(VM * (NSTAGE - 2)) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (t + NSTAGE - 1 < ntile) issue(kt0 + (NSTAGE - 1) * KT, slot == 0 ? NSTAGE - 1 : slot - 1);      // (that slot held tile t - 1: every wave is past it)
+    if (!decltype(masked_tag)::value || kt0 < see_max) compute(kt0, smem + slot * STAGE, masked_tag);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // this wave has read the tile when it meets the next barrier
-  }
+    slot = slot == NSTAGE - 1 ? 0 : slot + 1;
+  };
+  const int t_full = rows_here ? min(ntile, max(0, see_min - kbeg) / KT) : 0;
+  int t = 0;
+  for (; t < t_full; ++t) tile(t, std::false_type{});
+  for (; t < ntile; ++t) tile(t, std::true_type{});
   if (bad_page && lane == 0) paged_report(p.kv.status, kBadPage);
 
 #pragma unroll
@@ -1044,7 +1088,10 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
       O = p.part + at_row * HD;
     } else if (p.lse && g == 0) p.lse[row[c] * p.n_heads + head[c]] = l == 0.f ? -INFINITY : (m_run[c] + log2f(l)) * 0.69314718055994530942f;
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4*>(O + dt * 16 + 4 * g) = o[c][dt] * inv;
+    for (int j = 0; j < HD / 64; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(O + f32_dim(4 * j, 4 * g + q)) = f32x4{o[c][4 * j][q], o[c][4 * j + 1][q], o[c][4 * j + 2][q], o[c][4 * j + 3][q]} * inv;
   }
 }
 
