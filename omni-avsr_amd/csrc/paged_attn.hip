@@ -2,7 +2,7 @@
 //
 // A kv head serves a group of G = n_heads / n_kv_heads query heads, so the (new token, head of the group) pairs of a sequence are the rows of one problem:
 // packed row r = token * G + head, all against the same keys and values, which a workgroup fetches once for its rows.  Softmax in one pass over the keys:
-// running maximum m, sum l and O, rescaled when m grows, in base 2 (scale * log2 e folded into the scores).
+// running maximum m (nearly), sum l and O, rescaled when m is raised, in base 2 (scale * log2 e folded into the scores).
 //
 // S^T = K Q^T and O^T = V^T P^T on 16x16 matrix instructions: a lane then owns one query column, its softmax is lane-local but for two exchanges, and the
 // accumulator registers of S^T are the B operand of the second product.
@@ -123,6 +123,17 @@ __device__ __forceinline__ float max_xor16_32(float x) {
   asm volatile("" : "+v"(y));
   const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
   return max_xor32(fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1])));
+}
+
+// The running maximum need not be the maximum: any number near it keeps the exponentials in range and cancels in O / l.  It is raised, and O and l rescaled,
+// only when some row's scores pass it by kSlack, so that probabilities stay below 2^8 at the same relative precision.  (With the exact maximum some
+// row of a wave finds a new one in nearly every of the first dozens of tiles, and each time all of O is multiplied.)
+constexpr float kSlack = 8.f;
+__device__ __forceinline__ float raise_max(float& m_run, float mt) {
+  const bool up = mt > m_run + kSlack;                 // of this row alone: a row's bits do not follow the wave's other rows
+  const float m_new = up ? mt : m_run, alpha = up ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.f;
+  m_run = m_new;
+  return alpha;
 }
 
 // Where 16-byte piece c of row r lies in an image of rows of RB bytes: c ^ swizzle.  Rows that one LDS access reads together fall into different banks.
@@ -347,8 +358,13 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
       }
     }
     mt = max_xor16_32(mt);
-    const float m_new = fmaxf(m_run, mt), m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+    if (__builtin_amdgcn_ballot_w64(mt > m_run + kSlack) != 0ull) {
+      const float alpha = raise_max(m_run, mt);
+      l_run *= alpha;
+#pragma unroll
+      for (int i = 0; i < NDT; ++i) o[i] *= alpha;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
     float sum = 0.f;
 #pragma unroll
     for (int kt = 0; kt < NSUB; ++kt) {
@@ -363,12 +379,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
         s[kt][i] = e;
       }
     }
-    l_run = l_run * alpha + sum;
-    m_run = m_new;
-    if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0ull) {
-#pragma unroll
-      for (int i = 0; i < NDT; ++i) o[i] *= alpha;
-    }
+    l_run += sum;
 
     // infinities and NaN among the values of an edge tile (of several new tokens: a later one's)
     bool odd = false;
@@ -689,14 +700,15 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttn
       for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[t2][e]);
     mt = max_xor32(mt);
     if constexpr (!F8) mt *= p.scale2;                 // scale > 0
-    const float m_new = fmaxf(m_run, mt), m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = __builtin_amdgcn_exp2f(m_run - m_use), nm = -m_use;
-    if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0ull) {
+    if (__builtin_amdgcn_ballot_w64(mt > m_run + kSlack) != 0ull) {
+      const float alpha = raise_max(m_run, mt);
+      l_run *= alpha;
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
     }
+    const float nm = m_run == -INFINITY ? 0.f : -m_run;
     bool odd = false;                                  // infinities or NaN among the values of a masked tile
     if constexpr (MASKED) {
       bool ok = true;
@@ -771,8 +783,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttn
         }
       }
     });
-    l_run = l_run * alpha + (sum[0] + sum[1]);
-    m_run = m_new;
+    l_run += sum[0] + sum[1];
   };
 
   int slot = 0;                                        // of tile t
@@ -995,8 +1006,13 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
         }
       }
       mt = max_xor16_32(mt);
-      const float m_new = fmaxf(m_run[c], mt), m_use = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = __builtin_amdgcn_exp2f(m_run[c] - m_use);
+      if (__builtin_amdgcn_ballot_w64(mt > m_run[c] + kSlack) != 0ull) {
+        const float alpha = raise_max(m_run[c], mt);
+        l_run[c] *= alpha;
+#pragma unroll
+        for (int i = 0; i < NDT; ++i) o[c][i] *= alpha;
+      }
+      const float m_use = m_run[c] == -INFINITY ? 0.f : m_run[c];
       float sum = 0.f;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
@@ -1011,12 +1027,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
           s[c][kt][i] = e;
         }
       }
-      l_run[c] = l_run[c] * alpha + sum;
-      m_run[c] = m_new;
-      if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0ull) {
-#pragma unroll
-        for (int i = 0; i < NDT; ++i) o[c][i] *= alpha;
-      }
+      l_run[c] += sum;
       if (MASKED && __builtin_expect(odd, 0)) {
         for (int k = 0; k < KT; ++k) {
           float e = 0.f;
