@@ -136,9 +136,11 @@ __device__ __forceinline__ float raise_max(float& m_run, float mt) {
   return alpha;
 }
 
-// Where 16-byte piece c of row r lies in an image of rows of RB bytes: c ^ swizzle.  Rows that one LDS access reads together fall into different banks.
+// Where 16-byte piece c of row r lies in an image of rows of RB bytes: c ^ swizzle.  LDS has 64 banks of 4 bytes, and serves 16 lanes of a 16-byte read at
+// a time (of 16 rows that differ mod 16) or 32 of an 8-byte transposing one (4 neighbouring rows, 64 bytes of each).  So 16 rows have to put one piece into 16
+// different places of 256 bytes, and 4 neighbouring rows their groups of four pieces into different quarters.
 template <int RB> __device__ __forceinline__ constexpr int swizzle(int row) {
-  return RB >= 256 ? (row & 7) << 1 : RB == 128 ? row & 7 : (row >> 2) & 3;
+  return RB >= 256 ? ((row & 3) << 2) | ((row >> 2) & 3) : RB == 128 ? ((row & 2) << 1) | ((row >> 2) & 3) : (row >> 2) & 3;
 }
 
 // A page's number by scalar load (the table is the kernel's to read only), checked.
@@ -166,28 +168,28 @@ __device__ __forceinline__ bf16x4 e4m3_to_bf16(unsigned w) {
   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true);
   return bf16x4{a[0], a[1], b[0], b[1]};                // exact
 }
-// Transposing reads of four (two) 16-column blocks, AT bytes behind the given addresses, waited for where they are made (the builtin makes the compiler wait for every LDS-DMA on its way first):
-// lane 4 q + p of 16 gives the address of columns 4 p .. of row q and gets rows 0 .. 3 of its own column.  b16: two row blocks, OFF bytes apart; b8: eight rows,
-// lane 2 q + h giving bytes 8 h .. of row q.
-template <int AT, int OFF>
-__device__ __forceinline__ void read_tr16_x4(const unsigned (&at)[4], u32x4 (&out)[4]) {
+// Transposing reads of four (two) 16-column blocks, waited for where they are made (the builtin makes the compiler wait for every LDS-DMA on its way
+// first): lane 4 q + p of 16 gives the address of columns 4 p .. of row q and gets rows 0 .. 3 of its own column.  b16: two blocks of rows, AT bytes behind
+// `at` and BT behind `bt`; b8: eight rows, lane 2 q + h giving bytes 8 h .. of row q.
+template <int AT, int BT>
+__device__ __forceinline__ void read_tr16_x4(const unsigned (&at)[4], const unsigned (&bt)[4], u32x4 (&out)[4]) {
   i32x2 a[4], b[4];
-  asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\tds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
-               "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\tds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+  asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%16\n\tds_read_b64_tr_b16 %1, %12 offset:%17\n\tds_read_b64_tr_b16 %2, %9 offset:%16\n\tds_read_b64_tr_b16 %3, %13 offset:%17\n\t"
+               "ds_read_b64_tr_b16 %4, %10 offset:%16\n\tds_read_b64_tr_b16 %5, %14 offset:%17\n\tds_read_b64_tr_b16 %6, %11 offset:%16\n\tds_read_b64_tr_b16 %7, %15 offset:%17\n\t"
                "s_waitcnt lgkmcnt(0)"
                : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1]), "=&v"(a[2]), "=&v"(b[2]), "=&v"(a[3]), "=&v"(b[3])
-               : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(AT), "n"(AT + OFF)
+               : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(bt[0]), "v"(bt[1]), "v"(bt[2]), "v"(bt[3]), "n"(AT), "n"(BT)
                : "memory");
 #pragma unroll
   for (int i = 0; i < 4; ++i) out[i] = u32x4{(unsigned)a[i][0], (unsigned)a[i][1], (unsigned)b[i][0], (unsigned)b[i][1]};
 }
-template <int AT, int OFF>
-__device__ __forceinline__ void read_tr16_x2(const unsigned (&at)[2], u32x4 (&out)[2]) {
+template <int AT, int BT>
+__device__ __forceinline__ void read_tr16_x2(const unsigned (&at)[2], const unsigned (&bt)[2], u32x4 (&out)[2]) {
   i32x2 a[2], b[2];
-  asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %4 offset:%7\n\tds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+  asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%8\n\tds_read_b64_tr_b16 %1, %6 offset:%9\n\tds_read_b64_tr_b16 %2, %5 offset:%8\n\tds_read_b64_tr_b16 %3, %7 offset:%9\n\t"
                "s_waitcnt lgkmcnt(0)"
                : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1])
-               : "v"(at[0]), "v"(at[1]), "n"(AT), "n"(AT + OFF)
+               : "v"(at[0]), "v"(at[1]), "v"(bt[0]), "v"(bt[1]), "n"(AT), "n"(BT)
                : "memory");
 #pragma unroll
   for (int i = 0; i < 2; ++i) out[i] = u32x4{(unsigned)a[i][0], (unsigned)a[i][1], (unsigned)b[i][0], (unsigned)b[i][1]};
@@ -219,7 +221,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
   using Sh = DecodeShape<T, F8, HD>;
   constexpr int KT = Sh::KT, RB = Sh::RB, IMG = Sh::IMG, STAGE = Sh::STAGE, NCH = RB / 16;
   constexpr int RPI = 1024 / RB, NI = IMG / 1024;      // rows per DMA instruction, instructions per image
-  constexpr int NSUB = KT / 16, NDT = HD / 16, NOFF = RPI >= 8 ? 1 : 8 / RPI;
+  constexpr int NSUB = KT / 16, NDT = HD / 16, NOFF = 16 / RPI;
   constexpr int VM = 2 * NI + (F8 ? 1 : 0);
   constexpr int RING = STAGE * NS > HD * 64 + 128 ? STAGE * NS : HD * 64 + 128;      // the ring, afterwards (m, l, O) of the wave
   static_assert(VM * (NS - 1) <= 63, "vmcnt");
@@ -422,7 +424,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
           u32x4 w[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) at[j] = vb + krow * RB + ((((d4 + j) * 2 + (pp >> 1)) ^ swizzle<RB>(krow)) << 4) + (pp & 1) * 8;
-          read_tr16_x4<0, 16 * RB>(at, w);
+          read_tr16_x4<0, 16 * RB>(at, at, w);
 #pragma unroll
           for (int j = 0; j < 4; ++j) vf[j] = __builtin_bit_cast(bf16x8, w[j]);
         }
@@ -638,7 +640,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttn
   for (int ds = 0; ds < NDS; ++ds) asm volatile("" : "+v"(qf[ds].v));      // waited for here, not in the loop
 
   // LDS offsets inside a stage.  K (A operand): row ql (+ 32), piece 2 ds + h.  V^T (transposing reads: 16 lanes fetch 4 rows x 16 columns): row 4 h + qq
-  // (+ 16 per step, + 8), piece 4 dt + 2 d16 + (pp >> 1); the row offsets are multiples of 8, which the swizzle does not see.
+  // (+ 16 per step, + 8), piece 4 dt + 2 d16 + (pp >> 1); of the row offsets the swizzle sees only the 8, as a bit of its own.
   unsigned kbase[NDS], vbase[NDT];
   {
     const unsigned s0 = lds_address(smem);
@@ -762,9 +764,9 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttn
         }
       }
     }
-    unsigned vat[NDT];
+    unsigned vat[NDT], vat8[NDT];
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) vat[dt] = vbase[dt] + so;
+    for (int dt = 0; dt < NDT; ++dt) { vat[dt] = vbase[dt] + so; vat8[dt] = vat[dt] ^ (swizzle<RB>(8) << 4); }
     static_for<0, 4>([&](auto ST) __attribute__((always_inline)) {
       constexpr int st = decltype(ST)::value, t2 = st / 2, sl = st & 1;      // 16 keys
       {
@@ -773,8 +775,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttn
 #pragma unroll
         for (int q = 0; q < 8; ++q) pf[q] = (bf16_t)s[t2][8 * sl + q];
         u32x4 w[NDT];
-        if constexpr (NDT == 4) read_tr16_x4<st * 16 * RB, 8 * RB>(vat, w);
-        else read_tr16_x2<st * 16 * RB, 8 * RB>(vat, w);
+        if constexpr (NDT == 4) read_tr16_x4<st * 16 * RB, (st * 16 + 8) * RB>(vat, vat8, w);
+        else read_tr16_x2<st * 16 * RB, (st * 16 + 8) * RB>(vat, vat8, w);
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
           bf16x8 vf = __builtin_bit_cast(bf16x8, w[dt]);
