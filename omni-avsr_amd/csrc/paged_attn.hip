@@ -533,10 +533,10 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
 // workgroups of one kv head then share an XCD (8 of them take the numbers in turn), and its L2 serves their common keys.
 // A wave skips the tiles none of its rows sees, and masks only those that some row sees in part.
 template <bool F8, int HD, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttnKArgs p) {
-  constexpr int ROWS = NW * 32, RB = HD * 2, IMG = KT * RB, NSTAGE = F8 || (HD == 128 && NW == 4) ? 2 : 3, STAGE = 2 * IMG + (F8 ? 2 * KT * 4 : 0);
-  constexpr int NCH = RB / 16, RPI = 1024 / RB, NSEG = IMG / 1024 / NW, NDS = HD / 16, NDT = HD / 32, VM = 2 * NSEG;
-  constexpr int FB = HD / NW, RW = KT / NW;            // 8 bits: bytes per thread, image and tile; rows per wave
+__global__ __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) void paged_chunk_kernel(const PagedAttnKArgs p) {
+  constexpr int ROWS = NW * 32, RB = HD * 2, IMG = KT * RB, NSTAGE = 2, STAGE = 2 * IMG + (F8 ? 2 * KT * 4 : 0);
+  constexpr int NDS = HD / 16, NDT = HD / 32;
+  constexpr int CB = F8 ? HD : RB, FB = CB / NW, RW = KT / NW, NC = FB < 16 ? 1 : FB / 16;      // bytes of a cached row, of them per thread; rows per wave; 16-byte loads
   __shared__ __attribute__((aligned(1024))) char smem[NSTAGE * STAGE];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ql = lane & 31, h = lane >> 5;
@@ -569,55 +569,58 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttn
   const char* Vb = reinterpret_cast<const char*>(p.kv.V);
   const int64_t page_bytes = p.kv.page_stride * (F8 ? 1 : 2);
   bool bad_page = false;
-  int page[NSEG];                                      // of the next tile to fetch
-  auto next_pages = [&](int kt0) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < NSEG; ++j) {
-      const int key = kt0 + (F8 ? wave * RW : (wave + NW * j) * RPI);
-      page[j] = -1;
-      if (key < kend) { page[j] = uniform_page(p, seq, key, shift); bad_page |= page[j] < 0; }
-    }
+  int page;                                            // of this wave's rows of the next tile to fetch
+  auto next_page = [&](int kt0) __attribute__((always_inline)) {
+    const int key = kt0 + wave * RW;
+    page = -1;
+    if (key < kend) { page = uniform_page(p, seq, key, shift); bad_page |= page < 0; }
   };
   const char* zero = reinterpret_cast<const char*>(kZeroRows);
-  // bf16: instruction (wave + 8 j) fills 1 KiB = RPI rows of an image
-  auto issue = [&](int kt0, int slot) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < NSEG; ++j) {
-      const int key = kt0 + (wave + NW * j) * RPI, lrow = (wave + NW * j) * RPI + lane / NCH;
-      const int off = (lane / NCH) * RB + (((lane % NCH) ^ swizzle<RB>(lrow)) << 4);
-      const int64_t at = (int64_t)page[j] * page_bytes + ((int64_t)kvh * p.kv.page_size + (key & pmask)) * RB;
-      const char *k = page[j] < 0 ? zero : Kb + at, *v = page[j] < 0 ? zero : Vb + at;
-      char* dst = smem + slot * STAGE + (wave + NW * j) * 1024;
-      if (kt0 + KT > kend && kt0 + lrow >= kend) { k = zero; v = zero; }      // behind the context: whatever the page holds must not meet a zero
-      __builtin_amdgcn_global_load_lds((global_ptr)(k + off), (lds_ptr)dst, 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((global_ptr)(v + off), (lds_ptr)(dst + IMG), 16, 0, 0);
-    }
-  };
-  // 8 bits: thread = FB bytes of a row of both images, NW threads a row; the first 2 RW lanes of a wave the scales of its rows
-  struct Raw { unsigned k[FB / 4], v[FB / 4]; float scale; };
+  // thread = FB bytes of a row of both images, NW threads a row; 8 bits: the first 2 RW lanes of a wave the scales of its rows
+  struct Raw { u32x4 k[NC], v[NC]; float scale; };
   auto fetch = [&](int kt0, Raw& x) __attribute__((always_inline)) {
     const int key = kt0 + wave * RW + lane / NW;
-    const bool ok = page[0] >= 0 && key < kend;
-    const int64_t tok_at = (int64_t)kvh * p.kv.page_size + (key & pmask);
-    const int64_t at = (int64_t)page[0] * page_bytes + tok_at * HD + (lane % NW) * FB;
+    const bool ok = page >= 0 && key < kend;
+    const int64_t at = (int64_t)page * page_bytes + ((int64_t)kvh * p.kv.page_size + (key & pmask)) * CB + (lane % NW) * (FB < 16 ? FB : 16);
     const char *k = ok ? Kb + at : zero, *v = ok ? Vb + at : zero;
-    __builtin_memcpy(x.k, __builtin_assume_aligned(k, FB < 16 ? FB : 16), FB);
-    __builtin_memcpy(x.v, __builtin_assume_aligned(v, FB < 16 ? FB : 16), FB);
-    const int skey = kt0 + wave * RW + lane % RW;
-    const int64_t sat = (int64_t)page[0] * p.kv.scale_stride + (int64_t)kvh * p.kv.page_size + (skey & pmask);
-    const float* sp = page[0] >= 0 && skey < kend ? ((lane & RW) ? p.kv.v_scale : p.kv.k_scale) + sat : reinterpret_cast<const float*>(zero);
-    x.scale = *sp;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if constexpr (FB < 16) {
+        const uint2 a = *reinterpret_cast<const uint2*>(k), b = *reinterpret_cast<const uint2*>(v);
+        x.k[c] = u32x4{a.x, a.y, 0u, 0u};
+        x.v[c] = u32x4{b.x, b.y, 0u, 0u};
+      } else {
+        x.k[c] = *reinterpret_cast<const u32x4*>(k + c * NW * 16);
+        x.v[c] = *reinterpret_cast<const u32x4*>(v + c * NW * 16);
+      }
+    }
+    if constexpr (F8) {
+      const int skey = kt0 + wave * RW + lane % RW;
+      const int64_t sat = (int64_t)page * p.kv.scale_stride + (int64_t)kvh * p.kv.page_size + (skey & pmask);
+      const float* sp = page >= 0 && skey < kend ? ((lane & RW) ? p.kv.v_scale : p.kv.k_scale) + sat : reinterpret_cast<const float*>(zero);
+      x.scale = *sp;
+    }
   };
-  auto widen = [&](const Raw& x, int slot) __attribute__((always_inline)) {
+  auto store = [&](const Raw& x, int slot) __attribute__((always_inline)) {
     char* dst = smem + slot * STAGE;
     const int lrow = wave * RW + lane / NW;
+    auto put = [&](char* img, int c, u32x4 w) { *reinterpret_cast<u32x4*>(img + lrow * RB + ((c ^ swizzle<RB>(lrow)) << 4)) = w; };
 #pragma unroll
-    for (int c = 0; c < FB / 8; ++c) {
-      const int at = lrow * RB + ((((lane % NW) * (FB / 8) + c) ^ swizzle<RB>(lrow)) << 4);
-      *reinterpret_cast<bf16x8*>(dst + at) = join(e4m3_to_bf16(x.k[2 * c]), e4m3_to_bf16(x.k[2 * c + 1]));
-      *reinterpret_cast<bf16x8*>(dst + IMG + at) = join(e4m3_to_bf16(x.v[2 * c]), e4m3_to_bf16(x.v[2 * c + 1]));
+    for (int c = 0; c < NC; ++c) {
+      const int at = lane % NW + c * NW;
+      if constexpr (F8) {
+#pragma unroll
+        for (int w = 0; w < (FB < 16 ? 1 : 2); ++w) {
+          const int to = FB < 16 ? at : 2 * at + w;
+          put(dst, to, __builtin_bit_cast(u32x4, join(e4m3_to_bf16(x.k[c][2 * w]), e4m3_to_bf16(x.k[c][2 * w + 1]))));
+          put(dst + IMG, to, __builtin_bit_cast(u32x4, join(e4m3_to_bf16(x.v[c][2 * w]), e4m3_to_bf16(x.v[c][2 * w + 1]))));
+        }
+      } else {
+        put(dst, at, x.k[c]);
+        put(dst + IMG, at, x.v[c]);
+      }
     }
-    if (lane < 2 * RW) reinterpret_cast<float*>(dst + 2 * IMG)[((lane & RW) ? KT : 0) + wave * RW + lane % RW] = (lane & RW) ? x.scale : x.scale * p.scale2;
+    if (F8 && lane < 2 * RW) reinterpret_cast<float*>(dst + 2 * IMG)[((lane & RW) ? KT : 0) + wave * RW + lane % RW] = (lane & RW) ? x.scale : x.scale * p.scale2;
   };
 
   // Q^T fragments (B operand: lane = row ql, k-group h): step ds covers d = 16 ds + 8 h .. + 7
@@ -628,14 +631,9 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttn
     for (int ds = 0; ds < NDS; ++ds) qf[ds] = *reinterpret_cast<const Chunk16*>(qp + ds * 32 + h * 16);
   }
   Raw raw;
-  next_pages(kbeg);
-  if constexpr (F8) {
-    if (ntile > 0) { fetch(kbeg, raw); next_pages(kbeg + KT); widen(raw, 0); }
-    if (ntile > 1) { fetch(kbeg + KT, raw); next_pages(kbeg + 2 * KT); }
-  } else {
-    if (ntile > 0) { issue(kbeg, 0); next_pages(kbeg + KT); }
-    if (NSTAGE == 3 && ntile > 1) { issue(kbeg + KT, 1); next_pages(kbeg + 2 * KT); }
-  }
+  next_page(kbeg);
+  if (ntile > 0) { fetch(kbeg, raw); next_page(kbeg + KT); store(raw, 0); }
+  if (ntile > 1) { fetch(kbeg + KT, raw); next_page(kbeg + 2 * KT); }
 #pragma unroll
   for (int ds = 0; ds < NDS; ++ds) asm volatile("" : "+v"(qf[ds].v));      // waited for here, not in the loop
 
@@ -767,19 +765,27 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttn
     unsigned vat[NDT], vat8[NDT];
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) { vat[dt] = vbase[dt] + so; vat8[dt] = vat[dt] ^ (swizzle<RB>(8) << 4); }
-    static_for<0, 4>([&](auto ST) __attribute__((always_inline)) {
-      constexpr int st = decltype(ST)::value, t2 = st / 2, sl = st & 1;      // 16 keys
-      {
-        if constexpr (!MASKED && sl == 0) weights(std::integral_constant<int, t2>{});
+    static_for<0, 2>([&](auto T2) __attribute__((always_inline)) {
+      constexpr int t2 = decltype(T2)::value;
+      // the values of 32 keys are on their way while the weights are formed
+      s16x4 va[2][NDT], vb[2][NDT];
+#pragma unroll
+      for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) {
+          va[sl][dt] = __builtin_bit_cast(s16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vat[dt] + (2 * t2 + sl) * 16 * RB)));
+          vb[sl][dt] = __builtin_bit_cast(s16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vat8[dt] + ((2 * t2 + sl) * 16 + 8) * RB)));
+        }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (!MASKED) weights(T2);
+#pragma unroll
+      for (int sl = 0; sl < 2; ++sl) {
         bf16x8 pf;
 #pragma unroll
         for (int q = 0; q < 8; ++q) pf[q] = (bf16_t)s[t2][8 * sl + q];
-        u32x4 w[NDT];
-        if constexpr (NDT == 4) read_tr16_x4<st * 16 * RB, (st * 16 + 8) * RB>(vat, vat8, w);
-        else read_tr16_x2<st * 16 * RB, (st * 16 + 8) * RB>(vat, vat8, w);
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
-          bf16x8 vf = __builtin_bit_cast(bf16x8, w[dt]);
+          bf16x8 vf = join(__builtin_bit_cast(bf16x4, va[sl][dt]), __builtin_bit_cast(bf16x4, vb[sl][dt]));
           if (MASKED && odd) vf = finite_part(vf);
           o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o[dt], 0, 0, 0);
         }
@@ -791,22 +797,11 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttn
   int slot = 0;                                        // of tile t
   auto tile = [&](int t, auto masked_tag) __attribute__((always_inline)) {
     const int kt0 = kbeg + t * KT;
-    if constexpr (F8) {
-      __syncthreads();
-      if (t + 1 < ntile) widen(raw, 1 - slot);         // (that slot held tile t - 1: every wave is past it)
-      if (t + 2 < ntile) { fetch(kt0 + 2 * KT, raw); next_pages(kt0 + 3 * KT); }
-    } else {
-      // tile t has landed once only tile t + 1's instructions of this wave are on their way
-      if (NSTAGE == 3 && t + 1 < ntile) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(VM) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      constexpr int AHEAD = NSTAGE - 1;
-      if (t + AHEAD < ntile) { issue(kt0 + AHEAD * KT, slot == 0 ? AHEAD : slot - 1); next_pages(kt0 + (AHEAD + 1) * KT); }      // (that slot held tile t - 1)
-    }
+    __syncthreads();
+    if (t + 1 < ntile) store(raw, 1 - slot);           // (that slot held tile t - 1: every wave is past it)
+    if (t + 2 < ntile) { fetch(kt0 + 2 * KT, raw); next_page(kt0 + 3 * KT); }
     if (!decltype(masked_tag)::value || kt0 < see_max) compute(kt0, slot * STAGE, masked_tag);
     slot = slot == NSTAGE - 1 ? 0 : slot + 1;
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // this wave has read the tile when it meets the next barrier
   };
   // two loops, each with one body: as two branches of one loop the bodies' accumulators met in copies of all of them
   const int t_full = rows_here ? min(ntile, max(0, see_min - kbeg) / KT) : 0;
@@ -845,9 +840,6 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttn
     }
 }
 
-#ifndef F32_NC
-#define F32_NC 1
-#endif
 // ---- many rows per sequence, f32 ---------------------------------------------------------------------------------------------------------------
 //
 // The exact-f32 mode: a workgroup of 4 waves takes 64 packed rows, 16 per wave, on 16x16x4 matrix instructions, which bound it (32 cycles for 2048 flop;
@@ -855,7 +847,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_chunk_kernel(const PagedAttn
 // cached bytes: 8-bit ones are widened where they are read.
 template <bool F8, int HD>
 __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnKArgs p) {
-  constexpr int NW = 4, NC = F32_NC, ROWS = NW * 16 * NC, KT = 32, RB = HD * (F8 ? 1 : 4), IMG = KT * RB, STAGE = 2 * IMG + (F8 ? 256 : 0), NSTAGE = STAGE > 16 * 1024 ? 2 : 4;
+  constexpr int NW = 4, ROWS = NW * 16, KT = 32, RB = HD * (F8 ? 1 : 4), IMG = KT * RB, STAGE = 2 * IMG + (F8 ? 256 : 0), NSTAGE = STAGE > 16 * 1024 ? 2 : 4;
   constexpr int NCH = RB / 16, RPI = 1024 / RB, NI = IMG / 1024, NSEG = 2 * NI / NW, VM = NSEG + (F8 ? 1 : 0), NDT = HD / 16, NQ = HD / (F8 ? 64 : 16);
   __shared__ __attribute__((aligned(1024))) char smem[NSTAGE * STAGE];
 
@@ -875,24 +867,17 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
   const int kend = p.split ? min(kend_all, kbeg + p.split) : kend_all;
   const int ntile = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
 
-  const int w0 = r0 + wave * 16 * NC;
+  const int w0 = r0 + wave * 16;
   const bool rows_here = w0 < packed;
-  const int see_min = min(first_pos + min(w0, packed - 1) / G + 1, kmax), see_max = rows_here ? min(first_pos + min(w0 + 16 * NC - 1, packed - 1) / G + 1, kmax) : 0;
-  int see[NC], head[NC];
-  int64_t row[NC];
-  Chunk16 qf[NC][NQ][F8 ? 4 : 1];
+  const int see_min = min(first_pos + min(w0, packed - 1) / G + 1, kmax), see_max = rows_here ? min(first_pos + min(w0 + 15, packed - 1) / G + 1, kmax) : 0;
+  const int rc = min(w0 + qi, packed - 1), tok = rc / G, head = kvh * G + (rc - tok * G), see = min(first_pos + tok + 1, kmax);
+  const int64_t row = sq.q0 + tok;
+  Chunk16 qf[NQ][F8 ? 4 : 1];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int rc = min(w0 + c * 16 + qi, packed - 1), tok = rc / G;
-    head[c] = kvh * G + (rc - tok * G);
-    row[c] = sq.q0 + tok;
-    see[c] = min(first_pos + tok + 1, kmax);
-    const float* qp = reinterpret_cast<const float*>(p.Q) + row[c] * p.ldq + (int64_t)head[c] * HD;
+  for (int b = 0; b < NQ; ++b)
 #pragma unroll
-    for (int b = 0; b < NQ; ++b)
-#pragma unroll
-      for (int e = 0; e < (F8 ? 4 : 1); ++e) qf[c][b][e] = reinterpret_cast<const Chunk16*>(qp)[(b * 4 + g) * (F8 ? 4 : 1) + e];
-  }
+    for (int e = 0; e < (F8 ? 4 : 1); ++e)
+      qf[b][e] = reinterpret_cast<const Chunk16*>(reinterpret_cast<const float*>(p.Q) + row * p.ldq + (int64_t)head * HD)[(b * 4 + g) * (F8 ? 4 : 1) + e];
 
   const int shift = page_shift_of(p.kv), pmask = p.kv.page_size - 1;
   const int64_t page_bytes = p.kv.page_stride * (F8 ? 1 : 4);
@@ -930,30 +915,22 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
   for (int i = 0; i < NSTAGE - 1; ++i)
     if (i < ntile) issue(kbeg + i * KT, i);
 #pragma unroll
-  for (int c = 0; c < NC; ++c)
+  for (int b = 0; b < NQ; ++b)
 #pragma unroll
-    for (int b = 0; b < NQ; ++b)
-#pragma unroll
-      for (int e = 0; e < (F8 ? 4 : 1); ++e) asm volatile("" : "+v"(qf[c][b][e].v));      // waited for here, not in the loop
+    for (int e = 0; e < (F8 ? 4 : 1); ++e) asm volatile("" : "+v"(qf[b][e].v));      // waited for here, not in the loop
 
-  f32x4 o[NC][NDT];
-  float m_run[NC], l_run[NC];
+  f32x4 o[NDT];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    m_run[c] = -INFINITY;
-    l_run[c] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NDT; ++i) o[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int i = 0; i < NDT; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m_run = -INFINITY, l_run = 0.f;
 
   auto compute = [&](int kt0, const char* sK, auto masked_tag) __attribute__((always_inline)) {
     constexpr bool MASKED = decltype(masked_tag)::value;
     const char* sV = sK + IMG;
     const float* sc = reinterpret_cast<const float*>(sK + 2 * IMG);
 
-    f32x4 s[NC][2];
-#pragma unroll
-    for (int c = 0; c < NC; ++c) s[c][0] = s[c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 s[2];
+    s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int b = 0; b < NQ; ++b) {
       Chunk16 kc[2];
@@ -971,8 +948,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
         for (int e = 0; e < 4; ++e)
 #pragma unroll
           for (int kt = 0; kt < 2; ++kt)              // chains of products that do not wait for each other
-#pragma unroll
-            for (int c = 0; c < NC; ++c) s[c][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[kt][e], __builtin_bit_cast(f32x4, qf[c][b][w].v)[e], s[c][kt], 0, 0, 0);
+            s[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[kt][e], __builtin_bit_cast(f32x4, qf[b][w].v)[e], s[kt], 0, 0, 0);
       }
     }
     auto v_at = [&](int krow, int d) -> float {
@@ -992,63 +968,60 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
       }
       odd = __builtin_amdgcn_ballot_w64(!ok) != 0ull;
     }
+    float mt = -INFINITY;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      float mt = -INFINITY;
+    for (int kt = 0; kt < 2; ++kt) {
+      f32x4 ks = f32x4{p.scale2, p.scale2, p.scale2, p.scale2};
+      if constexpr (F8) ks *= *reinterpret_cast<const f32x4*>(sc + kt * 16 + 4 * g);
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        f32x4 ks = f32x4{p.scale2, p.scale2, p.scale2, p.scale2};
-        if constexpr (F8) ks *= *reinterpret_cast<const f32x4*>(sc + kt * 16 + 4 * g);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float v = s[c][kt][i] * ks[i];
-          if (MASKED && kt0 + kt * 16 + 4 * g + i >= see[c]) v = -INFINITY;
-          s[c][kt][i] = v;
-          mt = fmaxf(mt, v);
-        }
+      for (int i = 0; i < 4; ++i) {
+        float v = s[kt][i] * ks[i];
+        if (MASKED && kt0 + kt * 16 + 4 * g + i >= see) v = -INFINITY;
+        s[kt][i] = v;
+        mt = fmaxf(mt, v);
       }
-      mt = max_xor16_32(mt);
-      if (__builtin_amdgcn_ballot_w64(mt > m_run[c] + kSlack) != 0ull) {
-        const float alpha = raise_max(m_run[c], mt);
-        l_run[c] *= alpha;
+    }
+    mt = max_xor16_32(mt);
+    if (__builtin_amdgcn_ballot_w64(mt > m_run + kSlack) != 0ull) {
+      const float alpha = raise_max(m_run, mt);
+      l_run *= alpha;
 #pragma unroll
-        for (int i = 0; i < NDT; ++i) o[c][i] *= alpha;
+      for (int i = 0; i < NDT; ++i) o[i] *= alpha;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    float sum = 0.f;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      f32x4 vs = f32x4{1.f, 1.f, 1.f, 1.f};
+      if constexpr (F8) vs = *reinterpret_cast<const f32x4*>(sc + 32 + kt * 16 + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float e = __builtin_amdgcn_exp2f(s[kt][i] - m_use);
+        sum += e;
+        if constexpr (F8) e *= vs[i];
+        if (MASKED && kt0 + kt * 16 + 4 * g + i >= see) e = 0.f;
+        s[kt][i] = e;
       }
-      const float m_use = m_run[c] == -INFINITY ? 0.f : m_run[c];
-      float sum = 0.f;
+    }
+    l_run += sum;
+    if (MASKED && __builtin_expect(odd, 0)) {
+      for (int k = 0; k < KT; ++k) {
+        float e = 0.f;
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        f32x4 vs = f32x4{1.f, 1.f, 1.f, 1.f};
-        if constexpr (F8) vs = *reinterpret_cast<const f32x4*>(sc + 32 + kt * 16 + 4 * g);
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float e = __builtin_amdgcn_exp2f(s[c][kt][i] - m_use);
-          sum += e;
-          if constexpr (F8) e *= vs[i];
-          if (MASKED && kt0 + kt * 16 + 4 * g + i >= see[c]) e = 0.f;
-          s[c][kt][i] = e;
-        }
-      }
-      l_run[c] += sum;
-      if (MASKED && __builtin_expect(odd, 0)) {
-        for (int k = 0; k < KT; ++k) {
-          float e = 0.f;
+          for (int i = 0; i < 4; ++i)
+            if ((k & 3) == i && (k >> 4) == kt) e = s[kt][i];
+        e = __shfl(e, ((k >> 2) & 3) * 16 + qi, 64);
+        if (kt0 + k < see)
 #pragma unroll
-          for (int kt = 0; kt < 2; ++kt)
+          for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if ((k & 3) == i && (k >> 4) == kt) e = s[c][kt][i];
-          e = __shfl(e, ((k >> 2) & 3) * 16 + qi, 64);
-          if (kt0 + k < see[c])
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const float vv = v_at(k, f32_dim(dt, 4 * g + q));
-                if (!is_finite(vv)) o[c][dt][q] += e * vv;
-                if (q & 1) asm volatile("" ::: "memory");
-              }
-        }
+            for (int q = 0; q < 4; ++q) {
+              const float vv = v_at(k, f32_dim(dt, 4 * g + q));
+              if (!is_finite(vv)) o[dt][q] += e * vv;
+              if (q & 1) asm volatile("" ::: "memory");
+            }
       }
     }
 #pragma unroll
@@ -1062,8 +1035,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             if (MASKED && odd && !is_finite(vv[w])) vv[w] = 0.f;
-#pragma unroll
-            for (int c = 0; c < NC; ++c) o[c][4 * j + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[w], s[c][kt][i], o[c][4 * j + w], 0, 0, 0);
+            o[4 * j + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[w], s[kt][i], o[4 * j + w], 0, 0, 0);
           }
         }
   };
@@ -1085,27 +1057,23 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
   for (; t < ntile; ++t) tile(t, std::true_type{});
   if (bad_page && lane == 0) paged_report(p.kv.status, kBadPage);
 
+  if (w0 + qi >= packed) return;
+  float l = l_run;
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int n = splits_of(p, see);
+  if (split >= n) return;
+  float* O = reinterpret_cast<float*>(p.O) + row * p.ldo + (int64_t)head * HD;
+  if (n > 1) {
+    const int64_t at_row = ((int64_t)split * p.b.rows + row) * p.n_heads + head;
+    if (g == 0) p.part_ml[at_row] = make_float2(m_run, l);
+    O = p.part + at_row * HD;
+  } else if (p.lse && g == 0) p.lse[row * p.n_heads + head] = l == 0.f ? -INFINITY : (m_run + log2f(l)) * 0.69314718055994530942f;
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    if (w0 + c * 16 + qi >= packed) continue;
-    float l = l_run[c];
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int n = splits_of(p, see[c]);
-    if (split >= n) continue;
-    float* O = reinterpret_cast<float*>(p.O) + row[c] * p.ldo + (int64_t)head[c] * HD;
-    if (n > 1) {
-      const int64_t at_row = ((int64_t)split * p.b.rows + row[c]) * p.n_heads + head[c];
-      if (g == 0) p.part_ml[at_row] = make_float2(m_run[c], l);
-      O = p.part + at_row * HD;
-    } else if (p.lse && g == 0) p.lse[row[c] * p.n_heads + head[c]] = l == 0.f ? -INFINITY : (m_run[c] + log2f(l)) * 0.69314718055994530942f;
+  for (int j = 0; j < HD / 64; ++j)
 #pragma unroll
-    for (int j = 0; j < HD / 64; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<f32x4*>(O + f32_dim(4 * j, 4 * g + q)) = f32x4{o[c][4 * j][q], o[c][4 * j + 1][q], o[c][4 * j + 2][q], o[c][4 * j + 3][q]} * inv;
-  }
+    for (int q = 0; q < 4; ++q) *reinterpret_cast<f32x4*>(O + f32_dim(4 * j, 4 * g + q)) = f32x4{o[4 * j][q], o[4 * j + 1][q], o[4 * j + 2][q], o[4 * j + 3][q]} * inv;
 }
 
 // Joins the splits of the rows whose keys lie in more than one:  out = sum_z w_z O_z / sum_z w_z,  w_z = l_z 2^(m_z - max m).  NG groups of HD / 4 threads share
@@ -1180,8 +1148,10 @@ int cu_count() {
 //           tokens, where keys are fetched once per 256 rows and few tiles are cut by the diagonal (2048 new tokens over 16384, 32 / 8 heads: 582 us against
 //           628; a prompt of 8192 alone: 746 against 734).
 //   split   keys per workgroup.  Single tokens: as many splits as give two rounds of workgroups, rounded down where there are many (131072 keys of 3
-//           sequences: 40 splits fill 1.9 rounds, 161 us; 43 begin a third, 193) and up where there are few.  Chunks: an even batch only up to
-//           one round, a ragged one two, since its longest sequence else runs on alone (24 sequences, 5 of them chunks of up to 701: 87 us, unsplit 145).
+//           sequences: 40 splits fill 1.9 rounds, 161 us; 43 begin a third, 193) and up where there are few.  Chunks of an even batch: the number
+//           that leaves the last round fullest, a round being worth more than 3 % a split (1024 new tokens over 32768, 40 / 8 heads, 160 workgroups: XXX us,
+//           unsplit 872).  A ragged one: two rounds, since its longest sequence else runs on alone (24 sequences, 5 of them chunks of up to 701: 83 us,
+//           unsplit 128).
 struct Plan { int64_t tiles; int split, splits, nw; bool decode; };
 Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
   Plan pl;
@@ -1190,7 +1160,8 @@ Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
   const bool even = b.rows >= (int64_t)b.n_seqs * b.max_q;      // all sequences bring max_q tokens
   pl.decode = (int64_t)b.max_q * G <= 16;
   pl.nw = !pl.decode && kv.dtype == DT_BF16 && kv.head_dim == 128 && even && b.max_ctx >= 4ll * b.max_q ? 8 : 4;
-  pl.tiles = pl.decode ? b.n_seqs : packed / (kv.dtype == DT_F32 ? 64 * F32_NC : 32 * pl.nw) + b.n_seqs;
+  const int rows = kv.dtype == DT_F32 ? 64 : 32 * pl.nw;
+  pl.tiles = pl.decode ? b.n_seqs : std::min<int64_t>(packed / rows + b.n_seqs, b.n_seqs * ceil_div64((int64_t)b.max_q * G, rows));
   const int64_t wgs = std::max<int64_t>(1, pl.tiles * kv.n_kv_heads);
   const int64_t slots = (int64_t)cus * (pl.nw == 8 ? 1 : 2);      // workgroups side by side
   pl.split = a.split_keys;
@@ -1198,7 +1169,15 @@ Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
     if (pl.decode && wgs <= cus && b.max_ctx <= 1024) pl.split = 1024;
     else {
       const int64_t down = 2 * slots / wgs, up = ceil_div64(2 * slots, wgs);
-      const int64_t n = pl.decode ? (down >= 8 ? down : up) : even ? slots / wgs : up;
+      int64_t n = pl.decode ? (down >= 8 ? down : up) : up;
+      if (!pl.decode && even) {
+        double best = 1e30;
+        n = 1;
+        for (int i = 1; i <= 32; ++i) {
+          const double cost = (double)ceil_div64(wgs * i, slots) / i + 0.03 * (i - 1);
+          if (cost < best) best = cost, n = i;
+        }
+      }
       pl.split = (int)std::max<int64_t>(512, ceil_div64(ceil_div64(b.max_ctx, std::max<int64_t>(1, n)), 256) * 256);
     }
   }
