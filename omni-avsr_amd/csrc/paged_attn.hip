@@ -403,9 +403,13 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
     }
 
     if constexpr (sizeof(T) == 2) {
-      bf16x8 pf;
+      bf16x8 pf, pl;                                   // the weights as a sum of two numbers: one rounding of them less, and products are not what is short here
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { pf[i] = (bf16_t)s[0][i]; pf[4 + i] = (bf16_t)s[1][i]; }
+      for (int i = 0; i < 8; ++i) {
+        const float e = s[i >> 2][i & 3];
+        pf[i] = (bf16_t)e;
+        pl[i] = (bf16_t)(e - (float)pf[i]);
+      }
       const unsigned vb = lds_address(sV);
 #pragma unroll
       for (int d4 = 0; d4 < NDT; d4 += 4) {
@@ -432,6 +436,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
         for (int j = 0; j < 4; ++j) {
           if (MASKED && odd) vf[j] = finite_part(vf[j]);
           o[d4 + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[j], pf, o[d4 + j], 0, 0, 0);
+          o[d4 + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[j], pl, o[d4 + j], 0, 0, 0);
         }
       }
     } else {
@@ -1149,7 +1154,7 @@ int cu_count() {
 //           628; a prompt of 8192 alone: 746 against 734).
 //   split   keys per workgroup.  Single tokens: as many splits as give two rounds of workgroups, rounded down where there are many (131072 keys of 3
 //           sequences: 40 splits fill 1.9 rounds, 161 us; 43 begin a third, 193) and up where there are few.  Chunks of an even batch: the number
-//           that leaves the last round fullest, a round being worth more than 3 % a split (1024 new tokens over 32768, 40 / 8 heads, 160 workgroups: XXX us,
+//           that leaves the last round fullest, a round being worth more than 3 % a split (1024 new tokens over 32768, 40 / 8 heads, 160 workgroups: 707 us,
 //           unsplit 872).  A ragged one: two rounds, since its longest sequence else runs on alone (24 sequences, 5 of them chunks of up to 701: 83 us,
 //           unsplit 128).
 struct Plan { int64_t tiles; int split, splits, nw; bool decode; };
