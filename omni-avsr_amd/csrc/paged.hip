@@ -15,11 +15,18 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
 
+// 16 bytes that the kernel reads once (non-temporal: norm + rotation of 16384 rows of 32 + 8 heads x 128 58.5 us, 5.7 TB/s; 68.9 without the hint.  The
+// same hint on its stores costs 8 %.)
+__device__ __forceinline__ Chunk16 load_once(const void* p) {
+  Chunk16 c;
+  c.v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+  return c;
+}
 template <typename T> __device__ __forceinline__ void load8(const T* p, float* x);
-template <> __device__ __forceinline__ void load8<bf16_t>(const bf16_t* p, float* x) { chunk_to_f32<bf16_t>(*reinterpret_cast<const Chunk16*>(p), x); }
+template <> __device__ __forceinline__ void load8<bf16_t>(const bf16_t* p, float* x) { chunk_to_f32<bf16_t>(load_once(p), x); }
 template <> __device__ __forceinline__ void load8<float>(const float* p, float* x) {
-  chunk_to_f32<float>(*reinterpret_cast<const Chunk16*>(p), x);
-  chunk_to_f32<float>(*reinterpret_cast<const Chunk16*>(p + 4), x + 4);
+  chunk_to_f32<float>(load_once(p), x);
+  chunk_to_f32<float>(load_once(p + 4), x + 4);
 }
 template <typename T> __device__ __forceinline__ void store8(T* p, const float* x);
 template <> __device__ __forceinline__ void store8<bf16_t>(bf16_t* p, const float* x) { *reinterpret_cast<Chunk16*>(p) = chunk_from_f32<bf16_t>(x); }
@@ -111,11 +118,12 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(const QkRopeArgs p, c
         for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor(ss, o, 64);
         const float r = 1.f / sqrtf(ss * (1.f / HD) + p.eps);
         const float* gain = is_q ? p.q_gain : p.k_gain;
-        float g[16];
-        load8<float>(gain + e0, g);
-        load8<float>(gain + e1, g + 8);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = x[i] * r * g[i];
+        for (int i = 0; i < 16; i += 4) {
+          const f32x4 g = *reinterpret_cast<const f32x4*>(gain + (i < 8 ? e0 + i : e1 + i - 8));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[i + j] = x[i + j] * r * g[j];
+        }
       }
       if (c < rl) {
         if (p.interleaved) {
@@ -214,9 +222,10 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(const PagedKv kv, 
       const int64_t tok = (int64_t)kh * kv.page_size + off;
       const void* base = is_v ? kv.V : kv.K;
       if constexpr (F8) {
-        const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(base) + (int64_t)page * kv.page_stride + tok * HD + 16 * c);
+        const u32x4 w = load_once(reinterpret_cast<const char*>(base) + (int64_t)page * kv.page_stride + tok * HD + 16 * c).v;
         const float scale = (is_v ? kv.v_scale : kv.k_scale)[(int64_t)page * kv.scale_stride + tok];
-        e4m3_to_f32(w.x, x); e4m3_to_f32(w.y, x + 4); e4m3_to_f32(w.z, x + 8); e4m3_to_f32(w.w, x + 12);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e4m3_to_f32(w[i], x + 4 * i);
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] *= scale;
       } else {

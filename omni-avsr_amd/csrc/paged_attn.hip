@@ -209,7 +209,9 @@ __device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) { return bf16x8{a[0],
 // A workgroup per (sequence, kv head, split of its keys) whose packed rows are the <= 16 columns of the matrix instructions.  HBM bound: 2 G flop per byte
 // of a bf16 cache.  Each wave streams its own tiles of KT keys (wave, wave + NW, ...) through a private ring of NS tiles in LDS, fetched by LDS-DMA and
 // awaited by counted vmcnt, so there is no barrier in the loop and (NS - 1) tiles are on their way while one is computed.  16 keys lie in one page, so
-// an instruction's page is uniform: scalar loads, one page base per 16 keys.  The waves' (m, l, O) meet in LDS in wave order.
+// an instruction's page is uniform: scalar loads, one page base per 16 keys.  The waves' (m, l, O) meet in LDS in wave order.  The cache is read once and
+// the loads say so (non-temporal): 691 MB of 97 sequences 124 us, 5.6 TB/s with the join; 143 without the hint.
+constexpr int kOnce = 2;                              // nt of a load to LDS
 template <typename T, bool F8, int HD> struct DecodeShape {
   static constexpr int KT = sizeof(T) == 4 ? 16 : 32;                        // keys per wave tile
   static constexpr int RB = HD * (F8 ? 1 : (int)sizeof(T));                  // bytes of a cached row
@@ -228,15 +230,15 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
   __shared__ __attribute__((aligned(1024))) char smem[NW * RING];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), qi = lane & 15, g = lane >> 4;
-  const int seq = blockIdx.x, kvh = blockIdx.y, G = p.group;
+  const int G = p.group, KV = p.kv.n_kv_heads, kvh = blockIdx.x % KV, unit = blockIdx.x / KV, split = unit / p.tiles, seq = unit - split * p.tiles;
   const SeqInfo sq = paged_seq(p.b, seq);
   if (sq.bad && tid == 0) paged_report(p.kv.status, kBadLength);
   const int packed = sq.nq * G;
   if (packed == 0) return;
   const int first_pos = sq.ctx - sq.nq, kmax = min(sq.ctx, p.b.max_ctx);
   const int kend_all = max(0, min(first_pos + sq.nq, kmax));
-  const int kbeg = p.split ? (int)blockIdx.z * p.split : 0;
-  if (blockIdx.z > 0 && kbeg >= kend_all) return;
+  const int kbeg = p.split ? split * p.split : 0;
+  if (split > 0 && kbeg >= kend_all) return;
   const int kend = p.split ? min(kend_all, kbeg + p.split) : kend_all;
   char* ring = smem + wave * RING;
 
@@ -267,8 +269,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
       const int64_t at = (int64_t)page[j] * page_bytes + ((int64_t)kvh * p.kv.page_size + (key & (p.kv.page_size - 1)) + (i * RPI) % 16) * RB;
       const char* k = page[j] < 0 ? reinterpret_cast<const char*>(kZeroRows) : Kb + at;
       const char* v = page[j] < 0 ? reinterpret_cast<const char*>(kZeroRows) : Vb + at;
-      __builtin_amdgcn_global_load_lds((global_ptr)(k + loff[i % NOFF]), (lds_ptr)(dst + i * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((global_ptr)(v + loff[i % NOFF]), (lds_ptr)(dst + IMG + i * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((global_ptr)(k + loff[i % NOFF]), (lds_ptr)(dst + i * 1024), 16, 0, kOnce);
+      __builtin_amdgcn_global_load_lds((global_ptr)(v + loff[i % NOFF]), (lds_ptr)(dst + IMG + i * 1024), 16, 0, kOnce);
     }
     if constexpr (F8) {                                // lanes 0 .. KT - 1: the keys' scales, then the values'
       const int l = lane & (2 * KT - 1), key = kt0 + (l & (KT - 1));
@@ -515,9 +517,9 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int64_t prow = sq.q0 + ptok;
     const int n = splits_of(p, min(first_pos + ptok + 1, kmax));
-    if ((int)blockIdx.z >= n) continue;
+    if (split >= n) continue;
     if (n > 1) {
-      const int64_t at = ((int64_t)blockIdx.z * p.b.rows + prow) * p.n_heads + phead;
+      const int64_t at = ((int64_t)split * p.b.rows + prow) * p.n_heads + phead;
       if (d0 == 0) p.part_ml[at] = make_float2(m, l);
       *reinterpret_cast<f32x4*>(p.part + at * HD + d0) = acc * inv;
     } else {
@@ -1208,10 +1210,9 @@ template <typename T, bool F8, int HD>
 int launch_t(const PagedAttnKArgs& k, const Plan& pl, hipStream_t st) {
   const dim3 line((unsigned)(pl.tiles * k.kv.n_kv_heads * pl.splits));
   if (pl.decode) {
-    const dim3 grid((unsigned)pl.tiles, k.kv.n_kv_heads, pl.splits);
     constexpr int STAGE = DecodeShape<T, F8, HD>::STAGE, NS = 33 * 1024 / STAGE > 4 ? 4 : 33 * 1024 / STAGE, NS8 = 17 * 1024 / STAGE > 2 ? 2 : 17 * 1024 / STAGE;
-    if (pl.nw == 2) hipLaunchKernelGGL((paged_decode_kernel<T, F8, HD, 2, NS>), grid, dim3(128), 0, st, k);
-    else hipLaunchKernelGGL((paged_decode_kernel<T, F8, HD, 8, NS8>), grid, dim3(512), 0, st, k);
+    if (pl.nw == 2) hipLaunchKernelGGL((paged_decode_kernel<T, F8, HD, 2, NS>), line, dim3(128), 0, st, k);
+    else hipLaunchKernelGGL((paged_decode_kernel<T, F8, HD, 8, NS8>), line, dim3(512), 0, st, k);
   } else if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((paged_rows_f32_kernel<F8, HD>), line, dim3(256), 0, st, k);
   else {
     if constexpr (HD == 128) {
