@@ -1156,7 +1156,7 @@ int cu_count() {
 //           628; a prompt of 8192 alone: 746 against 734).
 //   split   keys per workgroup.  Single tokens: as many splits as give two rounds of workgroups, rounded down where there are many (131072 keys of 3
 //           sequences: 40 splits fill 1.9 rounds, 161 us; 43 begin a third, 193) and up where there are few.  Chunks of an even batch: the number
-//           that leaves the last round fullest, a round being worth more than 3 % a split (1024 new tokens over 32768, 40 / 8 heads, 160 workgroups: 707 us,
+//           that leaves the last round fullest, against 3 % of a full round for each (1024 new tokens over 32768, 40 / 8 heads, 160 workgroups: 707 us,
 //           unsplit 872).  A ragged one: two rounds, since its longest sequence else runs on alone (24 sequences, 5 of them chunks of up to 701: 83 us,
 //           unsplit 128).
 struct Plan { int64_t tiles; int split, splits, nw; bool decode; };
@@ -1166,7 +1166,7 @@ Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
   const int64_t packed = (int64_t)b.rows * G;
   const bool even = b.rows >= (int64_t)b.n_seqs * b.max_q;      // all sequences bring max_q tokens
   pl.decode = (int64_t)b.max_q * G <= 16;
-  pl.nw = !pl.decode && kv.dtype == DT_BF16 && kv.head_dim == 128 && even && b.max_ctx >= 4ll * b.max_q ? 8 : 4;
+  pl.nw = !pl.decode && kv.dtype == DT_BF16 && kv.head_dim == 128 && even && (int64_t)b.max_q * G > 128 && b.max_ctx >= 4ll * b.max_q ? 8 : 4;
   const int rows = kv.dtype == DT_F32 ? 64 : 32 * pl.nw;
   pl.tiles = pl.decode ? b.n_seqs : std::min<int64_t>(packed / rows + b.n_seqs, b.n_seqs * ceil_div64((int64_t)b.max_q * G, rows));
   const int64_t wgs = std::max<int64_t>(1, pl.tiles * kv.n_kv_heads);
@@ -1178,10 +1178,11 @@ Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
       const int64_t down = 2 * slots / wgs, up = ceil_div64(2 * slots, wgs);
       int64_t n = pl.decode ? (down >= 8 ? down : up) : up;
       if (!pl.decode && even) {
+        const double each = 0.03 * (double)std::min(wgs, slots) / slots;
         double best = 1e30;
         n = 1;
-        for (int i = 1; i <= 32; ++i) {
-          const double cost = (double)ceil_div64(wgs * i, slots) / i + 0.03 * (i - 1);
+        for (int i = 1; i <= 64; ++i) {
+          const double cost = (double)ceil_div64(wgs * i, slots) / i + each * (i - 1);
           if (cost < best) best = cost, n = i;
         }
       }

@@ -12,6 +12,7 @@ tensors, and sets its bit in `PagedKV.status` (`PagedKV.check()` raises)."""
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -56,13 +57,12 @@ def _rows_of(t, name, width, dtype, index, rows=None, written=False):
     return stride[0]
 
 
-def _stream(index):
-    """The current stream of the device, which is made the current one by the callers."""
-    return torch._C._cuda_getCurrentRawStream(index)
+_lib = functools.lru_cache(None)(L.load)
+_stream = torch._C._cuda_getCurrentRawStream      # of a device's index
 
 
 def _elsewhere(index):
-    return torch.cuda.current_device() != index
+    return torch._C._cuda_getDevice() != index
 
 
 class PagedKV:
@@ -166,7 +166,7 @@ class PagedBatch:
             if n_heads:
                 a = L.PagedAttnDesc(n_heads, scale)
                 a.split_keys = split_keys
-                need = L.load().oavsr_paged_attention_workspace(C.byref(kv._for(dtype)), C.byref(d), C.byref(a))
+                need = _lib().oavsr_paged_attention_workspace(C.byref(kv._for(dtype)), C.byref(d), C.byref(a))
                 if need < 0:
                     _checked(-1)
             if len(self._plans) >= 64:
@@ -181,18 +181,22 @@ def _rope_args(rows, index, head_dim, pos, inv_freq, q_gain, k_gain):
     rot = 0
     if pos is not None:
         _on_gpu(pos, "pos", torch.int32, index)
-        _need(pos.dim() == 1 and pos.shape[0] == rows and (rows <= 1 or pos.stride(0) == 1), f"pos is {tuple(pos.shape)}, one number per row is wanted")
+        if not (pos.dim() == 1 and pos.shape[0] == rows and (rows <= 1 or pos.stride(0) == 1)):
+            _need(False, f"pos is {tuple(pos.shape)}, one number per row is wanted")
         at_pos = pos.data_ptr()
     if inv_freq is not None:
         _on_gpu(inv_freq, "inv_freq", torch.float32, index)
         rot = 2 * inv_freq.numel()
-        _need(inv_freq.dim() == 1 and rot > 0 and inv_freq.is_contiguous(), f"inv_freq is {tuple(inv_freq.shape)}, one piece of memory is wanted")
+        if not (inv_freq.dim() == 1 and rot > 0 and inv_freq.is_contiguous()):
+            _need(False, f"inv_freq is {tuple(inv_freq.shape)}, one piece of memory is wanted")
         at_freq = inv_freq.data_ptr()
     if q_gain is not None or k_gain is not None:
-        _need(q_gain is not None and k_gain is not None, "gains for both queries and keys, or for neither")
+        if not (q_gain is not None and k_gain is not None):
+            _need(False, "gains for both queries and keys, or for neither")
         for t, name in ((q_gain, "q_gain"), (k_gain, "k_gain")):
             _on_gpu(t, name, torch.float32, index)
-            _need(t.shape == (head_dim,) and t.is_contiguous(), f"{name} is {tuple(t.shape)}, ({head_dim},) is wanted")
+            if not (t.shape == (head_dim,) and t.is_contiguous()):
+                _need(False, f"{name} is {tuple(t.shape)}, ({head_dim},) is wanted")
         at_q, at_k = q_gain.data_ptr(), k_gain.data_ptr()
     return at_pos, at_freq, rot, at_q, at_k
 
@@ -208,13 +212,15 @@ def qk_norm_rope(qkv, n_heads, n_kv_heads, pos, inv_freq, *, q_gain=None, k_gain
     """Norm (with q_gain, k_gain) and rotation (by pos * inv_freq; None: none) of the query and key heads of fused rows [rows][(n_heads + 2 n_kv_heads) *
     head_dim].  Returns q [rows][n_heads][head_dim] and k [rows][n_kv_heads][head_dim]; `out` = (q, k) to write into, which may be qkv's own parts.
     inv_freq [rot_dim / 2]: the first rot_dim dimensions of a head turn, halves against each other, or neighbours when interleaved."""
-    _need(isinstance(qkv, torch.Tensor) and qkv.dim() == 2 and qkv.dtype in _DT and qkv.is_cuda, "qkv has to be rows of float32 or bfloat16 on a GPU")
+    if not (isinstance(qkv, torch.Tensor) and qkv.dim() == 2 and qkv.dtype in _DT and qkv.is_cuda):
+        _need(False, "qkv has to be rows of float32 or bfloat16 on a GPU")
     rows, width = qkv.shape
     dtype, index, all_heads = qkv.dtype, qkv.get_device(), n_heads + 2 * n_kv_heads
     if _elsewhere(index):
         with torch.cuda.device(index):
             return qk_norm_rope(qkv, n_heads, n_kv_heads, pos, inv_freq, q_gain=q_gain, k_gain=k_gain, eps=eps, interleaved=interleaved, rot_scale=rot_scale, out=out)
-    _need(n_heads > 0 and n_kv_heads > 0 and width % all_heads == 0, f"rows of {width} values do not hold {n_heads} + 2 x {n_kv_heads} heads")
+    if not (n_heads > 0 and n_kv_heads > 0 and width % all_heads == 0):
+        _need(False, f"rows of {width} values do not hold {n_heads} + 2 x {n_kv_heads} heads")
     head_dim = width // all_heads
     at_pos, at_freq, rot, at_q, at_k = _rope_args(rows, index, head_dim, pos, inv_freq, q_gain, k_gain)
     ld, ldq, ldk = _rows_of(qkv, "qkv", width, dtype, index), n_heads * head_dim, n_kv_heads * head_dim
@@ -225,14 +231,15 @@ def qk_norm_rope(qkv, n_heads, n_kv_heads, pos, inv_freq, *, q_gain=None, k_gain
         ldq, ldk = _rows_of(q, "out[0]", ldq, dtype, index, rows, True), _rows_of(k, "out[1]", ldk, dtype, index, rows, True)
     d = L.QkRopeDesc(_DT[dtype], rows, n_heads, n_kv_heads, head_dim, qkv.data_ptr(), ld, q.data_ptr(), ldq, k.data_ptr(), ldk, at_pos, at_freq, rot,
                      bool(interleaved), rot_scale, at_q, at_k, eps)
-    _checked(L.load().oavsr_op_qk_norm_rope(C.byref(d), _stream(index)))
+    _checked(_lib().oavsr_op_qk_norm_rope(C.byref(d), _stream(index)))
     return q, k
 
 
 def append(kv, batch, qkv, inv_freq=None, *, pos=None, q_gain=None, k_gain=None, eps=1e-6, interleaved=False, rot_scale=1.0, out=None):
     """qk_norm_rope of the batch's rows, the keys and values going into their sequences' pages.  Returns q [rows][n_heads][head_dim] (`out`: where to, which
     may be qkv's own part).  pos [rows]: positions to turn by where they are not the tokens' places in their sequences.  Rows of no sequence are left."""
-    _need(isinstance(qkv, torch.Tensor) and qkv.dim() == 2 and qkv.is_cuda, "qkv has to be rows on a GPU")
+    if not (isinstance(qkv, torch.Tensor) and qkv.dim() == 2 and qkv.is_cuda):
+        _need(False, "qkv has to be rows on a GPU")
     heads, head_dim, index = kv.heads, kv.head_dim, kv.index
     if _elsewhere(index):
         with torch.cuda.device(index):
@@ -241,7 +248,8 @@ def append(kv, batch, qkv, inv_freq=None, *, pos=None, q_gain=None, k_gain=None,
     dtype = qkv.dtype
     desc = kv._for(dtype)
     n_heads = width // head_dim - 2 * heads
-    _need(n_heads > 0 and width % head_dim == 0, f"rows of {width} values do not hold query heads beside 2 x {heads} heads of {head_dim}")
+    if not (n_heads > 0 and width % head_dim == 0):
+        _need(False, f"rows of {width} values do not hold query heads beside 2 x {heads} heads of {head_dim}")
     ld = _rows_of(qkv, "qkv", width, dtype, index)
     at_pos, at_freq, rot, at_q, at_k = _rope_args(rows, index, head_dim, pos, inv_freq, q_gain, k_gain)
     b, _ = batch._for(rows, kv)
@@ -252,7 +260,7 @@ def append(kv, batch, qkv, inv_freq=None, *, pos=None, q_gain=None, k_gain=None,
         ldq = _rows_of(out, "out", ldq, dtype, index, rows, True)
     d = L.QkRopeDesc(_DT[dtype], rows, n_heads, heads, head_dim, qkv.data_ptr(), ld, out.data_ptr(), ldq, None, 0, at_pos, at_freq, rot, bool(interleaved), rot_scale,
                      at_q, at_k, eps)
-    _checked(L.load().oavsr_op_paged_append(C.byref(desc), C.byref(b), C.byref(d), _stream(index)))
+    _checked(_lib().oavsr_op_paged_append(C.byref(desc), C.byref(b), C.byref(d), _stream(index)))
     return out
 
 
@@ -265,7 +273,8 @@ def read(kv, batch, rows=None, *, dtype=None, out=None):
             return read(kv, batch, rows, dtype=dtype, out=out)
     ldk = ldv = width = heads * head_dim
     if out is None:
-        _need(rows is not None, "rows or out is needed")
+        if not (rows is not None):
+            _need(False, "rows or out is needed")
         if dtype is None:
             dtype = torch.bfloat16 if kv.is_8bit else kv.k.dtype
         desc = kv._for(dtype)
@@ -273,7 +282,8 @@ def read(kv, batch, rows=None, *, dtype=None, out=None):
         at_k, at_v = k.data_ptr(), v.data_ptr()
     else:
         given = [t for t in out if t is not None]
-        _need(len(out) == 2 and given and all(isinstance(t, torch.Tensor) for t in given), "out is (k, v), one of them at least a tensor")
+        if not (len(out) == 2 and given and all(isinstance(t, torch.Tensor) for t in given)):
+            _need(False, "out is (k, v), one of them at least a tensor")
         k, v = out
         dtype = given[0].dtype if dtype is None else dtype
         rows = given[0].shape[0] if rows is None else rows
@@ -284,7 +294,7 @@ def read(kv, batch, rows=None, *, dtype=None, out=None):
         if v is not None:
             ldv, at_v = _rows_of(v, "out[1]", width, dtype, index, rows, True), v.data_ptr()
     b, _ = batch._for(rows, kv)
-    _checked(L.load().oavsr_op_paged_read(C.byref(desc), C.byref(b), at_k, ldk, at_v, ldv, _stream(index)))
+    _checked(_lib().oavsr_op_paged_read(C.byref(desc), C.byref(b), at_k, ldk, at_v, ldv, _stream(index)))
     return k, v
 
 
@@ -293,7 +303,8 @@ def attention(kv, batch, q, scale=None, *, out=None, lse=None, split_keys=0):
     out, shaped like q.  scale: default head_dim ** -0.5.  lse: float32 [rows][n_heads] to fill.  split_keys: keys per workgroup (a multiple of 256; 0: the
     library's rule), for results whose last bits do not follow the batch a row is in."""
     index, head_dim = kv.index, kv.head_dim
-    _need(isinstance(q, torch.Tensor) and q.dim() in (2, 3) and q.is_cuda, "q has to be rows on a GPU")
+    if not (isinstance(q, torch.Tensor) and q.dim() in (2, 3) and q.is_cuda):
+        _need(False, "q has to be rows on a GPU")
     if _elsewhere(index):
         with torch.cuda.device(index):
             return attention(kv, batch, q, scale, out=out, lse=lse, split_keys=split_keys)
@@ -301,7 +312,8 @@ def attention(kv, batch, q, scale=None, *, out=None, lse=None, split_keys=0):
     desc, rows = kv._for(dtype), shape[0]
     width = shape[1] * shape[2] if len(shape) == 3 else shape[1]
     n_heads = width // head_dim
-    _need(width % head_dim == 0 and (len(shape) == 2 or shape[2] == head_dim), f"q is {tuple(shape)}, the cache's heads have {head_dim} dimensions")
+    if not (width % head_dim == 0 and (len(shape) == 2 or shape[2] == head_dim)):
+        _need(False, f"q is {tuple(shape)}, the cache's heads have {head_dim} dimensions")
     scale = head_dim ** -0.5 if scale is None else scale
     ldq = _rows_of(q, "q", width, dtype, index)
     b, need = batch._for(rows, kv, dtype, n_heads, split_keys)
@@ -313,9 +325,10 @@ def attention(kv, batch, q, scale=None, *, out=None, lse=None, split_keys=0):
     at_lse = None
     if lse is not None:
         _on_gpu(lse, "lse", torch.float32, index)
-        _need(lse.shape == (rows, n_heads) and lse.is_contiguous(), f"lse is {tuple(lse.shape)}, ({rows}, {n_heads}) in one piece is wanted")
+        if not (lse.shape == (rows, n_heads) and lse.is_contiguous()):
+            _need(False, f"lse is {tuple(lse.shape)}, ({rows}, {n_heads}) in one piece is wanted")
         at_lse = lse.data_ptr()
     work = torch.empty(need, dtype=torch.uint8, device=kv.device) if need else None      # of this call alone; the allocator reuses it in stream order
     d = L.PagedAttnDesc(n_heads, scale, q.data_ptr(), ldq, out.data_ptr(), ldo, at_lse, split_keys, None if work is None else work.data_ptr(), need)
-    _checked(L.load().oavsr_op_paged_attention(C.byref(desc), C.byref(b), C.byref(d), _stream(index)))
+    _checked(_lib().oavsr_op_paged_attention(C.byref(desc), C.byref(b), C.byref(d), _stream(index)))
     return out
