@@ -38,12 +38,14 @@ def _on_gpu(t, name, dtype, index=None):
 
 def _rows_of(t, name, width, dtype, index, rows=None, written=False):
     """Row stride of [rows][width] or [rows][heads][head_dim] rows, each of them one piece of memory; rows that are written must not overlap."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index and t.is_contiguous():      # the common case
+        n = t.shape[0] if t.dim() in (2, 3) else -1
+        if n == rows if rows is not None else n >= 0:
+            if t.numel() == n * width and n > 0:
+                return width
     _on_gpu(t, name, dtype, index)
     shape, stride = t.shape, t.stride()
     n = shape[0] if len(shape) > 1 else -1
-    if len(shape) == 3 and shape[1] * shape[2] == width and stride[2] == 1 and (stride[1] == shape[2] or shape[1] == 1) or len(shape) == 2 and shape[1] == width and stride[1] == 1:
-        if (rows is None or n == rows) and n > 1 and stride[0] >= width:
-            return stride[0]
     _need(len(shape) in (2, 3), f"{name} has {len(shape)} dimensions")
     _need(shape[1] * (shape[2] if len(shape) == 3 else 1) == width, f"{name} has rows of shape {tuple(shape[1:])}, {width} values are wanted")
     _need(rows is None or n == rows, f"{name} has {n} rows, {rows} are wanted")
@@ -61,8 +63,7 @@ _lib = functools.lru_cache(None)(L.load)
 _stream = torch._C._cuda_getCurrentRawStream      # of a device's index
 
 
-def _elsewhere(index):
-    return torch._C._cuda_getDevice() != index
+_device = torch._C._cuda_getDevice               # the current one's index
 
 
 class PagedKV:
@@ -104,7 +105,7 @@ class PagedKV:
         if self.is_8bit:
             self.descs[torch.float32] = type(d).from_buffer_copy(d)
             self.descs[torch.float32].dtype = L.DT_F32
-        self.heads, self.head_dim, self.shape = heads, dim, (heads, dim, page, d.format)
+        self.heads, self.head_dim, self.page, self.shape = heads, dim, page, (heads, dim, page, d.format)
 
     @classmethod
     def empty(cls, n_pages, page_size, n_kv_heads, head_dim, dtype=torch.bfloat16, device="cuda"):
@@ -151,54 +152,51 @@ class PagedBatch:
         d.cu_q, d.ctx_len, d.table = cu_q.data_ptr(), ctx_len.data_ptr(), table.data_ptr()
         d.ld_table = table.stride(0) if n > 1 else self.width
         _need(n <= 1 or d.ld_table >= self.width, f"rows of table overlap (strides {table.stride()})")
-        self._plans = {}
+        self._descs, self._work = {}, {}
 
-    def _for(self, rows, kv, dtype=None, n_heads=0, split_keys=0, scale=1.0):
-        """The description for so many rows, and with n_heads the workspace that attention of them needs: of the bounds alone, so kept."""
-        key = (rows, kv.shape, dtype, n_heads, split_keys)
-        found = self._plans.get(key)
-        if found is None or self.index != kv.index:
+    def _for(self, rows, kv):
+        """The description for so many rows."""
+        if self.index != kv.index or self.desc.max_ctx > self.width * kv.page:
             _need(self.index == kv.index, f"the batch is on cuda:{self.index}, the cache on cuda:{kv.index}")
-            page = kv.desc.page_size
-            _need(self.desc.max_ctx <= self.width * page, f"a table of {self.width} pages of {page} does not hold max_ctx {self.desc.max_ctx}")
-            d, need = L.PagedBatchDesc.from_buffer_copy(self.desc), 0
+            _need(False, f"a table of {self.width} pages of {kv.page} does not hold max_ctx {self.desc.max_ctx}")
+        d = self._descs.get(rows)
+        if d is None:
+            d = L.PagedBatchDesc.from_buffer_copy(self.desc)
             d.rows = rows
-            if n_heads:
-                a = L.PagedAttnDesc(n_heads, scale)
-                a.split_keys = split_keys
-                need = _lib().oavsr_paged_attention_workspace(C.byref(kv._for(dtype)), C.byref(d), C.byref(a))
-                if need < 0:
-                    _checked(-1)
-            if len(self._plans) >= 64:
-                self._plans.clear()
-            found = self._plans[key] = d, need
-        return found
+            if len(self._descs) >= 64:
+                self._descs.clear()
+            self._descs[rows] = d
+        return d
+
+    def _workspace(self, d, kv, dtype, n_heads, split_keys):
+        """Bytes that attention needs: they follow from bounds that do not change, so they are kept."""
+        key = (d.rows, kv.shape, dtype, n_heads, split_keys)
+        need = self._work.get(key)
+        if need is None:
+            a = L.PagedAttnDesc(n_heads, 1.0)
+            a.split_keys = split_keys
+            need = _lib().oavsr_paged_attention_workspace(C.byref(kv._for(dtype)), C.byref(d), C.byref(a))
+            if need < 0:
+                _checked(-1)
+            if len(self._work) >= 64:
+                self._work.clear()
+            self._work[key] = need
+        return need
 
 
-def _rope_args(rows, index, head_dim, pos, inv_freq, q_gain, k_gain):
-    """Checked pointers of the rotation: (pos, inv_freq, rot_dim, q_gain, k_gain)."""
-    at_pos = at_freq = at_q = at_k = None
-    rot = 0
-    if pos is not None:
-        _on_gpu(pos, "pos", torch.int32, index)
-        if not (pos.dim() == 1 and pos.shape[0] == rows and (rows <= 1 or pos.stride(0) == 1)):
-            _need(False, f"pos is {tuple(pos.shape)}, one number per row is wanted")
-        at_pos = pos.data_ptr()
-    if inv_freq is not None:
-        _on_gpu(inv_freq, "inv_freq", torch.float32, index)
-        rot = 2 * inv_freq.numel()
-        if not (inv_freq.dim() == 1 and rot > 0 and inv_freq.is_contiguous()):
-            _need(False, f"inv_freq is {tuple(inv_freq.shape)}, one piece of memory is wanted")
-        at_freq = inv_freq.data_ptr()
-    if q_gain is not None or k_gain is not None:
-        if not (q_gain is not None and k_gain is not None):
-            _need(False, "gains for both queries and keys, or for neither")
-        for t, name in ((q_gain, "q_gain"), (k_gain, "k_gain")):
-            _on_gpu(t, name, torch.float32, index)
-            if not (t.shape == (head_dim,) and t.is_contiguous()):
-                _need(False, f"{name} is {tuple(t.shape)}, ({head_dim},) is wanted")
-        at_q, at_k = q_gain.data_ptr(), k_gain.data_ptr()
-    return at_pos, at_freq, rot, at_q, at_k
+def _vector(t, name, dtype, index, n=None):
+    """Address of a vector (of n) in one piece."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index and t.dim() == 1 and (n is None or t.numel() == n) and t.is_contiguous()):
+        _on_gpu(t, name, dtype, index)
+        _need(False, f"{name} is {tuple(t.shape)} (strides {t.stride()}), a vector{'' if n is None else f' of {n}'} in one piece is wanted")
+    return t.data_ptr()
+
+
+def _gains(q_gain, k_gain, index, head_dim):
+    if q_gain is None and k_gain is None:
+        return None, None
+    _need(q_gain is not None and k_gain is not None, "gains for both queries and keys, or for neither")
+    return _vector(q_gain, "q_gain", torch.float32, index, head_dim), _vector(k_gain, "k_gain", torch.float32, index, head_dim)
 
 
 def _checked(rc):
@@ -216,13 +214,15 @@ def qk_norm_rope(qkv, n_heads, n_kv_heads, pos, inv_freq, *, q_gain=None, k_gain
         _need(False, "qkv has to be rows of float32 or bfloat16 on a GPU")
     rows, width = qkv.shape
     dtype, index, all_heads = qkv.dtype, qkv.get_device(), n_heads + 2 * n_kv_heads
-    if _elsewhere(index):
+    if _device() != index:
         with torch.cuda.device(index):
             return qk_norm_rope(qkv, n_heads, n_kv_heads, pos, inv_freq, q_gain=q_gain, k_gain=k_gain, eps=eps, interleaved=interleaved, rot_scale=rot_scale, out=out)
     if not (n_heads > 0 and n_kv_heads > 0 and width % all_heads == 0):
         _need(False, f"rows of {width} values do not hold {n_heads} + 2 x {n_kv_heads} heads")
     head_dim = width // all_heads
-    at_pos, at_freq, rot, at_q, at_k = _rope_args(rows, index, head_dim, pos, inv_freq, q_gain, k_gain)
+    at_freq, rot = (None, 0) if inv_freq is None else (_vector(inv_freq, "inv_freq", torch.float32, index), 2 * inv_freq.numel())
+    at_pos = None if pos is None else _vector(pos, "pos", torch.int32, index, rows)
+    at_q, at_k = _gains(q_gain, k_gain, index, head_dim)
     ld, ldq, ldk = _rows_of(qkv, "qkv", width, dtype, index), n_heads * head_dim, n_kv_heads * head_dim
     if out is None:
         q, k = qkv.new_empty((rows, n_heads, head_dim)), qkv.new_empty((rows, n_kv_heads, head_dim))
@@ -241,7 +241,7 @@ def append(kv, batch, qkv, inv_freq=None, *, pos=None, q_gain=None, k_gain=None,
     if not (isinstance(qkv, torch.Tensor) and qkv.dim() == 2 and qkv.is_cuda):
         _need(False, "qkv has to be rows on a GPU")
     heads, head_dim, index = kv.heads, kv.head_dim, kv.index
-    if _elsewhere(index):
+    if _device() != index:
         with torch.cuda.device(index):
             return append(kv, batch, qkv, inv_freq, pos=pos, q_gain=q_gain, k_gain=k_gain, eps=eps, interleaved=interleaved, rot_scale=rot_scale, out=out)
     rows, width = qkv.shape
@@ -251,8 +251,10 @@ def append(kv, batch, qkv, inv_freq=None, *, pos=None, q_gain=None, k_gain=None,
     if not (n_heads > 0 and width % head_dim == 0):
         _need(False, f"rows of {width} values do not hold query heads beside 2 x {heads} heads of {head_dim}")
     ld = _rows_of(qkv, "qkv", width, dtype, index)
-    at_pos, at_freq, rot, at_q, at_k = _rope_args(rows, index, head_dim, pos, inv_freq, q_gain, k_gain)
-    b, _ = batch._for(rows, kv)
+    at_freq, rot = (None, 0) if inv_freq is None else (_vector(inv_freq, "inv_freq", torch.float32, index), 2 * inv_freq.numel())
+    at_pos = None if pos is None else _vector(pos, "pos", torch.int32, index, rows)
+    at_q, at_k = _gains(q_gain, k_gain, index, head_dim)
+    b = batch._for(rows, kv)
     ldq = n_heads * head_dim
     if out is None:
         out = qkv.new_empty((rows, n_heads, head_dim))
@@ -268,7 +270,7 @@ def read(kv, batch, rows=None, *, dtype=None, out=None):
     """The cached keys and values of the batch's `rows` rows (cu_q[-1]; more are left out), as (k, v) [rows][n_kv_heads][head_dim] in `dtype` (default: the
     cache's; bfloat16 of an 8-bit one).  `out` = (k, v) to write into, either may be None; rows of no sequence are left as they were."""
     heads, head_dim, index = kv.heads, kv.head_dim, kv.index
-    if _elsewhere(index):
+    if _device() != index:
         with torch.cuda.device(index):
             return read(kv, batch, rows, dtype=dtype, out=out)
     ldk = ldv = width = heads * head_dim
@@ -293,7 +295,7 @@ def read(kv, batch, rows=None, *, dtype=None, out=None):
             ldk, at_k = _rows_of(k, "out[0]", width, dtype, index, rows, True), k.data_ptr()
         if v is not None:
             ldv, at_v = _rows_of(v, "out[1]", width, dtype, index, rows, True), v.data_ptr()
-    b, _ = batch._for(rows, kv)
+    b = batch._for(rows, kv)
     _checked(_lib().oavsr_op_paged_read(C.byref(desc), C.byref(b), at_k, ldk, at_v, ldv, _stream(index)))
     return k, v
 
@@ -305,7 +307,7 @@ def attention(kv, batch, q, scale=None, *, out=None, lse=None, split_keys=0):
     index, head_dim = kv.index, kv.head_dim
     if not (isinstance(q, torch.Tensor) and q.dim() in (2, 3) and q.is_cuda):
         _need(False, "q has to be rows on a GPU")
-    if _elsewhere(index):
+    if _device() != index:
         with torch.cuda.device(index):
             return attention(kv, batch, q, scale, out=out, lse=lse, split_keys=split_keys)
     dtype, shape = q.dtype, q.shape
@@ -316,7 +318,8 @@ def attention(kv, batch, q, scale=None, *, out=None, lse=None, split_keys=0):
         _need(False, f"q is {tuple(shape)}, the cache's heads have {head_dim} dimensions")
     scale = head_dim ** -0.5 if scale is None else scale
     ldq = _rows_of(q, "q", width, dtype, index)
-    b, need = batch._for(rows, kv, dtype, n_heads, split_keys)
+    b = batch._for(rows, kv)
+    need = batch._workspace(b, kv, dtype, n_heads, split_keys)
     ldo = width
     if out is None:
         out = q.new_empty(shape)

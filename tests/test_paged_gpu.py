@@ -377,13 +377,15 @@ def test_prompts_in_chunks_then_single_tokens(dtype, fmt, H, KV, d):
     within(torch.cat([torch.cat(x) for x in outs]), y, err + U[dt] * (y.abs() + err), "attention over the cache")
 
 
-def test_a_step_captured_into_a_graph():
-    """append + attention of a decode step in a graph, its lengths and tables refilled in place between replays, eager work between them: the eager results."""
+@pytest.mark.parametrize("fmt,top", [("same", 600), ("same", 5000), ("e4m3", 5000)])
+def test_a_step_captured_into_a_graph(fmt, top):
+    """append + attention of a decode step in a graph (one launch of attention, and split ones with their workspace), its lengths and tables refilled in place
+    between replays, eager work between them: the eager results."""
     H, KV, d, page, n = 8, 2, 64, 16, 5
-    pool = Pool(KV, d, page, "bf16", "same", [600] * n)
-    start = [37, 512, 1, 255, 300]
-    pool.fill([600] * n)
-    b = pool.batch([1] * n, start, max_ctx=600)
+    pool = Pool(KV, d, page, "bf16", fmt, [top] * n)
+    start = [37, top - 88, 1, 255, 300]
+    pool.fill([top] * n)
+    b = pool.batch([1] * n, start, max_ctx=top)
     rows, inv = torch.zeros(n, (H + 2 * KV) * d, dtype=torch.bfloat16, device=DEV), freqs(d).to(DEV)
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
@@ -418,6 +420,55 @@ def test_two_streams_at_once():
                 o.append(paged.attention(pool.kv, b, q))
     torch.cuda.synchronize()
     assert all(torch.equal(x, want) for o in got for x in o)
+
+
+def test_many_sequences():
+    """More sequences than a wave looks through at once: single tokens of 5000, and ragged chunks of 150 with empty ones among them."""
+    d, page = 64, 16
+    for new, ctx in (([1] * 5000, [1 + i % 40 for i in range(5000)]), ([(i * 7) % 23 for i in range(150)], [(i * 7) % 23 + (i * 5) % 60 for i in range(150)])):
+        pool = Pool(1, d, page, "bf16", "same", ctx)
+        k, v = pool.fill(ctx)
+        q = rnd(sum(new), 4, d, seed=1, dtype=torch.bfloat16)
+        out = paged.attention(pool.kv, pool.batch(new, ctx), q.to(DEV))
+        pool.kv.check()
+        y, err, _ = attended(q, k, v, new, ctx, d ** -0.5, True)
+        within(out, y, err + U[torch.bfloat16] * (y.abs() + err), "attention")
+
+
+@pytest.mark.parametrize("fmt,new", [("same", 1), ("same", 50), ("e4m3", 1), ("e4m3", 50)])
+def test_pages_behind_four_gigabytes(fmt, new):
+    """Page numbers whose bytes lie behind 2^32 (and their elements behind 2^31): written, read and attended there."""
+    KV, d, page, ctx = 4, 128, 128, 300
+    bytes_per_page = KV * page * d * (1 if fmt == "e4m3" else 2)
+    n = (5 << 30) // bytes_per_page
+    dt = E4M3 if fmt == "e4m3" else torch.bfloat16
+    t = [torch.empty(n, KV, page, d, dtype=dt, device=DEV) for _ in range(2)]
+    if fmt == "e4m3":
+        t += [torch.empty(n, KV, page, device=DEV) for _ in range(2)]
+    pool = Pool(KV, d, page, "bf16", fmt, [ctx])
+    pool.kv, pool.table = paged.PagedKV(*t), torch.tensor([[n - 1, n - 7, n - 2]], dtype=torch.int32)
+    k, v = pool.fill([ctx])
+    q = rnd(new, 8, d, seed=1, dtype=torch.bfloat16)
+    out = paged.attention(pool.kv, pool.batch([new], [ctx]), q.to(DEV))
+    y, err, _ = attended(q, k, v, [new], [ctx], d ** -0.5, True)
+    within(out, y, err + U[torch.bfloat16] * (y.abs() + err), "attention")
+
+
+@pytest.mark.parametrize("dtype,fmt,H,KV,d,page,new,ctx", [
+    ("bf16", "same", 8, 2, 64, 16, [64, 64], [5000, 5000]), ("bf16", "same", 4, 1, 128, 64, [300], [4000]), ("bf16", "e4m3", 32, 8, 128, 32, [40], [2500]),
+    ("f32", "same", 8, 2, 64, 16, [100, 9], [900, 2100]), ("f32", "e4m3", 4, 2, 128, 16, [33], [1300]), ("bf16", "same", 14, 2, 64, 256, [5, 400], [3000, 410])])
+def test_attention_long_contexts(dtype, fmt, H, KV, d, page, new, ctx):
+    """Chunks over contexts that the library's own rule splits, and does not split, in every kernel's several tiles."""
+    dt = tdt(dtype)
+    pool = Pool(KV, d, page, dtype, fmt, ctx)
+    k, v = pool.fill(ctx)
+    q = rnd(sum(new), H, d, seed=8, scale=1.5, dtype=dt)
+    lse = torch.empty(sum(new), H, device=DEV)
+    out = paged.attention(pool.kv, pool.batch(new, ctx), q.to(DEV), lse=lse)
+    y, err, z = attended(q, k, v, new, ctx, d ** -0.5, dtype == "bf16")
+    within(out, y, err + U[dt] * (y.abs() + err), "attention")
+    top = q.double().abs().amax() * d ** 0.5 * 6
+    within(lse, z, 2 * (d + 4) * U32 * top + 2 * (max(ctx) + 8) * U32 + 4e-6, "lse")
 
 
 # ---- bad lengths and page numbers (the host-side twin of these checks runs on the CPU) -----------------------------------------------------------------
