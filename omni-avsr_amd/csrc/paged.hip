@@ -57,8 +57,11 @@ __device__ __forceinline__ float quotient_odd(float x, float scale, float inv) {
   return __builtin_bit_cast(float, bits);
 }
 
+struct Pages { PagedKv kv; PagedBatch b; };
+struct NoPages {};
+
 template <typename T, int HD, bool CACHE, bool F8>
-__global__ __launch_bounds__(kThreads) void qk_rope_kernel(const QkRopeArgs p, const PagedKv kv, const PagedBatch b, int parts) {
+__global__ __launch_bounds__(kThreads) void qk_rope_kernel(const QkRopeArgs p, const std::conditional_t<CACHE, Pages, NoPages> pages, int parts) {
   constexpr int LPH = HD / 16, HPW = 64 / LPH;       // lanes per head, heads per wave
   __shared__ float2 turns[kWaves][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -68,6 +71,8 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(const QkRopeArgs p, c
 
   int pos = 0, page = -1, off = 0;
   if constexpr (CACHE) {
+    const PagedKv& kv = pages.kv;
+    const PagedBatch& b = pages.b;
     const int s = wave_find_seq(b.cu_q, b.n_seqs, row, lane);
     const SeqInfo q = paged_seq(b, s);
     if (q.bad && lane == 0 && part == 0) paged_report(kv.status, kBadLength);
@@ -148,7 +153,8 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(const QkRopeArgs p, c
                     : reinterpret_cast<T*>(p.k_out) + (int64_t)row * p.ldk + (int64_t)(h - p.n_heads) * HD;
       store8<T>(dst + e0, x);
       store8<T>(dst + e1, x + 8);
-    } else {
+    } else if constexpr (CACHE) {
+      const PagedKv& kv = pages.kv;
       const int kh = is_v ? h - p.n_heads - p.n_kv_heads : h - p.n_heads;
       const int64_t tok = (int64_t)kh * kv.page_size + off;
       void* base = is_v ? kv.V : kv.K;
@@ -263,8 +269,10 @@ int launch_rope_t(const QkRopeArgs& a, const PagedKv& kv, const PagedBatch& b, h
   const int parts = a.rows >= kManyRows ? 1 : ceil_div(heads, hpw);
   const int64_t blocks = ceil_div64((int64_t)a.rows * parts, kWaves);
   OAVSR_REQUIRE(blocks < (1ll << 31), "paged: %d rows are too many for one launch", a.rows);
-  if (a.head_dim == 64) hipLaunchKernelGGL((qk_rope_kernel<T, 64, CACHE, F8>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a, kv, b, parts);
-  else hipLaunchKernelGGL((qk_rope_kernel<T, 128, CACHE, F8>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a, kv, b, parts);
+  std::conditional_t<CACHE, Pages, NoPages> pages;
+  if constexpr (CACHE) { pages.kv = kv; pages.b = b; }
+  if (a.head_dim == 64) hipLaunchKernelGGL((qk_rope_kernel<T, 64, CACHE, F8>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a, pages, parts);
+  else hipLaunchKernelGGL((qk_rope_kernel<T, 128, CACHE, F8>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a, pages, parts);
   OAVSR_CHECK_HIP(hipGetLastError());
   return 0;
 }

@@ -405,12 +405,14 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
     }
 
     if constexpr (sizeof(T) == 2) {
-      bf16x8 pf, pl;                                   // the weights as a sum of two numbers: one rounding of them less, and products are not what is short here
+      // The weights as sums of two numbers: a rounding less, and products are not what is short here.  The first is cut off, so that the second has its
+      // sign, and the second is never zero beside one that is not: an infinite value stays what it is.
+      bf16x8 pf, pl;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float e = s[i >> 2][i & 3];
-        pf[i] = (bf16_t)e;
-        pl[i] = (bf16_t)(e - (float)pf[i]);
+        const float e = s[i >> 2][i & 3], hi = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, e) & 0xffff0000u);
+        pf[i] = (bf16_t)hi;
+        pl[i] = (bf16_t)fmaxf(e - hi, e * 0x1p-30f);
       }
       const unsigned vb = lds_address(sV);
 #pragma unroll
@@ -1191,7 +1193,7 @@ Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
   }
   pl.splits = ceil_div(b.max_ctx, pl.split);
   if (pl.splits <= 1) pl.split = 0, pl.splits = 1;
-  if (pl.decode) pl.nw = wgs * pl.splits > cus ? 2 : 8;
+  if (pl.decode) pl.nw = a.split_keys || wgs * pl.splits > cus ? 2 : 8;      // (a pinned split: the waves' shares too)
   return pl;
 }
 uint64_t workspace_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a, const Plan& pl) {

@@ -336,17 +336,42 @@ def test_attention_reads_strided_rows_and_a_shared_prefix():
     assert (hold[:, :32] == 7).all() and (hold[:, 32 + H * d:] == 7).all()
 
 
+@pytest.mark.parametrize("fmt", ["same", "e4m3"])
 @pytest.mark.parametrize("new", [1, 2, 40])
-def test_attention_split_by_the_caller_is_the_same_in_any_batch(new):
-    """split_keys given: a sequence's rows have the same bits alone and among others (the same max_q)."""
-    lens = [1200, 300, 2049, 70]
-    pool = Pool(2, 128, 64, "bf16", "same", lens)
+def test_attention_split_by_the_caller_is_the_same_in_any_batch(fmt, new):
+    """split_keys given: a sequence's rows have the same bits alone, among a few and among many others (the same max_q), where the library's own rule takes
+    other splits and workgroups."""
+    lens = [1200, 300, 2049, 70] + [130 + 9 * i for i in range(76)]
+    pool = Pool(2, 128, 64, "bf16", fmt, lens)
     pool.fill(lens)
-    q = rnd(4 * new, 8, 128, seed=1, dtype=torch.bfloat16).to(DEV)
-    both = paged.attention(pool.kv, pool.batch([new] * 4, lens), q, split_keys=512)
+    q = rnd(len(lens) * new, 8, 128, seed=1, dtype=torch.bfloat16).to(DEV)
+
+    def some(which):
+        rows = torch.cat([q[s * new:(s + 1) * new] for s in which])
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+        b = paged.PagedBatch(i32([new * i for i in range(len(which) + 1)]), i32([lens[s] for s in which]), pool.table[which].to(DEV), max_q=new, max_ctx=max(lens[s] for s in which))
+        return paged.attention(pool.kv, b, rows, split_keys=512).split(new)
+
+    every = some(list(range(len(lens))))
     for s in range(4):
-        alone = paged.PagedBatch(*(torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([0, new], [lens[s]], [pool.table[s].tolist()])), max_q=new, max_ctx=lens[s])
-        assert torch.equal(paged.attention(pool.kv, alone, q[s * new:(s + 1) * new].contiguous(), split_keys=512), both[s * new:(s + 1) * new])
+        assert torch.equal(some([s])[0], every[s])
+    assert all(torch.equal(x, every[s]) for s, x in enumerate(some([0, 1, 2, 3])))
+
+
+@pytest.mark.parametrize("dtype,H,KV,d", [("bf16", 8, 2, 128), ("f32", 4, 2, 64)])
+@pytest.mark.parametrize("new", [1, 60])
+def test_attention_infinite_values_that_are_seen(dtype, H, KV, d, new):
+    """A seen value that is infinite makes its dimension infinite, and leaves the others."""
+    ctx, dt = 150, tdt(dtype)
+    pool = Pool(KV, d, 16, dtype, "same", [ctx])
+    pool.fill([ctx])
+    q, b = rnd(new, H, d, seed=3, dtype=dt).to(DEV), pool.batch([new], [ctx])
+    good = paged.attention(pool.kv, b, q)
+    pool.kv.v[int(pool.table[0, 1]), 0, 3, 7] = float("-inf")
+    out = paged.attention(pool.kv, b, q)
+    assert (out[:, :H // KV, 7] == -math.inf).all()
+    out[:, :H // KV, 7] = good[:, :H // KV, 7]
+    within(out, good.cpu().double(), 4 * U[dt] * good.cpu().double().abs() + 4 * U[dt] * good.cpu().double().abs().amax(), "the other dimensions")
 
 
 # ---- together -----------------------------------------------------------------------------------------------------------------------------------
