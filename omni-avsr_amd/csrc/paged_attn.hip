@@ -535,12 +535,16 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
 
 // ---- many rows per sequence: chunks and whole prompts, bf16 ------------------------------------------------------------------------------------
 //
-// A workgroup of 8 waves takes 256 packed rows of a (sequence, kv head), 32 per wave, on 32x32x16 matrix instructions; tiles of 64 keys are shared by the
-// waves.  Bound by the matrix pipe and the vector issue of the softmax together (per tile and wave at head_dim 128: 32 products of 32 cycles, about 200 vector
-// instructions of 4).  A bf16 cache goes to a ring of three tiles in LDS by LDS-DMA, two tiles ahead, one barrier per tile; an 8-bit one through
-// registers, each thread widening its 16 bytes once per tile for all waves, into a ring of two.  The kv head is the fastest part of a workgroup's number:
-// workgroups of one kv head then share an XCD (8 of them take the numbers in turn), and its L2 serves their common keys.
-// A wave skips the tiles none of its rows sees, and masks only those that some row sees in part.
+// A workgroup of 4 (8) waves takes 128 (256) packed rows of a (sequence, kv head), 32 per wave, on 32x32x16 matrix instructions; tiles of 64 keys are shared by
+// the waves.  Bound by the matrix pipe and the vector issue of the softmax together (per tile and wave at head_dim 128: 32 products of 32 cycles, about 200
+// vector instructions of 4; at head_dim 64 half the products for the same softmax).  A tile travels through registers into one of two LDS images, one barrier per
+// tile, its loads issued a tile ahead: each thread widens 8-bit bytes once for all waves, and the transposing reads of the values, which the compiler would
+// hold behind every LDS-DMA in flight, can be requested before the exponentials that hide them (533 us with LDS-DMA and a ring of three, 515 so).
+// The kv head is the fastest part of a workgroup's number: workgroups of one kv head then share an XCD (8 of them take the numbers in turn), and its L2
+// serves their common keys.  Sequences' tiles are taken from the last to the first, so that a prompt's long rows are not what remains at the end (a prompt
+// of 8192, 32 / 8 heads: 642 us in rising order, 576 so, 549 with 256 rows; one level of all sequences at a time: the same there, but 4 chunks over
+// 12000 keys 704 us against 447, since the L2 no longer sees a sequence's keys once).  2048 new tokens over 16384: 500 us, 1030 TFLOP/s.
+// A wave skips the tiles none of its rows sees, and masks only those that some row sees in part, in a loop of its own.
 template <bool F8, int HD, int NW>
 __global__ __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) void paged_chunk_kernel(const PagedAttnKArgs p) {
   constexpr int ROWS = NW * 32, RB = HD * 2, IMG = KT * RB, NSTAGE = 2, STAGE = 2 * IMG + (F8 ? 2 * KT * 4 : 0);
@@ -551,7 +555,7 @@ __global__ __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) void paged_chunk_kernel(
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ql = lane & 31, h = lane >> 5;
   const int G = p.group, KV = p.kv.n_kv_heads;
   const int kvh = blockIdx.x % KV, unit = blockIdx.x / KV, split = unit / p.tiles;
-  const TileAt at = wave_find_tile<ROWS>(p.b, G, unit - split * p.tiles, lane);
+  const TileAt at = wave_find_tile<ROWS>(p.b, G, p.tiles - 1 - (unit - split * p.tiles), lane);      // the last rows, which see the most keys, first
   if (at.seq < 0) return;
   const int seq = __builtin_amdgcn_readfirstlane(at.seq), r0 = __builtin_amdgcn_readfirstlane(at.r0);
   const SeqInfo sq = paged_seq(p.b, seq);
@@ -852,18 +856,19 @@ __global__ __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) void paged_chunk_kernel(
 // ---- many rows per sequence, f32 ---------------------------------------------------------------------------------------------------------------
 //
 // The exact-f32 mode: a workgroup of 4 waves takes 64 packed rows, 16 per wave, on 16x16x4 matrix instructions, which bound it (32 cycles for 2048 flop;
-// reading the fragments from LDS takes a quarter of that).  Tiles of 32 keys through a ring that the waves share, as
-// cached bytes: 8-bit ones are widened where they are read.
+// reading the fragments from LDS takes a quarter of that).  Tiles of 32 keys (f32 at head_dim 128: 16, so that three workgroups share a CU: 256 new tokens of 8
+// sequences over 4096, 28 / 4 heads 1060 us, 110 TFLOP/s, against 1100 with two of 32 keys) through a ring that the waves share, as cached bytes: 8-bit ones
+// are widened where they are read.
 template <bool F8, int HD>
-__global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnKArgs p) {
-  constexpr int NW = 4, ROWS = NW * 16, KT = 32, RB = HD * (F8 ? 1 : 4), IMG = KT * RB, STAGE = 2 * IMG + (F8 ? 256 : 0), NSTAGE = STAGE > 16 * 1024 ? 2 : 4;
+__global__ __launch_bounds__(256, 3) void paged_rows_f32_kernel(const PagedAttnKArgs p) {
+  constexpr int NW = 4, ROWS = NW * 16, KT = !F8 && HD == 128 ? 16 : 32, NKT = KT / 16, RB = HD * (F8 ? 1 : 4), IMG = KT * RB, STAGE = 2 * IMG + (F8 ? 256 : 0), NSTAGE = F8 ? 4 : 3;
   constexpr int NCH = RB / 16, RPI = 1024 / RB, NI = IMG / 1024, NSEG = 2 * NI / NW, VM = NSEG + (F8 ? 1 : 0), NDT = HD / 16, NQ = HD / (F8 ? 64 : 16);
   __shared__ __attribute__((aligned(1024))) char smem[NSTAGE * STAGE];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), qi = lane & 15, g = lane >> 4;
   const int G = p.group, KV = p.kv.n_kv_heads;
   const int kvh = blockIdx.x % KV, unit = blockIdx.x / KV, split = unit / p.tiles;
-  const TileAt at = wave_find_tile<ROWS>(p.b, G, unit - split * p.tiles, lane);
+  const TileAt at = wave_find_tile<ROWS>(p.b, G, p.tiles - 1 - (unit - split * p.tiles), lane);      // the last rows, which see the most keys, first
   if (at.seq < 0) return;
   const int seq = __builtin_amdgcn_readfirstlane(at.seq), r0 = __builtin_amdgcn_readfirstlane(at.r0);
   const SeqInfo sq = paged_seq(p.b, seq);
@@ -892,10 +897,10 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
   const int64_t page_bytes = p.kv.page_stride * (F8 ? 1 : 4);
   const char* zero = reinterpret_cast<const char*>(kZeroRows);
   bool bad_page = false;
-  int page[2];                                         // of the two halves of the next tile to fetch
+  int page[NKT];                                         // of the two halves of the next tile to fetch
   auto next_pages = [&](int kt0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < NKT; ++j) {
       page[j] = -1;
       if (kt0 + 16 * j < kend) { page[j] = uniform_page(p, seq, kt0 + 16 * j, shift); bad_page |= page[j] < 0; }
     }
@@ -903,7 +908,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
   auto issue = [&](int kt0, int slot) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < NSEG; ++j) {
-      const int u = wave + NW * j, i = u % NI, key = kt0 + i * RPI, lrow = i * RPI + lane / NCH, pg = i * RPI < 16 ? page[0] : page[1];
+      const int u = wave + NW * j, i = u % NI, key = kt0 + i * RPI, lrow = i * RPI + lane / NCH, pg = i * RPI < 16 ? page[0] : page[NKT - 1];
       const char* base = reinterpret_cast<const char*>(u < NI ? p.kv.K : p.kv.V);
       const char* src = pg < 0 ? zero : base + (int64_t)pg * page_bytes + ((int64_t)kvh * p.kv.page_size + (key & pmask)) * RB;
       if (kt0 + KT > kend && kt0 + lrow >= kend) src = zero;      // behind the context: whatever the page holds must not meet a zero
@@ -911,7 +916,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
       __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(smem + slot * STAGE + u * 1024), 16, 0, 0);
     }
     if constexpr (F8) {                                // (every wave the same 64 scales: one instruction, and the same count of them in every wave)
-      const int key = kt0 + (lane & 31), pg = (lane & 16) ? page[1] : page[0];
+      const int key = kt0 + (lane & 31), pg = (lane & 16) ? page[NKT - 1] : page[0];
       const float* base = lane < 32 ? p.kv.k_scale : p.kv.v_scale;
       const float* src = pg < 0 || key >= kend ? reinterpret_cast<const float*>(zero)
                                                : base + (int64_t)pg * p.kv.scale_stride + (int64_t)kvh * p.kv.page_size + (key & pmask);
@@ -938,28 +943,31 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
     const char* sV = sK + IMG;
     const float* sc = reinterpret_cast<const float*>(sK + 2 * IMG);
 
-    f32x4 s[2];
+    f32x4 s[2];                                        // (of a 16-key tile: the two halves of its sums)
     s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int b = 0; b < NQ; ++b) {
-      Chunk16 kc[2];
+      Chunk16 kc[NKT];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) kc[kt] = *reinterpret_cast<const Chunk16*>(sK + (kt * 16 + qi) * RB + (((b * 4 + g) ^ swizzle<RB>(qi)) << 4));      // (+ 16 rows: the same swizzle)
+      for (int kt = 0; kt < NKT; ++kt) kc[kt] = *reinterpret_cast<const Chunk16*>(sK + (kt * 16 + qi) * RB + (((b * 4 + g) ^ swizzle<RB>(qi)) << 4));      // (+ 16 rows: the same swizzle)
 #pragma unroll
       for (int w = 0; w < (F8 ? 4 : 1); ++w) {
-        float x[2][4];
+        float x[NKT][4];
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
+        for (int kt = 0; kt < NKT; ++kt) {
           if constexpr (F8) e4m3_to_f32(kc[kt].v[w], x[kt]);
           else chunk_to_f32<float>(kc[kt], x[kt]);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int kt = 0; kt < 2; ++kt)              // chains of products that do not wait for each other
-            s[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[kt][e], __builtin_bit_cast(f32x4, qf[b][w].v)[e], s[kt], 0, 0, 0);
+          for (int kt = 0; kt < NKT; ++kt) {          // chains of products that do not wait for each other
+            const int c = NKT == 2 ? kt : e & 1;
+            s[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[kt][e], __builtin_bit_cast(f32x4, qf[b][w].v)[e], s[c], 0, 0, 0);
+          }
       }
     }
+    if constexpr (NKT == 1) s[0] += s[1];
     auto v_at = [&](int krow, int d) -> float {
       const int byte = d * (F8 ? 1 : 4);
       const char* a = sV + krow * RB + (((byte >> 4) ^ swizzle<RB>(krow)) << 4) + (byte & 15);
@@ -979,7 +987,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
     }
     float mt = -INFINITY;
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
+    for (int kt = 0; kt < NKT; ++kt) {
       f32x4 ks = f32x4{p.scale2, p.scale2, p.scale2, p.scale2};
       if constexpr (F8) ks *= *reinterpret_cast<const f32x4*>(sc + kt * 16 + 4 * g);
 #pragma unroll
@@ -1000,7 +1008,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
     const float m_use = m_run == -INFINITY ? 0.f : m_run;
     float sum = 0.f;
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
+    for (int kt = 0; kt < NKT; ++kt) {
       f32x4 vs = f32x4{1.f, 1.f, 1.f, 1.f};
       if constexpr (F8) vs = *reinterpret_cast<const f32x4*>(sc + 32 + kt * 16 + 4 * g);
 #pragma unroll
@@ -1017,7 +1025,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
       for (int k = 0; k < KT; ++k) {
         float e = 0.f;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int kt = 0; kt < NKT; ++kt)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if ((k & 3) == i && (k >> 4) == kt) e = s[kt][i];
@@ -1034,7 +1042,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_f32_kernel(const PagedAttnK
       }
     }
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < NKT; ++kt)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1153,42 +1161,46 @@ int cu_count() {
 // How a call is laid out: by its sizes' bounds alone, since the lengths are on the device.
 //   decode  up to 16 packed rows per sequence: the streaming kernel.  Eight waves a workgroup where that gives every one of few workgroups a CU, two where
 //           there are more (two workgroups side by side: 97 rows of 6000 keys 145 us, eight waves 160).
-//   chunk   more: 128 packed rows a workgroup, two side by side; in bf16 256 at head_dim 128 for even batches whose context is long against the new
-//           tokens, where keys are fetched once per 256 rows and few tiles are cut by the diagonal (2048 new tokens over 16384, 32 / 8 heads: 582 us against
-//           628; a prompt of 8192 alone: 746 against 734).
+//   chunk   more.  f32: 64 packed rows a workgroup, three side by side.  bf16: 128, two side by side; at head_dim 128 256 rows, which fetch the keys once for
+//           twice as many, unless most sequences bring far less than the longest (2048 new tokens over 16384, 32 / 8 heads: 500 us against 543; a prompt
+//           of 8192 549 against 578; 8 ragged prompts up to 2000 208 against 218; 6 chunks up to 512 among 24 single tokens 186 against 167).
 //   split   keys per workgroup.  Single tokens: as many splits as give two rounds of workgroups, rounded down where there are many (131072 keys of 3
-//           sequences: 40 splits fill 1.9 rounds, 161 us; 43 begin a third, 193) and up where there are few.  Chunks of an even batch: the number
-//           that leaves the last round fullest, against 3 % of a full round for each (1024 new tokens over 32768, 40 / 8 heads, 160 workgroups: 707 us,
-//           unsplit 872).  A ragged one: two rounds, since its longest sequence else runs on alone (24 sequences, 5 of them chunks of up to 701: 83 us,
-//           unsplit 128).
+//           sequences: 40 splits fill 1.9 rounds, 161 us; 43 begin a third, 193) and up where there are few.  bf16 chunks of an even batch: the number
+//           that leaves the last round fullest, against 3 % of a full round for each (1024 new tokens over 32768, 40 / 8 heads, 160 workgroups: 680 us,
+//           unsplit 880).  The others: two rounds, since a ragged batch's longest sequence else runs on alone (24 sequences, 5 of them chunks of up to
+//           701: 76 us, unsplit 131); in bf16 with a last split that is short, so that only the longest sequences have one and the short work comes
+//           last (2.6 % over 15 ragged batches, 0 .. 13 %; the 256 keys' grain already does that to f32's many short ones).
 struct Plan { int64_t tiles; int split, splits, nw; bool decode; };
 Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
   Plan pl;
   const int G = a.n_heads / kv.n_kv_heads, cus = cu_count();
   const int64_t packed = (int64_t)b.rows * G;
+  const bool f32 = kv.dtype == DT_F32;
   const bool even = b.rows >= (int64_t)b.n_seqs * b.max_q;      // all sequences bring max_q tokens
   pl.decode = (int64_t)b.max_q * G <= 16;
-  pl.nw = !pl.decode && kv.dtype == DT_BF16 && kv.head_dim == 128 && even && (int64_t)b.max_q * G > 128 && b.max_ctx >= 4ll * b.max_q ? 8 : 4;
-  const int rows = kv.dtype == DT_F32 ? 64 : 32 * pl.nw;
+  pl.nw = !pl.decode && !f32 && kv.head_dim == 128 && (int64_t)b.max_q * G > 128 && 2ll * b.rows >= (int64_t)b.n_seqs * b.max_q ? 8 : 4;
+  const int rows = f32 ? 64 : 32 * pl.nw;
   pl.tiles = pl.decode ? b.n_seqs : std::min<int64_t>(packed / rows + b.n_seqs, b.n_seqs * ceil_div64((int64_t)b.max_q * G, rows));
   const int64_t wgs = std::max<int64_t>(1, pl.tiles * kv.n_kv_heads);
-  const int64_t slots = (int64_t)cus * (pl.nw == 8 ? 1 : 2);      // workgroups side by side
+  const int64_t slots = (int64_t)cus * (pl.decode ? 2 : f32 ? 3 : pl.nw == 8 ? 1 : 2);      // workgroups side by side
   pl.split = a.split_keys;
   if (!pl.split) {
     if (pl.decode && wgs <= cus && b.max_ctx <= 1024) pl.split = 1024;
     else {
       const int64_t down = 2 * slots / wgs, up = ceil_div64(2 * slots, wgs);
-      int64_t n = pl.decode ? (down >= 8 ? down : up) : up;
-      if (!pl.decode && even) {
-        const double each = 0.03 * (double)std::min(wgs, slots) / slots;
-        double best = 1e30;
-        n = 1;
-        for (int i = 1; i <= 64; ++i) {
-          const double cost = (double)ceil_div64(wgs * i, slots) / i + each * (i - 1);
-          if (cost < best) best = cost, n = i;
+      int64_t n = std::max<int64_t>(1, pl.decode ? (down >= 8 ? down : up) : up), tenths = 10 * n;
+      if (!pl.decode && !f32) {
+        if (!even) tenths -= n > 1 ? 2 : 0;
+        else {
+          const double each = 0.03 * (double)std::min(wgs, slots) / slots;
+          double best = 1e30;
+          for (int i = 1; i <= 64; ++i) {
+            const double cost = (double)ceil_div64(wgs * i, slots) / i + each * (i - 1);
+            if (cost < best) best = cost, tenths = 10 * i;
+          }
         }
       }
-      pl.split = (int)std::max<int64_t>(512, ceil_div64(ceil_div64(b.max_ctx, std::max<int64_t>(1, n)), 256) * 256);
+      pl.split = (int)std::max<int64_t>(f32 && !pl.decode ? 256 : 512, ceil_div64(ceil_div64(10ll * b.max_ctx, tenths), 256) * 256);
     }
   }
   pl.splits = ceil_div(b.max_ctx, pl.split);

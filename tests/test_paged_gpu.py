@@ -358,6 +358,19 @@ def test_attention_split_by_the_caller_is_the_same_in_any_batch(fmt, new):
     assert all(torch.equal(x, every[s]) for s, x in enumerate(some([0, 1, 2, 3])))
 
 
+@pytest.mark.parametrize("dtype,fmt", [("bf16", "same"), ("bf16", "e4m3"), ("f32", "same")])
+def test_attention_of_chunks_among_single_tokens_is_that_of_chunks_alone(dtype, fmt):
+    """split_keys given and the same max_q: chunks of one batch have the same bits beside ten single tokens, where workgroups hold fewer rows."""
+    new, lens = [90, 77, 41] + [1] * 10, [700, 1300, 41] + [60 + 150 * i for i in range(10)]
+    pool = Pool(2, 128, 32, dtype, fmt, lens)
+    pool.fill(lens)
+    q = rnd(sum(new), 8, 128, seed=2, dtype=tdt(dtype)).to(DEV)
+    every = pool.batch(new, lens)
+    few = paged.PagedBatch(every.cu_q[:4].clone(), every.ctx_len[:3].clone(), every.table[:3], max_q=90, max_ctx=1300)
+    alone = paged.attention(pool.kv, few, q[:sum(new[:3])], split_keys=512)
+    assert torch.equal(paged.attention(pool.kv, every, q, split_keys=512)[:sum(new[:3])], alone)
+
+
 @pytest.mark.parametrize("dtype,H,KV,d", [("bf16", 8, 2, 128), ("f32", 4, 2, 64)])
 @pytest.mark.parametrize("new", [1, 60])
 def test_attention_infinite_values_that_are_seen(dtype, H, KV, d, new):
