@@ -39,6 +39,13 @@ __host__ __device__ __forceinline__ SeqInfo paged_seq(const PagedBatch& b, int s
   return i;
 }
 
+// Reports any bad sequence of the batch, those that bring no rows among them: one wave of a launch.
+__device__ __forceinline__ void report_bad_lengths(const PagedKv& kv, const PagedBatch& b, int lane) {
+  bool bad = false;
+  for (int s = lane; s < b.n_seqs; s += 64) bad |= paged_seq(b, s).bad;
+  if (bad) paged_report(kv.status, kBadLength);
+}
+
 // The page that holds place `pos` (0 <= pos < max_ctx) of sequence s; -1: its number is none of the pool's.
 __host__ __device__ __forceinline__ int paged_page(const PagedKv& kv, const PagedBatch& b, int s, int pos, int page_shift) {
   const int page = b.table[(int64_t)s * b.ld_table + (pos >> page_shift)];

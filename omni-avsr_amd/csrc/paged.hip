@@ -67,7 +67,11 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(const QkRopeArgs p, c
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t task = (int64_t)blockIdx.x * kWaves + wave;
   const int row = (int)(task / parts), part = (int)(task - (int64_t)row * parts);
-  if (row >= p.rows) return;
+  if (row >= p.rows) {
+    if constexpr (CACHE)
+      if (wave == 0) report_bad_lengths(pages.kv, pages.b, lane);      // the workgroup behind the rows
+    return;
+  }
 
   int pos = 0, page = -1, off = 0;
   if constexpr (CACHE) {
@@ -75,7 +79,6 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(const QkRopeArgs p, c
     const PagedBatch& b = pages.b;
     const int s = wave_find_seq(b.cu_q, b.n_seqs, row, lane);
     const SeqInfo q = paged_seq(b, s);
-    if (q.bad && lane == 0 && part == 0) paged_report(kv.status, kBadLength);
     if (row < q.q0 || row >= q.q0 + q.nq) return;    // behind the last sequence, or of a skipped one
     pos = q.ctx - (q.nq - (row - q.q0));
     if (pos < 0) return;
@@ -198,11 +201,13 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(const PagedKv kv, 
   constexpr int LPH = HD / 16, HPW = 64 / LPH;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t task = (int64_t)blockIdx.x * kWaves + wave;
-  if (task >= b.rows) return;
+  if (task >= b.rows) {
+    if (wave == 0) report_bad_lengths(kv, b, lane);      // the workgroup behind the rows
+    return;
+  }
   const int row = (int)task;
   const int s = wave_find_seq(b.cu_q, b.n_seqs, row, lane);
   const SeqInfo q = paged_seq(b, s);
-  if (q.bad && lane == 0) paged_report(kv.status, kBadLength);
   if (row < q.q0 || row >= q.q0 + q.nq) return;
   const int pos = q.ctx - (q.nq - (row - q.q0));
   if (pos < 0) return;
@@ -267,7 +272,7 @@ template <typename T, bool CACHE, bool F8>
 int launch_rope_t(const QkRopeArgs& a, const PagedKv& kv, const PagedBatch& b, hipStream_t st) {
   const int hpw = 64 / (a.head_dim / 16), heads = a.n_heads + (CACHE ? 2 : 1) * a.n_kv_heads;
   const int parts = a.rows >= kManyRows ? 1 : ceil_div(heads, hpw);
-  const int64_t blocks = ceil_div64((int64_t)a.rows * parts, kWaves);
+  const int64_t blocks = ceil_div64((int64_t)a.rows * parts, kWaves) + (CACHE ? 1 : 0);
   OAVSR_REQUIRE(blocks < (1ll << 31), "paged: %d rows are too many for one launch", a.rows);
   std::conditional_t<CACHE, Pages, NoPages> pages;
   if constexpr (CACHE) { pages.kv = kv; pages.b = b; }
@@ -279,7 +284,7 @@ int launch_rope_t(const QkRopeArgs& a, const PagedKv& kv, const PagedBatch& b, h
 
 template <typename T, bool F8>
 int launch_read_t(const PagedKv& kv, const PagedBatch& b, void* k_out, int64_t ldk, void* v_out, int64_t ldv, hipStream_t st) {
-  const dim3 grid(ceil_div(b.rows, kWaves));
+  const dim3 grid(ceil_div(b.rows, kWaves) + 1);
   if (kv.head_dim == 64) hipLaunchKernelGGL((paged_read_kernel<T, 64, F8>), grid, dim3(kThreads), 0, st, kv, b, (T*)k_out, ldk, (T*)v_out, ldv);
   else hipLaunchKernelGGL((paged_read_kernel<T, 128, F8>), grid, dim3(kThreads), 0, st, kv, b, (T*)k_out, ldk, (T*)v_out, ldv);
   OAVSR_CHECK_HIP(hipGetLastError());

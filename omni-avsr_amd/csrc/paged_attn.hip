@@ -555,11 +555,11 @@ __global__ __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) void paged_chunk_kernel(
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ql = lane & 31, h = lane >> 5;
   const int G = p.group, KV = p.kv.n_kv_heads;
   const int kvh = blockIdx.x % KV, unit = blockIdx.x / KV, split = unit / p.tiles;
+  if (blockIdx.x == 0 && wave == 0) report_bad_lengths(p.kv, p.b, lane);
   const TileAt at = wave_find_tile<ROWS>(p.b, G, p.tiles - 1 - (unit - split * p.tiles), lane);      // the last rows, which see the most keys, first
   if (at.seq < 0) return;
   const int seq = __builtin_amdgcn_readfirstlane(at.seq), r0 = __builtin_amdgcn_readfirstlane(at.r0);
   const SeqInfo sq = paged_seq(p.b, seq);
-  if (sq.bad && tid == 0) paged_report(p.kv.status, kBadLength);
   const int packed = sq.nq * G;
   const int first_pos = sq.ctx - sq.nq, kmax = min(sq.ctx, p.b.max_ctx);
   const int kend_all = max(0, min(first_pos + (min(r0 + ROWS, packed) - 1) / G + 1, kmax));
@@ -868,11 +868,11 @@ __global__ __launch_bounds__(256, 3) void paged_rows_f32_kernel(const PagedAttnK
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), qi = lane & 15, g = lane >> 4;
   const int G = p.group, KV = p.kv.n_kv_heads;
   const int kvh = blockIdx.x % KV, unit = blockIdx.x / KV, split = unit / p.tiles;
+  if (blockIdx.x == 0 && wave == 0) report_bad_lengths(p.kv, p.b, lane);
   const TileAt at = wave_find_tile<ROWS>(p.b, G, p.tiles - 1 - (unit - split * p.tiles), lane);      // the last rows, which see the most keys, first
   if (at.seq < 0) return;
   const int seq = __builtin_amdgcn_readfirstlane(at.seq), r0 = __builtin_amdgcn_readfirstlane(at.r0);
   const SeqInfo sq = paged_seq(p.b, seq);
-  if (sq.bad && tid == 0) paged_report(p.kv.status, kBadLength);
   const int packed = sq.nq * G;
   const int first_pos = sq.ctx - sq.nq, kmax = min(sq.ctx, p.b.max_ctx);
   const int kend_all = max(0, min(first_pos + (min(r0 + ROWS, packed) - 1) / G + 1, kmax));

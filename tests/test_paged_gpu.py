@@ -563,6 +563,22 @@ def test_bad_pages_and_lengths_are_reported_and_harmless():
     assert torch.equal(out[:4], want[:4]) and out[4:].isfinite().all()
 
 
+@pytest.mark.parametrize("cu,lens", [([0, 5, 3, 8], [64, 64, 64]), ([0, 4, 4, 8], [64, -1, 64]), ([0, 4, 4, 8], [64, 65, 64])])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_bad_sequences_without_rows_are_reported_by_every_call(dtype, cu, lens):
+    H, KV, d, page = 4, 2, 64, 16
+    pool = Pool(KV, d, page, dtype, "same", [64, 64, 64])
+    pool.fill([64, 64, 64])
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    rows, q = rnd(8, (H + 2 * KV) * d, seed=2, dtype=tdt(dtype)).to(DEV), rnd(8, H, d, seed=1, dtype=tdt(dtype)).to(DEV)
+    few, many = (paged.PagedBatch(i32(cu), i32(lens), pool.table.to(DEV), max_q=m, max_ctx=64) for m in (5, 20))
+    for call in (lambda: paged.append(pool.kv, few, rows), lambda: paged.read(pool.kv, few, 8), lambda: paged.attention(pool.kv, few, q), lambda: paged.attention(pool.kv, many, q)):
+        pool.kv.check()
+        call()
+        with pytest.raises(RuntimeError, match="length"):
+            pool.kv.check()
+
+
 # ---- refusals of the tensor layer ---------------------------------------------------------------------------------------------------------------
 def test_refusals():
     H, KV, d = 4, 2, 64
