@@ -7,8 +7,8 @@ A decoder layer with its cache in pages runs, per step,
 
 with one `PagedKV` per layer (its pool of pages) and one `PagedBatch` per step (row offsets, lengths and page table of the sequences, shared by all layers).
 Everything is queued on the current stream of the tensors' device; nothing is synchronised, and every call can be captured into a graph.  An argument that
-does not fit raises ValueError before anything is queued.  Lengths and page numbers are device data: a bad one never reaches memory outside the given
-tensors, and sets its bit in `PagedKV.status` (`PagedKV.check()` raises)."""
+does not fit raises ValueError before anything is queued, and so does one that asks for gradients: these are forward passes.  Lengths and page numbers are
+device data: a bad one never reaches memory outside the given tensors, and sets its bit in `PagedKV.status` (`PagedKV.check()` raises)."""
 from __future__ import annotations
 
 import ctypes as C
@@ -25,6 +25,10 @@ _E4M3 = torch.float8_e4m3fn
 def _need(ok, what):
     if not ok:
         raise ValueError("paged: " + what)
+
+
+def _no_gradient(name):
+    _need(not torch.is_grad_enabled(), f"{name} asks for gradients, and none are formed here: call under torch.no_grad(), or detach it")
 
 
 def _on_gpu(t, name, dtype, index=None):
@@ -189,6 +193,8 @@ def _vector(t, name, dtype, index, n=None):
     if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index and t.dim() == 1 and (n is None or t.numel() == n) and t.is_contiguous()):
         _on_gpu(t, name, dtype, index)
         _need(False, f"{name} is {tuple(t.shape)} (strides {t.stride()}), a vector{'' if n is None else f' of {n}'} in one piece is wanted")
+    if t.requires_grad:
+        _no_gradient(name)
     return t.data_ptr()
 
 
@@ -212,6 +218,8 @@ def qk_norm_rope(qkv, n_heads, n_kv_heads, pos, inv_freq, *, q_gain=None, k_gain
     inv_freq [rot_dim / 2]: the first rot_dim dimensions of a head turn, halves against each other, or neighbours when interleaved."""
     if not (isinstance(qkv, torch.Tensor) and qkv.dim() == 2 and qkv.dtype in _DT and qkv.is_cuda):
         _need(False, "qkv has to be rows of float32 or bfloat16 on a GPU")
+    if qkv.requires_grad:
+        _no_gradient("qkv")
     rows, width = qkv.shape
     dtype, index, all_heads = qkv.dtype, qkv.get_device(), n_heads + 2 * n_kv_heads
     if _device() != index:
@@ -244,6 +252,8 @@ def append(kv, batch, qkv, inv_freq=None, *, pos=None, q_gain=None, k_gain=None,
     if _device() != index:
         with torch.cuda.device(index):
             return append(kv, batch, qkv, inv_freq, pos=pos, q_gain=q_gain, k_gain=k_gain, eps=eps, interleaved=interleaved, rot_scale=rot_scale, out=out)
+    if qkv.requires_grad:
+        _no_gradient("qkv")
     rows, width = qkv.shape
     dtype = qkv.dtype
     desc = kv._for(dtype)
@@ -302,7 +312,7 @@ def read(kv, batch, rows=None, *, dtype=None, out=None):
 
 def attention(kv, batch, q, scale=None, *, out=None, lse=None, split_keys=0):
     """Causal attention of the batch's new tokens q [rows][n_heads][head_dim] (or [rows][n_heads * head_dim]) over their sequences' cached context.  Returns
-    out, shaped like q.  scale: default head_dim ** -0.5.  lse: float32 [rows][n_heads] to fill.  split_keys: keys per workgroup (a multiple of 256; 0: the
+    out, shaped like q (which it may be).  scale: default head_dim ** -0.5.  lse: float32 [rows][n_heads] to fill.  split_keys: keys per workgroup (a multiple of 256; 0: the
     library's rule), for results whose last bits do not follow the batch a row is in."""
     index, head_dim = kv.index, kv.head_dim
     if not (isinstance(q, torch.Tensor) and q.dim() in (2, 3) and q.is_cuda):
@@ -310,6 +320,8 @@ def attention(kv, batch, q, scale=None, *, out=None, lse=None, split_keys=0):
     if _device() != index:
         with torch.cuda.device(index):
             return attention(kv, batch, q, scale, out=out, lse=lse, split_keys=split_keys)
+    if q.requires_grad:
+        _no_gradient("q")
     dtype, shape = q.dtype, q.shape
     desc, rows = kv._for(dtype), shape[0]
     width = shape[1] * shape[2] if len(shape) == 3 else shape[1]

@@ -371,6 +371,18 @@ def test_attention_of_chunks_among_single_tokens_is_that_of_chunks_alone(dtype, 
     assert torch.equal(paged.attention(pool.kv, every, q, split_keys=512)[:sum(new[:3])], alone)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("new", [[1, 2], [90, 3, 40]])
+def test_attention_into_its_queries(dtype, new):
+    ctx = [700 + 13 * n for n in new]
+    pool = Pool(2, 128, 16, dtype, "same", ctx)
+    pool.fill(ctx)
+    q, b = rnd(sum(new), 4, 128, seed=5, dtype=tdt(dtype)).to(DEV), pool.batch(new, ctx)
+    for split in (0, 256, 1024):
+        want, buf = paged.attention(pool.kv, b, q, split_keys=split), q.clone()
+        assert paged.attention(pool.kv, b, buf, out=buf, split_keys=split) is buf and torch.equal(buf, want)
+
+
 @pytest.mark.parametrize("dtype,H,KV,d", [("bf16", 8, 2, 128), ("f32", 4, 2, 64)])
 @pytest.mark.parametrize("new", [1, 60])
 def test_attention_infinite_values_that_are_seen(dtype, H, KV, d, new):
@@ -606,6 +618,14 @@ def test_refusals():
     }
     for word, call in calls.items():
         with pytest.raises(ValueError, match=word.split(" nan")[0] if word != "v \\(" else "v"):
+            call()
+    # no gradients are formed: asking for them is refused, and a call under no_grad is none that asks
+    gain, freq = torch.ones(d, device=DEV, requires_grad=True), z(32, dt=torch.float32)
+    for call in (lambda: paged.attention(kv, b, q.clone().requires_grad_()), lambda: paged.append(kv, b, qkv.clone().requires_grad_()),
+                 lambda: paged.qk_norm_rope(qkv.clone().requires_grad_(), H, KV, i32(0, 1), freq), lambda: paged.append(kv, b, qkv, q_gain=gain, k_gain=gain)):
+        with pytest.raises(ValueError, match="gradients"):
+            call()
+        with torch.no_grad():
             call()
     # empty calls are calls
     none = paged.PagedBatch(i32(0), i32(), torch.zeros(0, 0, dtype=torch.int32, device=DEV), max_q=0, max_ctx=0)
