@@ -231,7 +231,8 @@ def qk_norm_rope(qkv, n_heads, n_kv_heads, pos, inv_freq, *, q_gain=None, k_gain
     at_freq, rot = (None, 0) if inv_freq is None else (_vector(inv_freq, "inv_freq", torch.float32, index), 2 * inv_freq.numel())
     at_pos = None if pos is None else _vector(pos, "pos", torch.int32, index, rows)
     at_q, at_k = _gains(q_gain, k_gain, index, head_dim)
-    ld, ldq, ldk = _rows_of(qkv, "qkv", width, dtype, index), n_heads * head_dim, n_kv_heads * head_dim
+    ld = width if rows and qkv.is_contiguous() else _rows_of(qkv, "qkv", width, dtype, index)
+    ldq, ldk = n_heads * head_dim, n_kv_heads * head_dim
     if out is None:
         q, k = qkv.new_empty((rows, n_heads, head_dim)), qkv.new_empty((rows, n_kv_heads, head_dim))
     else:
@@ -260,7 +261,7 @@ def append(kv, batch, qkv, inv_freq=None, *, pos=None, q_gain=None, k_gain=None,
     n_heads = width // head_dim - 2 * heads
     if not (n_heads > 0 and width % head_dim == 0):
         _need(False, f"rows of {width} values do not hold query heads beside 2 x {heads} heads of {head_dim}")
-    ld = _rows_of(qkv, "qkv", width, dtype, index)
+    ld = width if rows and qkv.is_contiguous() and qkv.get_device() == index else _rows_of(qkv, "qkv", width, dtype, index)
     at_freq, rot = (None, 0) if inv_freq is None else (_vector(inv_freq, "inv_freq", torch.float32, index), 2 * inv_freq.numel())
     at_pos = None if pos is None else _vector(pos, "pos", torch.int32, index, rows)
     at_q, at_k = _gains(q_gain, k_gain, index, head_dim)
@@ -329,12 +330,12 @@ def attention(kv, batch, q, scale=None, *, out=None, lse=None, split_keys=0):
     if not (width % head_dim == 0 and (len(shape) == 2 or shape[2] == head_dim)):
         _need(False, f"q is {tuple(shape)}, the cache's heads have {head_dim} dimensions")
     scale = head_dim ** -0.5 if scale is None else scale
-    ldq = _rows_of(q, "q", width, dtype, index)
+    ldq = width if rows and q.is_contiguous() and q.get_device() == index else _rows_of(q, "q", width, dtype, index)
     b = batch._for(rows, kv)
     need = batch._workspace(b, kv, dtype, n_heads, split_keys)
     ldo = width
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q) if ldq == width else q.new_empty(shape)
     else:
         ldo = _rows_of(out, "out", width, dtype, index, rows, True)
     at_lse = None
