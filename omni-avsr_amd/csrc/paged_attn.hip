@@ -1094,8 +1094,9 @@ __global__ __launch_bounds__(256, 3) void paged_rows_f32_kernel(const PagedAttnK
 }
 
 // Joins the splits of the rows whose keys lie in more than one:  out = sum_z w_z O_z / sum_z w_z,  w_z = l_z 2^(m_z - max m).  NG groups of HD / 4 threads share
-// a (row, head), each taking every NG-th split, joined in LDS in a fixed order: one group where the splits are few and the rows many, all of a
-// workgroup's where it is the other way round.
+// a (row, head), each taking every NG-th split, joined in LDS in a fixed order: all of a workgroup's where the splits are many, and one where they are
+// at most kFewSplits, with all of them on their way at once.  A row of few splits gets the same bits from both.
+constexpr int kFewSplits = 8;
 template <typename T, int HD, int NG>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnKArgs p) {
   constexpr int TPG = HD / 4, PER = kThreads / (TPG * NG);      // (row, head) pairs per workgroup: heads of one row
@@ -1111,7 +1112,31 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnKA
   if (n <= 1) return;
   float m = -INFINITY, l = 0.f;
   f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (head < p.n_heads) {
+  if (NG == 1 && head < p.n_heads) {
+    float2 ml[kFewSplits];
+    f32x4 x[kFewSplits];
+#pragma unroll
+    for (int z = 0; z < kFewSplits; ++z) {
+      ml[z] = make_float2(-INFINITY, 0.f);
+      x[z] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (z < n) {
+        const int64_t at = ((int64_t)z * p.b.rows + row) * p.n_heads + head;
+        ml[z] = p.part_ml[at];
+        x[z] = *reinterpret_cast<const f32x4*>(p.part + at * HD + d0);
+      }
+    }
+#pragma unroll
+    for (int z = 0; z < kFewSplits; ++z) m = fmaxf(m, ml[z].x);
+    const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int z = 0; z < kFewSplits; ++z) {
+      const float w = __builtin_amdgcn_exp2f(ml[z].x - mu);
+      l = fmaf(w, ml[z].y, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, ml[z].y * x[z][e], acc[e]);
+    }
+  }
+  if (NG > 1 && head < p.n_heads) {
 #pragma unroll 2
     for (int z = grp; z < n; z += NG) {
       const int64_t at = ((int64_t)z * p.b.rows + row) * p.n_heads + head;
@@ -1160,12 +1185,12 @@ int cu_count() {
 
 // How a call is laid out: by its sizes' bounds alone, since the lengths are on the device.
 //   decode  up to 16 packed rows per sequence: the streaming kernel.  Eight waves a workgroup where that gives every one of few workgroups a CU, two where
-//           there are more (two workgroups side by side: 97 rows of 6000 keys 145 us, eight waves 160).
+//           there are more (two workgroups side by side: 97 rows of 6000 keys 124 us, eight waves 135).
 //   chunk   more.  f32: 64 packed rows a workgroup, three side by side.  bf16: 128, two side by side; at head_dim 128 256 rows, which fetch the keys once for
 //           twice as many, unless most sequences bring far less than the longest (2048 new tokens over 16384, 32 / 8 heads: 500 us against 543; a prompt
 //           of 8192 549 against 578; 8 ragged prompts up to 2000 208 against 218; 6 chunks up to 512 among 24 single tokens 186 against 167).
 //   split   keys per workgroup.  Single tokens: as many splits as give two rounds of workgroups, rounded down where there are many (131072 keys of 3
-//           sequences: 40 splits fill 1.9 rounds, 161 us; 43 begin a third, 193) and up where there are few.  bf16 chunks of an even batch: the number
+//           sequences: 40 splits fill 1.9 rounds, 139 us; 43 begin a third, 168) and up where there are few.  bf16 chunks of an even batch: the number
 //           that leaves the last round fullest, against 3 % of a full round for each (1024 new tokens over 32768, 40 / 8 heads, 160 workgroups: 680 us,
 //           unsplit 880).  The others: two rounds, since a ragged batch's longest sequence else runs on alone (24 sequences, 5 of them chunks of up to
 //           701: 76 us, unsplit 131); in bf16 with a last split that is short, so that only the longest sequences have one and the short work comes
@@ -1238,7 +1263,8 @@ int launch_t(const PagedAttnKArgs& k, const Plan& pl, hipStream_t st) {
   OAVSR_CHECK_HIP(hipGetLastError());
   if (pl.split) {
     constexpr int ALL = kThreads / (HD / 4);
-    if (pl.splits > 8) hipLaunchKernelGGL((paged_merge_kernel<T, HD, ALL>), dim3((unsigned)((int64_t)k.b.rows * k.n_heads)), dim3(kThreads), 0, st, k);
+    static_assert(ALL >= kFewSplits, "groups");
+    if (pl.splits > kFewSplits) hipLaunchKernelGGL((paged_merge_kernel<T, HD, ALL>), dim3((unsigned)((int64_t)k.b.rows * k.n_heads)), dim3(kThreads), 0, st, k);
     else hipLaunchKernelGGL((paged_merge_kernel<T, HD, 1>), dim3((unsigned)((int64_t)k.b.rows * ceil_div(k.n_heads, ALL))), dim3(kThreads), 0, st, k);
     OAVSR_CHECK_HIP(hipGetLastError());
   }

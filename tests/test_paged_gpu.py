@@ -371,6 +371,19 @@ def test_attention_of_chunks_among_single_tokens_is_that_of_chunks_alone(dtype, 
     assert torch.equal(paged.attention(pool.kv, every, q, split_keys=512)[:sum(new[:3])], alone)
 
 
+@pytest.mark.parametrize("dtype,d", [("bf16", 64), ("bf16", 128), ("f32", 128)])
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_split_by_the_caller_is_the_same_beside_a_longer_context(dtype, d, new):
+    """split_keys given: the row's splits are joined alike where another sequence has many more of them."""
+    lens = [1900, 700, 6000]
+    pool = Pool(2, d, 64, dtype, "same", lens)
+    pool.fill(lens)
+    q = rnd(3 * new, 8, d, seed=4, dtype=tdt(dtype)).to(DEV)
+    every = pool.batch([new] * 3, lens)
+    few = paged.PagedBatch(every.cu_q[:3].clone(), every.ctx_len[:2].clone(), every.table[:2], max_q=new, max_ctx=1900)
+    assert torch.equal(paged.attention(pool.kv, few, q[:2 * new], split_keys=256), paged.attention(pool.kv, every, q, split_keys=256)[:2 * new])
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("new", [[1, 2], [90, 3, 40]])
 def test_attention_into_its_queries(dtype, new):
