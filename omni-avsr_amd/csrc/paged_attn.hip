@@ -225,7 +225,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
   constexpr int RPI = 1024 / RB, NI = IMG / 1024;      // rows per DMA instruction, instructions per image
   constexpr int NSUB = KT / 16, NDT = HD / 16, NOFF = 16 / RPI;
   constexpr int VM = 2 * NI + (F8 ? 1 : 0);
-  constexpr int RING = STAGE * NS > HD * 64 + 128 ? STAGE * NS : HD * 64 + 128;      // the ring, afterwards (m, l, O) of the wave
+  constexpr int RS = 17, JOIN = HD * RS * 4 + 128;      // (m, l, O) of the wave, O's dimensions RS floats apart: lanes that read every fourth meet other banks
+  constexpr int RING = STAGE * NS > JOIN ? STAGE * NS : JOIN;      // the ring, afterwards those
   static_assert(VM * (NS - 1) <= 63, "vmcnt");
   __shared__ __attribute__((aligned(1024))) char smem[NW * RING];
 
@@ -491,12 +492,12 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
   l_run += __shfl_xor(l_run, 16, 64);
   l_run += __shfl_xor(l_run, 32, 64);
   // ---- the waves' partial results, joined in wave order
-  float* so = reinterpret_cast<float*>(ring);          // [HD][16] O^T, then [16] m, [16] l
+  float* so = reinterpret_cast<float*>(ring);          // [HD][RS] O^T, then [16] m, [16] l
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) so[dim_of(dt, 4 * g + i) * 16 + qi] = o[dt][i];
-  if (g == 0) { so[HD * 16 + qi] = m_run; so[HD * 16 + 16 + qi] = l_run; }
+    for (int i = 0; i < 4; ++i) so[dim_of(dt, 4 * g + i) * RS + qi] = o[dt][i];
+  if (g == 0) { so[HD * RS + qi] = m_run; so[HD * RS + 16 + qi] = l_run; }
   __syncthreads();
   for (int i = tid; i < packed * (HD / 4); i += NW * 64) {
     const int pr = i / (HD / 4), d0 = (i - pr * (HD / 4)) * 4, ptok = pr / G, phead = kvh * G + (pr - ptok * G);
@@ -505,16 +506,16 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
       const float* x = reinterpret_cast<const float*>(smem + w * RING);
-      m = fmaxf(m, x[HD * 16 + pr]);
+      m = fmaxf(m, x[HD * RS + pr]);
     }
     const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
       const float* x = reinterpret_cast<const float*>(smem + w * RING);
-      const float f = __builtin_amdgcn_exp2f(x[HD * 16 + pr] - mu);
-      l = fmaf(f, x[HD * 16 + 16 + pr], l);
+      const float f = __builtin_amdgcn_exp2f(x[HD * RS + pr] - mu);
+      l = fmaf(f, x[HD * RS + 16 + pr], l);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = fmaf(f, x[(d0 + j) * 16 + pr], acc[j]);
+      for (int j = 0; j < 4; ++j) acc[j] = fmaf(f, x[(d0 + j) * RS + pr], acc[j]);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int64_t prow = sq.q0 + ptok;
