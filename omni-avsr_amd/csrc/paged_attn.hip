@@ -1185,17 +1185,18 @@ int cu_count() {
 }
 
 // How a call is laid out: by its sizes' bounds alone, since the lengths are on the device.
-//   decode  up to 16 packed rows per sequence: the streaming kernel.  Eight waves a workgroup where that gives every one of few workgroups a CU, two where
-//           there are more (two workgroups side by side: 97 rows of 6000 keys 124 us, eight waves 135).
+//   decode  up to 16 packed rows per sequence: the streaming kernel.  Workgroups of eight waves where a CU is there for each sequence and kv head, of two,
+//           two side by side, where there are more of those (97 rows of 6000 keys, 4 kv heads 124 us, eight waves 135).
 //   chunk   more.  f32: 64 packed rows a workgroup, three side by side.  bf16: 128, two side by side; at head_dim 128 256 rows, which fetch the keys once for
 //           twice as many, unless most sequences bring far less than the longest (2048 new tokens over 16384, 32 / 8 heads: 500 us against 543; a prompt
 //           of 8192 549 against 578; 8 ragged prompts up to 2000 208 against 218; 6 chunks up to 512 among 24 single tokens 186 against 167).
-//   split   keys per workgroup.  Single tokens: as many splits as give two rounds of workgroups, rounded down where there are many (131072 keys of 3
-//           sequences: 40 splits fill 1.9 rounds, 139 us; 43 begin a third, 168) and up where there are few.  bf16 chunks of an even batch: the number
-//           that leaves the last round fullest, against 3 % of a full round for each (1024 new tokens over 32768, 40 / 8 heads, 160 workgroups: 680 us,
-//           unsplit 880).  The others: two rounds, since a ragged batch's longest sequence else runs on alone (24 sequences, 5 of them chunks of up to
-//           701: 76 us, unsplit 131); in bf16 with a last split that is short, so that only the longest sequences have one and the short work comes
-//           last (2.6 % over 15 ragged batches, 0 .. 13 %; the 256 keys' grain already does that to f32's many short ones).
+//   split   keys per workgroup.  Single tokens: as many splits as leave each its CU, two also where they are a little too many (1 sequence of 40000, 8 kv
+//           heads: 33 us, in two rounds of two waves 42; 3 of 131072: 129 against 138; 20 ragged up to 8000: 66 against 76), none for few keys; where
+//           workgroups are many, two rounds of them.  bf16 chunks of an even batch: the number that leaves the last round fullest, against 3 % of a full
+//           round for each (1024 new tokens over 32768, 40 / 8 heads, 160 workgroups: 680 us, unsplit 880).  The others: two rounds, since a ragged
+//           batch's longest sequence else runs on alone (24 sequences, 5 of them chunks of up to 701: 76 us, unsplit 131); in bf16 with a last split
+//           that is short, so that only the longest sequences have one and the short work comes last (2.6 % over 15 ragged batches, 0 .. 13 %; the
+//           256 keys' grain already does that to f32's many short ones).
 struct Plan { int64_t tiles; int split, splits, nw; bool decode; };
 Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
   Plan pl;
@@ -1211,27 +1212,25 @@ Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
   const int64_t slots = (int64_t)cus * (pl.decode ? 2 : f32 ? 3 : pl.nw == 8 ? 1 : 2);      // workgroups side by side
   pl.split = a.split_keys;
   if (!pl.split) {
-    if (pl.decode && wgs <= cus && b.max_ctx <= 1024) pl.split = 1024;
-    else {
-      const int64_t down = 2 * slots / wgs, up = ceil_div64(2 * slots, wgs);
-      int64_t n = std::max<int64_t>(1, pl.decode ? (down >= 8 ? down : up) : up), tenths = 10 * n;
-      if (!pl.decode && !f32) {
-        if (!even) tenths -= n > 1 ? 2 : 0;
-        else {
-          const double each = 0.03 * (double)std::min(wgs, slots) / slots;
-          double best = 1e30;
-          for (int i = 1; i <= 64; ++i) {
-            const double cost = (double)ceil_div64(wgs * i, slots) / i + each * (i - 1);
-            if (cost < best) best = cost, tenths = 10 * i;
-          }
-        }
+    const int64_t up = ceil_div64(2 * slots, wgs), least = f32 ? 256 : 512;
+    int64_t tenths = 10 * up;                                   // of as many splits
+    if (pl.decode) {
+      if (wgs <= cus) tenths = 10 * (b.max_ctx <= 2 * least ? 1 : 2 * wgs > cus && 3 * wgs <= 2 * cus ? 2 : cus / wgs);
+    } else if (!f32 && !even) {
+      tenths -= up > 1 ? 2 : 0;
+    } else if (!f32) {
+      const double each = 0.03 * (double)std::min(wgs, slots) / slots;
+      double best = 1e30;
+      for (int i = 1; i <= 64; ++i) {
+        const double cost = (double)ceil_div64(wgs * i, slots) / i + each * (i - 1);
+        if (cost < best) best = cost, tenths = 10 * i;
       }
-      pl.split = (int)std::max<int64_t>(f32 && !pl.decode ? 256 : 512, ceil_div64(ceil_div64(10ll * b.max_ctx, tenths), 256) * 256);
     }
+    pl.split = (int)std::max<int64_t>(least, ceil_div64(ceil_div64(10ll * b.max_ctx, tenths), 256) * 256);
   }
   pl.splits = ceil_div(b.max_ctx, pl.split);
   if (pl.splits <= 1) pl.split = 0, pl.splits = 1;
-  if (pl.decode) pl.nw = a.split_keys || wgs * pl.splits > cus ? 2 : 8;      // (a pinned split: the waves' shares too)
+  if (pl.decode) pl.nw = a.split_keys || wgs > cus ? 2 : 8;      // (a pinned split: the waves' shares too)
   return pl;
 }
 uint64_t workspace_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a, const Plan& pl) {
