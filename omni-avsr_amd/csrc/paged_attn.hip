@@ -210,7 +210,7 @@ __device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) { return bf16x8{a[0],
 // of a bf16 cache.  Each wave streams its own tiles of KT keys (wave, wave + NW, ...) through a private ring of NS tiles in LDS, fetched by LDS-DMA and
 // awaited by counted vmcnt, so there is no barrier in the loop and (NS - 1) tiles are on their way while one is computed.  16 keys lie in one page, so
 // an instruction's page is uniform: scalar loads, one page base per 16 keys.  The waves' (m, l, O) meet in LDS in wave order.  The cache is read once and
-// the loads say so (non-temporal): 691 MB of 97 sequences 124 us, 5.6 TB/s with the join; 143 without the hint.
+// the loads say so (non-temporal): 691 MB of 97 sequences 121 us, 5.7 TB/s with the join; without the hint 15 % more.
 constexpr int kOnce = 2;                              // nt of a load to LDS
 template <typename T, bool F8, int HD> struct DecodeShape {
   static constexpr int KT = sizeof(T) == 4 ? 16 : 32;                        // keys per wave tile
@@ -1185,13 +1185,14 @@ int cu_count() {
 }
 
 // How a call is laid out: by its sizes' bounds alone, since the lengths are on the device.
-//   decode  up to 16 packed rows per sequence: the streaming kernel.  Workgroups of eight waves where a CU is there for each sequence and kv head, of two,
-//           two side by side, where there are more of those (97 rows of 6000 keys, 4 kv heads 124 us, eight waves 135).
+//   decode  up to 16 packed rows per sequence: the streaming kernel.  Workgroups of eight waves where a CU is there for each sequence and kv head, of four,
+//           two side by side, where there are more of those (97 rows of 6000 keys, 4 kv heads 121 us, with eight waves 126, two 124; 100 ragged up to 4000
+//           in 8 bits 52, 58, 69).
 //   chunk   more.  f32: 64 packed rows a workgroup, three side by side.  bf16: 128, two side by side; at head_dim 128 256 rows, which fetch the keys once for
 //           twice as many, unless most sequences bring far less than the longest (2048 new tokens over 16384, 32 / 8 heads: 500 us against 543; a prompt
 //           of 8192 549 against 578; 8 ragged prompts up to 2000 208 against 218; 6 chunks up to 512 among 24 single tokens 186 against 167).
 //   split   keys per workgroup.  Single tokens: as many splits as leave each its CU, two also where they are a little too many (1 sequence of 40000, 8 kv
-//           heads: 33 us, in two rounds of two waves 42; 3 of 131072: 129 against 138; 20 ragged up to 8000: 66 against 76), none for few keys; where
+//           heads: 33 us, in two rounds of them 42; 3 of 131072: 129 against 138; 20 ragged up to 8000: 66 against 76), none for few keys; where
 //           workgroups are many, two rounds of them.  bf16 chunks of an even batch: the number that leaves the last round fullest, against 3 % of a full
 //           round for each (1024 new tokens over 32768, 40 / 8 heads, 160 workgroups: 680 us, unsplit 880).  The others: two rounds, since a ragged
 //           batch's longest sequence else runs on alone (24 sequences, 5 of them chunks of up to 701: 76 us, unsplit 131); in bf16 with a last split
@@ -1215,7 +1216,8 @@ Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
     const int64_t up = ceil_div64(2 * slots, wgs), least = f32 ? 256 : 512;
     int64_t tenths = 10 * up;                                   // of as many splits
     if (pl.decode) {
-      if (wgs <= cus) tenths = 10 * (b.max_ctx <= 2 * least ? 1 : 2 * wgs > cus && 3 * wgs <= 2 * cus ? 2 : cus / wgs);
+      if (b.max_ctx <= 2 * least) tenths = 10;
+      else if (wgs <= cus) tenths = 2 * wgs > cus && 3 * wgs <= 2 * cus ? 20 : 10 * (cus / wgs);
     } else if (!f32 && !even) {
       tenths -= up > 1 ? 2 : 0;
     } else if (!f32) {
@@ -1230,7 +1232,7 @@ Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
   }
   pl.splits = ceil_div(b.max_ctx, pl.split);
   if (pl.splits <= 1) pl.split = 0, pl.splits = 1;
-  if (pl.decode) pl.nw = a.split_keys || wgs > cus ? 2 : 8;      // (a pinned split: the waves' shares too)
+  if (pl.decode) pl.nw = a.split_keys || wgs > cus ? 4 : 8;      // (a pinned split: the waves' shares too)
   return pl;
 }
 uint64_t workspace_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a, const Plan& pl) {
@@ -1250,9 +1252,9 @@ template <typename T, bool F8, int HD>
 int launch_t(const PagedAttnKArgs& k, const Plan& pl, hipStream_t st) {
   const dim3 line((unsigned)(pl.tiles * k.kv.n_kv_heads * pl.splits));
   if (pl.decode) {
-    constexpr int STAGE = DecodeShape<T, F8, HD>::STAGE, NS = 33 * 1024 / STAGE > 4 ? 4 : 33 * 1024 / STAGE, NS8 = 17 * 1024 / STAGE > 2 ? 2 : 17 * 1024 / STAGE;
-    if (pl.nw == 2) hipLaunchKernelGGL((paged_decode_kernel<T, F8, HD, 2, NS>), line, dim3(128), 0, st, k);
-    else hipLaunchKernelGGL((paged_decode_kernel<T, F8, HD, 8, NS8>), line, dim3(512), 0, st, k);
+    constexpr int FIT = 17 * 1024 / DecodeShape<T, F8, HD>::STAGE, NS = FIT > 2 ? 2 : FIT;      // a ring of at most 17 KB a wave, 8 waves a CU
+    if (pl.nw == 4) hipLaunchKernelGGL((paged_decode_kernel<T, F8, HD, 4, NS>), line, dim3(256), 0, st, k);
+    else hipLaunchKernelGGL((paged_decode_kernel<T, F8, HD, 8, NS>), line, dim3(512), 0, st, k);
   } else if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((paged_rows_f32_kernel<F8, HD>), line, dim3(256), 0, st, k);
   else {
     if constexpr (HD == 128) {
