@@ -3,8 +3,9 @@
 // qk_rope_kernel: a fused row is [q heads | k heads | v heads] x head_dim.  Per q and k head, in f32,
 //     x <- x * rsqrt(mean x^2 + eps) * gain,     (a, b) <- m (a cos t - b sin t, b cos t + a sin t),  t = pos * f_i,
 // one rounding at the end; then q to its buffer, k to its buffer or (CACHE) its page, v to its page, in 8 bits (F8) with one scale per head.
-//   * HBM bound: a row is read once and written once.  head_dim / 16 lanes own a head, a lane two 16-byte pieces of it (bf16): the two that turn with
-//     each other, so a rotation needs no exchange between lanes; the norm's and the scale's reductions are butterflies over those 4 or 8 lanes.
+//   * HBM bound: a row is read once and written once.  head_dim / 16 lanes own a head, a lane two (bf16) or four (f32) 16-byte pieces of it: neighbouring
+//     lanes' are neighbours (f32, 8192 rows of 32 + 8 heads x 128: 65 us with two of 32 bytes, 55 so), and those that turn with each other are one
+//     lane's, so a rotation needs no exchange between lanes; the norm's and the scale's reductions are butterflies over those 4 or 8 lanes.
 //   * The angle of a far position does not fit 32 bits (pos = 10^5, f = 1: spacing 0.008): it is formed in f64 as a number of quarter turns, whose
 //     fraction is exact to 2^-25 of a turn after the integer part is dropped.  A wave computes the row's <= 64 angles once, one per lane, and every head
 //     it handles reads them from LDS.
@@ -15,25 +16,27 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
 
-// 16 bytes that the kernel reads once (non-temporal: norm + rotation of 16384 rows of 32 + 8 heads x 128 58.5 us, 5.7 TB/s; 68.9 without the hint.  The
-// same hint on its stores costs 8 %.)
+// 16 bytes that the kernel reads once: non-temporal, which leaves the caches to what is written and read next (norm + rotation of 4096 rows of 32 + 8 heads x
+// 128 and a pass over its q: 28.3 us, without the hint 30.0, with one on the stores too 30.4; of 13500: 86, 95, 85.  Where the rows themselves still lie in
+// the Infinity Cache the hint costs: 28.5 against 25.7).  16384 rows alone 57 us, 5.9 TB/s.
 __device__ __forceinline__ Chunk16 load_once(const void* p) {
   Chunk16 c;
   c.v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
   return c;
 }
-template <typename T> __device__ __forceinline__ void load8(const T* p, float* x);
-template <> __device__ __forceinline__ void load8<bf16_t>(const bf16_t* p, float* x) { chunk_to_f32<bf16_t>(load_once(p), x); }
-template <> __device__ __forceinline__ void load8<float>(const float* p, float* x) {
-  chunk_to_f32<float>(load_once(p), x);
-  chunk_to_f32<float>(load_once(p + 4), x + 4);
-}
-template <typename T> __device__ __forceinline__ void store8(T* p, const float* x);
-template <> __device__ __forceinline__ void store8<bf16_t>(bf16_t* p, const float* x) { *reinterpret_cast<Chunk16*>(p) = chunk_from_f32<bf16_t>(x); }
-template <> __device__ __forceinline__ void store8<float>(float* p, const float* x) {
-  *reinterpret_cast<Chunk16*>(p) = chunk_from_f32<float>(x);
-  *reinterpret_cast<Chunk16*>(p + 4) = chunk_from_f32<float>(x + 4);
-}
+// 16 values of a head as the 16-byte pieces at elements at[0], at[1], ...
+template <typename T> struct Pieces {
+  static constexpr int E = 16 / (int)sizeof(T), N = 16 / E;
+  int at[N];
+  __device__ __forceinline__ void load(const T* p, float* x) const {
+#pragma unroll
+    for (int k = 0; k < N; ++k) chunk_to_f32<T>(load_once(p + at[k]), x + k * E);
+  }
+  __device__ __forceinline__ void store(T* p, const float* x) const {
+#pragma unroll
+    for (int k = 0; k < N; ++k) *reinterpret_cast<Chunk16*>(p + at[k]) = chunk_from_f32<T>(x + k * E);
+  }
+};
 
 // cos and sin of pos * f
 __device__ __forceinline__ float2 turn_of(int pos, float f) {
@@ -99,13 +102,21 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(const QkRopeArgs p, c
       turns[wave][lane] = make_float2(t.x * p.rot_scale, t.y * p.rot_scale);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    const int i0 = c < rl ? 8 * c : 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) { const float2 t = turns[wave][i0 + i]; cs[i] = t.x; sn[i] = t.y; }
   }
-  // the lane's two pieces of a head: the halves' partners where they turn, neighbours elsewhere
-  const bool halves = c < rl && !p.interleaved;
-  const int e0 = 8 * (halves ? c : 2 * c), e1 = 8 * (halves ? c + rl : 2 * c + 1);
+  // The lane's pieces of a head: neighbouring lanes' are neighbours, and what turns with each other is one lane's.
+  using P = Pieces<T>;
+  P pc;
+#pragma unroll
+  for (int k = 0; k < P::N; ++k)
+    pc.at[k] = c >= rl ? 16 * rl + P::E * (c - rl + k * (LPH - rl)) : p.interleaved ? P::E * (c + k * rl) : P::E * (c + k % (P::N / 2) * rl) + (k < P::N / 2 ? 0 : 8 * rl);
+  if (c < rl) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 t = turns[wave][p.interleaved ? (pc.at[2 * i / P::E] + 2 * i % P::E) / 2 : pc.at[i / P::E] + i % P::E];
+      cs[i] = t.x;
+      sn[i] = t.y;
+    }
+  }
 
   const int heads = p.n_heads + p.n_kv_heads + (CACHE ? p.n_kv_heads : 0);
   for (int h0 = part * HPW; h0 < heads; h0 += parts * HPW) {
@@ -115,8 +126,7 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(const QkRopeArgs p, c
     if (CACHE && !is_q && page < 0) continue;
     const T* src = reinterpret_cast<const T*>(p.qkv) + (int64_t)row * p.ld + (int64_t)h * HD;
     float x[16];
-    load8<T>(src + e0, x);
-    load8<T>(src + e1, x + 8);
+    pc.load(src, x);
     if (!is_v) {
       if (p.q_gain) {
         float ss = 0.f;
@@ -128,7 +138,7 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(const QkRopeArgs p, c
         const float* gain = is_q ? p.q_gain : p.k_gain;
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
-          const f32x4 g = *reinterpret_cast<const f32x4*>(gain + (i < 8 ? e0 + i : e1 + i - 8));
+          const f32x4 g = *reinterpret_cast<const f32x4*>(gain + pc.at[i / P::E] + i % P::E);
 #pragma unroll
           for (int j = 0; j < 4; ++j) x[i + j] = x[i + j] * r * g[j];
         }
@@ -154,8 +164,7 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(const QkRopeArgs p, c
     if (is_q || !CACHE) {
       T* dst = is_q ? reinterpret_cast<T*>(p.q_out) + (int64_t)row * p.ldq + (int64_t)h * HD
                     : reinterpret_cast<T*>(p.k_out) + (int64_t)row * p.ldk + (int64_t)(h - p.n_heads) * HD;
-      store8<T>(dst + e0, x);
-      store8<T>(dst + e1, x + 8);
+      pc.store(dst, x);
     } else if constexpr (CACHE) {
       const PagedKv& kv = pages.kv;
       const int kh = is_v ? h - p.n_heads - p.n_kv_heads : h - p.n_heads;
@@ -173,23 +182,23 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(const QkRopeArgs p, c
         const float inv = 1.f / scale;
         char* dst = reinterpret_cast<char*>(base) + (int64_t)page * kv.page_stride + tok * HD;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          unsigned w[2];
+        for (int k = 0; k < P::N; ++k) {
+          int w[P::E / 4];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float* y = x + 8 * half + 4 * j;
+          for (int j = 0; j < P::E / 4; ++j) {
+            const float* y = x + P::E * k + 4 * j;
             int pk = 0;
             pk = __builtin_amdgcn_cvt_pk_fp8_f32(quotient_odd(y[0], scale, inv), quotient_odd(y[1], scale, inv), pk, false);
             pk = __builtin_amdgcn_cvt_pk_fp8_f32(quotient_odd(y[2], scale, inv), quotient_odd(y[3], scale, inv), pk, true);
-            w[j] = (unsigned)pk;
+            w[j] = pk;
           }
-          *reinterpret_cast<uint2*>(dst + (half ? e1 : e0)) = make_uint2(w[0], w[1]);
+          if constexpr (P::E == 8) *reinterpret_cast<int2*>(dst + pc.at[k]) = make_int2(w[0], w[1]);
+          else *reinterpret_cast<int*>(dst + pc.at[k]) = w[0];
         }
         if (c == 0) (is_v ? kv.v_scale : kv.k_scale)[(int64_t)page * kv.scale_stride + tok] = scale;
       } else {
         T* dst = reinterpret_cast<T*>(base) + (int64_t)page * kv.page_stride + tok * HD;
-        store8<T>(dst + e0, x);
-        store8<T>(dst + e1, x + 8);
+        pc.store(dst, x);
       }
     }
   }
@@ -217,6 +226,10 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(const PagedKv kv, 
     if (page < 0 && lane == 0) paged_report(kv.status, kBadPage);
   }
   const int off = pos & (kv.page_size - 1), c = lane % LPH;
+  using P = Pieces<T>;
+  P pc;
+#pragma unroll
+  for (int k = 0; k < P::N; ++k) pc.at[k] = P::E * (c + k * LPH);
   for (int h0 = 0; h0 < 2 * kv.n_kv_heads; h0 += HPW) {
     const int h = h0 + lane / LPH;
     if (h >= 2 * kv.n_kv_heads) continue;
@@ -224,7 +237,7 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(const PagedKv kv, 
     const int kh = is_v ? h - kv.n_kv_heads : h;
     T* dst = is_v ? v_out : k_out;
     if (!dst) continue;
-    dst += (int64_t)row * (is_v ? ldv : ldk) + (int64_t)kh * HD + 16 * c;
+    dst += (int64_t)row * (is_v ? ldv : ldk) + (int64_t)kh * HD;
     float x[16];
     if (page < 0) {
 #pragma unroll
@@ -233,20 +246,20 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(const PagedKv kv, 
       const int64_t tok = (int64_t)kh * kv.page_size + off;
       const void* base = is_v ? kv.V : kv.K;
       if constexpr (F8) {
-        const u32x4 w = load_once(reinterpret_cast<const char*>(base) + (int64_t)page * kv.page_stride + tok * HD + 16 * c).v;
+        const char* src = reinterpret_cast<const char*>(base) + (int64_t)page * kv.page_stride + tok * HD;
         const float scale = (is_v ? kv.v_scale : kv.k_scale)[(int64_t)page * kv.scale_stride + tok];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e4m3_to_f32(w[i], x + 4 * i);
+        for (int k = 0; k < P::N; ++k)
+          if constexpr (P::E == 8) {
+            const auto w = __builtin_nontemporal_load(reinterpret_cast<const unsigned __attribute__((ext_vector_type(2)))*>(src + pc.at[k]));
+            e4m3_to_f32(w[0], x + 8 * k);
+            e4m3_to_f32(w[1], x + 8 * k + 4);
+          } else e4m3_to_f32(__builtin_nontemporal_load(reinterpret_cast<const unsigned*>(src + pc.at[k])), x + 4 * k);
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] *= scale;
-      } else {
-        const T* src = reinterpret_cast<const T*>(base) + (int64_t)page * kv.page_stride + tok * HD + 16 * c;
-        load8<T>(src, x);
-        load8<T>(src + 8, x + 8);
-      }
+      } else pc.load(reinterpret_cast<const T*>(base) + (int64_t)page * kv.page_stride + tok * HD, x);
     }
-    store8<T>(dst, x);
-    store8<T>(dst + 8, x + 8);
+    pc.store(dst, x);
   }
 }
 
