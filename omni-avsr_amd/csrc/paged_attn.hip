@@ -1193,11 +1193,13 @@ int cu_count() {
 //           of 8192 549 against 578; 8 ragged prompts up to 2000 208 against 218; 6 chunks up to 512 among 24 single tokens 186 against 167).
 //   split   keys per workgroup.  Single tokens: as many splits as leave each its CU, two also where they are a little too many (1 sequence of 40000, 8 kv
 //           heads: 33 us, in two rounds of them 42; 3 of 131072: 129 against 138; 20 ragged up to 8000: 66 against 76), none for few keys; where
-//           workgroups are many, two rounds of them.  bf16 chunks of an even batch: the number that leaves the last round fullest, against 3 % of a full
-//           round for each (1024 new tokens over 32768, 40 / 8 heads, 160 workgroups: 680 us, unsplit 880).  The others: two rounds, since a ragged
-//           batch's longest sequence else runs on alone (24 sequences, 5 of them chunks of up to 701: 76 us, unsplit 131); in bf16 with a last split
-//           that is short, so that only the longest sequences have one and the short work comes last (2.6 % over 15 ragged batches, 0 .. 13 %; the
-//           256 keys' grain already does that to f32's many short ones).
+//           workgroups are many, two rounds of them.  bf16 chunks of an even batch: what costs least by the estimate below -- rounds, or for prompts, whose
+//           rows see more and more keys and start with the most, the mean share -- with 150 keys' time for the join's launch and 200 for each split's
+//           partial results (1024 new tokens over 32768, 40 / 8 heads, 160 workgroups: 8 splits 703 us, unsplit 873; 2048 over 6144 of 3 sequences, 28 / 4
+//           heads: unsplit 484, 3 splits 561; 2 prompts of 6000: unsplit 539, 5 splits 743).  The others: two rounds, since a ragged batch's longest
+//           sequence else runs on alone (24 sequences, 5 of them chunks of up to 701: 76 us, unsplit 131); in bf16 with a last split that is short, so that
+//           only the longest sequences have one and the short work comes last (2.6 % over 15 ragged batches, 0 .. 13 %; the 256 keys' grain already does
+//           that to f32's many short ones).
 struct Plan { int64_t tiles; int split, splits, nw; bool decode; };
 Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
   Plan pl;
@@ -1221,10 +1223,13 @@ Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
     } else if (!f32 && !even) {
       tenths -= up > 1 ? 2 : 0;
     } else if (!f32) {
-      const double each = 0.03 * (double)std::min(wgs, slots) / slots;
+      // in keys: whole rounds, or the mean share and half a workgroup more, whichever is less, and never less than one workgroup; partial results
+      const double full = (double)wgs / slots, share = full * (b.max_ctx - 0.5 * std::min(b.max_q, b.max_ctx));
       double best = 1e30;
       for (int i = 1; i <= 64; ++i) {
-        const double cost = (double)ceil_div64(wgs * i, slots) / i + each * (i - 1);
+        const int64_t keys = ceil_div64(ceil_div64(b.max_ctx, i), 256) * 256;
+        const double half = 0.5 * (i == 1 ? std::max(0, b.max_ctx - b.max_q) : keys);
+        const double cost = std::max((double)keys, std::min((double)(ceil_div64(wgs * i, slots) * keys), share + half)) + (i > 1 ? 150 + 200 * i * full : 0);
         if (cost < best) best = cost, tenths = 10 * i;
       }
     }
