@@ -1199,7 +1199,8 @@ int cu_count() {
 //           heads: unsplit 484, 3 splits 561; 2 prompts of 6000: unsplit 539, 5 splits 743).  The others: two rounds, since a ragged batch's longest
 //           sequence else runs on alone (24 sequences, 5 of them chunks of up to 701: 76 us, unsplit 131); in bf16 with a last split that is short, so that
 //           only the longest sequences have one and the short work comes last (2.6 % over 15 ragged batches, 0 .. 13 %; the 256 keys' grain already does
-//           that to f32's many short ones).
+//           that to f32's many short ones).  Ragged prompts that fill the chip are not split, as even ones are not (3 of up to 2000, 28 / 4 heads: 104
+//           us, in two 134).
 struct Plan { int64_t tiles; int split, splits, nw; bool decode; };
 Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
   Plan pl;
@@ -1221,13 +1222,15 @@ Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
       if (b.max_ctx <= 2 * least) tenths = 10;
       else if (wgs <= cus) tenths = 2 * wgs > cus && 3 * wgs <= 2 * cus ? 20 : 10 * (cus / wgs);
     } else if (!f32 && !even) {
-      tenths -= up > 1 ? 2 : 0;
+      if (wgs >= slots && 2ll * b.max_ctx <= 5ll * b.max_q) tenths = 10;
+      tenths -= tenths > 10 ? 2 : 0;
     } else if (!f32) {
       // in keys: whole rounds, or the mean share and half a workgroup more, whichever is less, and never less than one workgroup; partial results
       const double full = (double)wgs / slots, share = full * (b.max_ctx - 0.5 * std::min(b.max_q, b.max_ctx));
       double best = 1e30;
       for (int i = 1; i <= 64; ++i) {
         const int64_t keys = ceil_div64(ceil_div64(b.max_ctx, i), 256) * 256;
+        if (i > 1 && keys < least) break;
         const double half = 0.5 * (i == 1 ? std::max(0, b.max_ctx - b.max_q) : keys);
         const double cost = std::max((double)keys, std::min((double)(ceil_div64(wgs * i, slots) * keys), share + half)) + (i > 1 ? 150 + 200 * i * full : 0);
         if (cost < best) best = cost, tenths = 10 * i;
