@@ -291,7 +291,8 @@ def read(kv, batch, rows=None, *, dtype=None, out=None):
         if dtype is None:
             dtype = torch.bfloat16 if kv.is_8bit else kv.k.dtype
         desc = kv._for(dtype)
-        k, v = (torch.empty((rows, heads, head_dim), dtype=dtype, device=kv.device) for _ in range(2))
+        k = torch.empty((rows, heads, head_dim), dtype=dtype, device=kv.device)
+        v = torch.empty_like(k)
         at_k, at_v = k.data_ptr(), v.data_ptr()
     else:
         given = [t for t in out if t is not None]
