@@ -4,7 +4,7 @@
 // packed row r = token * G + head, all against the same keys and values, which a workgroup fetches once for its rows.  Softmax in one pass over the keys:
 // running maximum m (nearly), sum l and O, rescaled when m is raised, in base 2 (scale * log2 e folded into the scores).
 //
-// S^T = K Q^T and O^T = V^T P^T on 16x16 matrix instructions: a lane then owns one query column, its softmax is lane-local but for two exchanges, and the
+// S^T = K Q^T and O^T = V^T P^T on 16x16 or 32x32 matrix instructions: a lane then owns one query column, its softmax is lane-local but for two exchanges, and the
 // accumulator registers of S^T are the B operand of the second product.
 //
 // Keys behind a sequence's context are never fetched.  A tile that some of the workgroup's rows see only in part (an edge tile) is masked; P = 0 there
@@ -208,9 +208,10 @@ __device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) { return bf16x8{a[0],
 //
 // A workgroup per (sequence, kv head, split of its keys) whose packed rows are the <= 16 columns of the matrix instructions.  HBM bound: 2 G flop per byte
 // of a bf16 cache.  Each wave streams its own tiles of KT keys (wave, wave + NW, ...) through a private ring of NS tiles in LDS, fetched by LDS-DMA and
-// awaited by counted vmcnt, so there is no barrier in the loop and (NS - 1) tiles are on their way while one is computed.  16 keys lie in one page, so
-// an instruction's page is uniform: scalar loads, one page base per 16 keys.  The waves' (m, l, O) meet in LDS in wave order.  The cache is read once and
-// the loads say so (non-temporal): 691 MB of 97 sequences 121 us, 5.7 TB/s with the join; without the hint 15 % more.
+// awaited by counted vmcnt, so there is no barrier in the loop.  The 8 waves of a CU share its LDS: two tiles each where they are small, one where they are
+// 16 KB (f32 or bf16 at head_dim 128), other waves' tiles being on their way while one is computed.  16 keys lie in one page, so an instruction's page is
+// uniform: scalar loads, one page base per 16 keys.  The waves' (m, l, O) meet in LDS in wave order.  The cache is read once and the loads say so
+// (non-temporal): 691 MB of 97 sequences 121 us, 5.7 TB/s with the join; without the hint 15 % more.
 constexpr int kOnce = 2;                              // nt of a load to LDS
 template <typename T, bool F8, int HD> struct DecodeShape {
   static constexpr int KT = sizeof(T) == 4 ? 16 : 32;                        // keys per wave tile
