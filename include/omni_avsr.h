@@ -391,7 +391,8 @@ int oavsr_op_paged_append(const oavsr_paged_kv* kv, const oavsr_paged_batch* b, 
 int oavsr_op_paged_read(const oavsr_paged_kv* kv, const oavsr_paged_batch* b, void* k_out, int64_t ldk, void* v_out, int64_t ldv, oavsr_stream stream);
 
 /* O[row][h] = softmax over the keys j <= p of the row's sequence of (scale q . k_j), times v_j;  kv head h / (n_heads / n_kv_heads).  Scores and softmax
- * statistics in f32; keys a row does not see do not count, whatever their bytes hold.  A row that sees no key (p < 0): zeros, lse = -infinity. */
+ * statistics in f32; keys a row does not see do not count, whatever their bytes hold.  A row that sees no key (p < 0): zeros, lse = -infinity.  A row of which
+ * every visible key scores -infinity: NaN, as its softmax is, lse = -infinity. */
 typedef struct oavsr_paged_attn_desc {
   int32_t n_heads;
   float scale;         /* > 0 */

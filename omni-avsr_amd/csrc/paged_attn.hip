@@ -103,6 +103,9 @@ __device__ __forceinline__ bf16x8 finite_part(bf16x8 x) {
 
 // Splits that hold keys of a row that sees `see` of them.  A row of one split (or none) is finished by that split's workgroup; the others leave partial results.
 __device__ __forceinline__ int splits_of(const PagedAttnKArgs& p, int see) { return p.split && see > p.split ? (see - 1) / p.split + 1 : 1; }
+// 1 / l of a finished row.  l = 0: no key is seen (zeros), or every seen one scores -infinity, of which the softmax is NaN.  (A split of such keys
+// beside others is a partial result like any: no weight.)
+__device__ __forceinline__ float inverse_sum(float l, bool sees_keys) { return l == 0.f ? (sees_keys ? NAN : 0.f) : 1.f / l; }
 
 // ---- pieces of the streaming kernels -----------------------------------------------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(2))) int i32x2;
@@ -518,10 +521,10 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[j] = fmaf(f, x[(d0 + j) * RS + pr], acc[j]);
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
     const int64_t prow = sq.q0 + ptok;
-    const int n = splits_of(p, min(first_pos + ptok + 1, kmax));
+    const int psee = min(first_pos + ptok + 1, kmax), n = splits_of(p, psee);
     if (split >= n) continue;
+    const float inv = inverse_sum(l, n == 1 && psee > 0);
     if (n > 1) {
       const int64_t at = ((int64_t)split * p.b.rows + prow) * p.n_heads + phead;
       if (d0 == 0) p.part_ml[at] = make_float2(m, l);
@@ -828,9 +831,9 @@ __global__ __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) void paged_chunk_kernel(
   if (r >= packed) return;
   float l = l_run;
   l += __shfl_xor(l, 32, 64);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
   const int n = splits_of(p, see);
   if (split >= n) return;
+  const float inv = inverse_sum(l, n == 1 && see > 0);
   if (n > 1) {
     const int64_t at_row = ((int64_t)split * p.b.rows + row) * p.n_heads + head;
     if (h == 0) p.part_ml[at_row] = make_float2(m_run, l);
@@ -1080,9 +1083,9 @@ __global__ __launch_bounds__(256, 3) void paged_rows_f32_kernel(const PagedAttnK
   float l = l_run;
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
   const int n = splits_of(p, see);
   if (split >= n) return;
+  const float inv = inverse_sum(l, n == 1 && see > 0);
   float* O = reinterpret_cast<float*>(p.O) + row * p.ldo + (int64_t)head * HD;
   if (n > 1) {
     const int64_t at_row = ((int64_t)split * p.b.rows + row) * p.n_heads + head;
@@ -1173,7 +1176,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnKA
     }
   }
   if (head >= p.n_heads) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = inverse_sum(l, true);
   if (p.lse && d0 == 0) p.lse[(int64_t)row * p.n_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
   T* O = reinterpret_cast<T*>(p.O) + (int64_t)row * p.ldo + (int64_t)head * HD + d0;
   if constexpr (sizeof(T) == 2) *reinterpret_cast<bf16x4*>(O) = bf16x4{(bf16_t)(acc[0] * inv), (bf16_t)(acc[1] * inv), (bf16_t)(acc[2] * inv), (bf16_t)(acc[3] * inv)};

@@ -646,3 +646,42 @@ def test_refusals():
     assert paged.append(kv, none, z(0, (H + 2 * KV) * d)).shape == (0, H, d)
     assert paged.read(kv, none, 0)[0].shape == (0, KV, d)
     assert paged.qk_norm_rope(z(0, (H + 2 * KV) * d), H, KV, i32(), z(32, dt=torch.float32))[1].shape == (0, KV, d)
+
+
+@pytest.mark.parametrize("dtype,fmt,H,KV,d", [("bf16", "same", 8, 2, 64), ("bf16", "same", 4, 1, 128), ("f32", "same", 4, 2, 64), ("bf16", "e4m3", 8, 2, 128), ("f32", "e4m3", 4, 2, 64)])
+@pytest.mark.parametrize("new,split", [(1, 0), (3, 256), (80, 0), (80, 256)])
+def test_attention_scores_of_minus_infinity(dtype, fmt, H, KV, d, new, split):
+    """Keys that score -infinity weigh nothing; a row of which every visible key does is NaN, as its softmax is, with lse -infinity; a row that sees none is zero."""
+    ctx, low, dt = new + 520, 500, tdt(dtype)
+    pool = Pool(KV, d, 16, dtype, fmt, [ctx, 1])
+    k, v = pool.fill([ctx, 1])
+    q = rnd(new + 3, H, d, seed=3, dtype=dt)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    b = pool.batch([new, 3], [ctx, 1], max_q=max(new, 3))
+
+    def bad_keys(s, n):                                              # the first n keys of sequence s: their products with any q are -infinity
+        p = torch.arange(n)
+        page, off = pool.table[s, p // 16].long().to(DEV), (p % 16).to(DEV)
+        if fmt == "e4m3":
+            key = torch.zeros(d, dtype=torch.uint8, device=DEV)
+            key[0] = 0xb8                                            # -1, of an infinite scale
+            pool.kv.k.view(torch.uint8)[page, :, off] = key
+            pool.kv.k_scale[page, :, off] = math.inf
+        else:
+            pool.kv.k[page, :, off, 0] = -math.inf
+
+    def run():
+        out, lse = torch.full((new + 3, H, d), 7.0, dtype=dt, device=DEV), torch.full((new + 3, H), 7.0, device=DEV)
+        paged.attention(pool.kv, b, q.to(DEV), out=out, lse=lse, split_keys=split)
+        return out, lse
+
+    bad_keys(0, low)
+    out, lse = run()
+    y, err, z = attended(q[:new], [k[0][low:]], [v[0][low:]], [new], [ctx - low], d ** -0.5, dtype == "bf16")
+    within(out[:new], y, err + U[dt] * (y.abs() + err), "beside keys that weigh nothing")
+    assert lse[:new].isfinite().all()
+    bad_keys(0, ctx)
+    bad_keys(1, 1)
+    out, lse = run()
+    assert out[:new].isnan().all() and out[-1].isnan().all() and (lse[:new] == -math.inf).all() and (lse[-3:] == -math.inf).all()
+    assert (out[new:new + 2] == 0).all()
