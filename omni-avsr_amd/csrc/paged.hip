@@ -51,9 +51,11 @@ __device__ __forceinline__ float2 turn_of(int pos, float f) {
 
 // x / scale as an f32 that rounds to e4m3 as the exact quotient does: cut off towards zero, the lowest bit set where anything was cut (round to odd).
 // Plain f32 division lands on the middle between two e4m3 values too often (bf16 inputs: 8-bit numerators) and then picks the even one on no ground.
+// x - y * scale has to be exact: its lowest bit is scale's times y's, 2^-56 of scale for the smallest y that does not become zero (2^-10), and f32 ends at
+// 2^-149.  So scale must not lie below 2^-93: the caller multiplies smaller ones, and their x, by a power of two.
 __device__ __forceinline__ float quotient_odd(float x, float scale, float inv) {
   const float y0 = x * inv, y = fmaf(fmaf(-y0, scale, x), inv, y0);
-  const float r = fmaf(-y, scale, x);                                            // x - y * scale, exact
+  const float r = fmaf(-y, scale, x);                                            // exact
   const bool unlike = (__builtin_bit_cast(int, r) ^ __builtin_bit_cast(int, y)) < 0;
   const int over = (r != 0.f && unlike) ? 1 : 0;                                 // |y| > |x / scale|
   const int bits = (__builtin_bit_cast(int, y) - over) | (r != 0.f ? 1 : 0);
@@ -179,7 +181,7 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(const QkRopeArgs p, c
 #pragma unroll
         for (int o = 1; o < LPH; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
         const float scale = m == INFINITY ? NAN : fmaxf(m / 448.f, 1.17549435e-38f);
-        const float inv = 1.f / scale;
+        const float up = scale < 0x1p-64f ? 0x1p64f : 1.f, qscale = scale * up, inv = 1.f / qscale;      // (exact, and the quotient's own)
         char* dst = reinterpret_cast<char*>(base) + (int64_t)page * kv.page_stride + tok * HD;
 #pragma unroll
         for (int k = 0; k < P::N; ++k) {
@@ -188,8 +190,8 @@ __global__ __launch_bounds__(kThreads) void qk_rope_kernel(const QkRopeArgs p, c
           for (int j = 0; j < P::E / 4; ++j) {
             const float* y = x + P::E * k + 4 * j;
             int pk = 0;
-            pk = __builtin_amdgcn_cvt_pk_fp8_f32(quotient_odd(y[0], scale, inv), quotient_odd(y[1], scale, inv), pk, false);
-            pk = __builtin_amdgcn_cvt_pk_fp8_f32(quotient_odd(y[2], scale, inv), quotient_odd(y[3], scale, inv), pk, true);
+            pk = __builtin_amdgcn_cvt_pk_fp8_f32(quotient_odd(y[0] * up, qscale, inv), quotient_odd(y[1] * up, qscale, inv), pk, false);
+            pk = __builtin_amdgcn_cvt_pk_fp8_f32(quotient_odd(y[2] * up, qscale, inv), quotient_odd(y[3] * up, qscale, inv), pk, true);
             w[j] = pk;
           }
           if constexpr (P::E == 8) *reinterpret_cast<int2*>(dst + pc.at[k]) = make_int2(w[0], w[1]);

@@ -685,3 +685,33 @@ def test_attention_scores_of_minus_infinity(dtype, fmt, H, KV, d, new, split):
     out, lse = run()
     assert out[:new].isnan().all() and out[-1].isnan().all() and (lse[:new] == -math.inf).all() and (lse[-3:] == -math.inf).all()
     assert (out[new:new + 2] == 0).all()
+
+
+def test_8bit_rows_next_to_ties_at_small_scales():
+    """The f32 (bf16) numbers next to the middle between two e4m3 values, times scales from 2^-126 to 2^-96: the residual of their quotients lies below the smallest f32."""
+    d = 64
+    g = torch.Generator().manual_seed(3)
+    steps = torch.arange(1, 128, dtype=torch.uint8)[:126].view(E4M3).double()               # the positive e4m3 values, 448 the last
+    middle = (steps[1:] + steps[:-1]) / 2
+    rows = []
+    for e in range(-126, -95):
+        for i in range(8):
+            scale = (2.0 ** e * (1 + torch.rand(1, generator=g, dtype=torch.float64))).float()
+            x = torch.zeros(d)
+            x[0] = scale * 448
+            scale = (x[0].double() / 448).float().clamp_min(2.0 ** -126).double()
+            t = (middle[torch.randint(0, len(middle), (d - 1,), generator=g)] * scale).float()
+            t = t.bfloat16().float() if i % 2 else torch.nextafter(t, t * (i / 2 - 1) * 2) if i in (0, 4) else t
+            sign = torch.randint(0, 2, (d - 1,), generator=g).float() * 2 - 1
+            x[1:] = t.clamp_max(float(x[0])) * sign
+            rows.append(x)
+    v = torch.stack(rows)
+    n = len(v)
+    pool = Pool(1, d, 16, "f32", "e4m3", [n])
+    b = pool.batch([n], [n])
+    paged.append(pool.kv, b, torch.cat([torch.zeros(n, 2 * d), v], 1).to(DEV))
+    _, got = paged.read(pool.kv, b, n, dtype=torch.float32)
+    want = v.double()
+    scale = (want.abs().amax(-1, keepdim=True) / 448).float().clamp_min(2.0 ** -126).double()
+    off = got.cpu()[:, 0] != e4m3(want, scale).float()
+    assert not off.any(), f"{int(off.sum())} of {off.numel()}, in rows {off.any(1).nonzero()[:, 0].tolist()[:8]}"
