@@ -7,14 +7,16 @@ A decoder layer with its cache in pages runs, per step,
 
 with one `PagedKV` per layer (its pool of pages) and one `PagedBatch` per step (row offsets, lengths and page table of the sequences, shared by all layers).
 Everything is queued on the current stream of the tensors' device; nothing is synchronised, and every call can be captured into a graph.  An argument that
-does not fit raises ValueError before anything is queued, and so does one that asks for gradients: these are forward passes.  Lengths and page numbers are
-device data: a bad one never reaches memory outside the given tensors, and sets its bit in `PagedKV.status` (`PagedKV.check()` raises)."""
+does not fit raises ValueError before anything is queued, and so does one that asks for gradients (an input, an output or a pool that requires grad or
+carries a tangent of forward mode): these are forward passes.  Lengths and page numbers are device data: a bad one never reaches memory outside the given
+tensors, and sets its bit in `PagedKV.status` (`PagedKV.check()` raises)."""
 from __future__ import annotations
 
 import ctypes as C
 import functools
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import lib as L
 
@@ -27,8 +29,12 @@ def _need(ok, what):
         raise ValueError("paged: " + what)
 
 
-def _no_gradient(name):
-    _need(not torch.is_grad_enabled(), f"{name} asks for gradients, and none are formed here: call under torch.no_grad(), or detach it")
+def _no_gradient(t, name):
+    """Refuses a tensor whose gradient, or whose tangent in forward mode (which no_grad leaves on), a pass of torch's would form."""
+    if t.requires_grad:
+        _need(not torch.is_grad_enabled(), f"{name} asks for gradients, and none are formed here: call under torch.no_grad(), or detach it")
+    if _forward_ad._current_level >= 0:
+        _need(_forward_ad.unpack_dual(t).tangent is None, f"{name} carries a tangent, and no gradients are formed here: detach it")
 
 
 def _on_gpu(t, name, dtype, index=None):
@@ -89,6 +95,7 @@ class PagedKV:
         stride = k.stride(0) if n > 1 else heads * page * dim
         _need(n <= 1 or v.stride(0) == stride, f"k's pages are {k.stride(0)} apart, v's {v.stride(0)}")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._pools = tuple(t for t in (k, v, k_scale, v_scale) if t is not None)
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
         d = self.desc = L.PagedKvDesc()
         d.format = L.KV_E4M3 if self.is_8bit else L.KV_SAME
@@ -120,7 +127,11 @@ class PagedKV:
         return cls(*kv, *scales)
 
     def _for(self, dtype):
-        """The description for rows of `dtype`."""
+        """The description for rows of `dtype`, of pools that ask for no gradients."""
+        dual = _forward_ad._current_level >= 0
+        for t in self._pools:
+            if t.requires_grad or dual:
+                _no_gradient(t, "a pool of the cache")
         d = self.descs.get(dtype)
         if d is None:
             _need(dtype in _DT, f"rows of {dtype} are not supported")
@@ -193,8 +204,8 @@ def _vector(t, name, dtype, index, n=None):
     if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index and t.dim() == 1 and (n is None or t.numel() == n) and t.is_contiguous()):
         _on_gpu(t, name, dtype, index)
         _need(False, f"{name} is {tuple(t.shape)} (strides {t.stride()}), a vector{'' if n is None else f' of {n}'} in one piece is wanted")
-    if t.requires_grad:
-        _no_gradient(name)
+    if t.requires_grad or _forward_ad._current_level >= 0:
+        _no_gradient(t, name)
     return t.data_ptr()
 
 
@@ -218,8 +229,8 @@ def qk_norm_rope(qkv, n_heads, n_kv_heads, pos, inv_freq, *, q_gain=None, k_gain
     inv_freq [rot_dim / 2]: the first rot_dim dimensions of a head turn, halves against each other, or neighbours when interleaved."""
     if not (isinstance(qkv, torch.Tensor) and qkv.dim() == 2 and qkv.dtype in _DT and qkv.is_cuda):
         _need(False, "qkv has to be rows of float32 or bfloat16 on a GPU")
-    if qkv.requires_grad:
-        _no_gradient("qkv")
+    if qkv.requires_grad or _forward_ad._current_level >= 0:
+        _no_gradient(qkv, "qkv")
     rows, width = qkv.shape
     dtype, index, all_heads = qkv.dtype, qkv.get_device(), n_heads + 2 * n_kv_heads
     if _device() != index:
@@ -238,6 +249,8 @@ def qk_norm_rope(qkv, n_heads, n_kv_heads, pos, inv_freq, *, q_gain=None, k_gain
     else:
         q, k = out
         ldq, ldk = _rows_of(q, "out[0]", ldq, dtype, index, rows, True), _rows_of(k, "out[1]", ldk, dtype, index, rows, True)
+        _no_gradient(q, "out[0]")
+        _no_gradient(k, "out[1]")
     d = L.QkRopeDesc(_DT[dtype], rows, n_heads, n_kv_heads, head_dim, qkv.data_ptr(), ld, q.data_ptr(), ldq, k.data_ptr(), ldk, at_pos, at_freq, rot,
                      bool(interleaved), rot_scale, at_q, at_k, eps)
     _checked(_lib().oavsr_op_qk_norm_rope(C.byref(d), _stream(index)))
@@ -253,8 +266,8 @@ def append(kv, batch, qkv, inv_freq=None, *, pos=None, q_gain=None, k_gain=None,
     if _device() != index:
         with torch.cuda.device(index):
             return append(kv, batch, qkv, inv_freq, pos=pos, q_gain=q_gain, k_gain=k_gain, eps=eps, interleaved=interleaved, rot_scale=rot_scale, out=out)
-    if qkv.requires_grad:
-        _no_gradient("qkv")
+    if qkv.requires_grad or _forward_ad._current_level >= 0:
+        _no_gradient(qkv, "qkv")
     rows, width = qkv.shape
     dtype = qkv.dtype
     desc = kv._for(dtype)
@@ -271,6 +284,7 @@ def append(kv, batch, qkv, inv_freq=None, *, pos=None, q_gain=None, k_gain=None,
         out = qkv.new_empty((rows, n_heads, head_dim))
     else:
         ldq = _rows_of(out, "out", ldq, dtype, index, rows, True)
+        _no_gradient(out, "out")
     d = L.QkRopeDesc(_DT[dtype], rows, n_heads, heads, head_dim, qkv.data_ptr(), ld, out.data_ptr(), ldq, None, 0, at_pos, at_freq, rot, bool(interleaved), rot_scale,
                      at_q, at_k, eps)
     _checked(_lib().oavsr_op_paged_append(C.byref(desc), C.byref(b), C.byref(d), _stream(index)))
@@ -305,8 +319,10 @@ def read(kv, batch, rows=None, *, dtype=None, out=None):
         at_k = at_v = None
         if k is not None:
             ldk, at_k = _rows_of(k, "out[0]", width, dtype, index, rows, True), k.data_ptr()
+            _no_gradient(k, "out[0]")
         if v is not None:
             ldv, at_v = _rows_of(v, "out[1]", width, dtype, index, rows, True), v.data_ptr()
+            _no_gradient(v, "out[1]")
     b = batch._for(rows, kv)
     _checked(_lib().oavsr_op_paged_read(C.byref(desc), C.byref(b), at_k, ldk, at_v, ldv, _stream(index)))
     return k, v
@@ -322,8 +338,8 @@ def attention(kv, batch, q, scale=None, *, out=None, lse=None, split_keys=0):
     if _device() != index:
         with torch.cuda.device(index):
             return attention(kv, batch, q, scale, out=out, lse=lse, split_keys=split_keys)
-    if q.requires_grad:
-        _no_gradient("q")
+    if q.requires_grad or _forward_ad._current_level >= 0:
+        _no_gradient(q, "q")
     dtype, shape = q.dtype, q.shape
     desc, rows = kv._for(dtype), shape[0]
     width = shape[1] * shape[2] if len(shape) == 3 else shape[1]
@@ -339,11 +355,13 @@ def attention(kv, batch, q, scale=None, *, out=None, lse=None, split_keys=0):
         out = torch.empty_like(q) if ldq == width else q.new_empty(shape)
     else:
         ldo = _rows_of(out, "out", width, dtype, index, rows, True)
+        _no_gradient(out, "out")
     at_lse = None
     if lse is not None:
         _on_gpu(lse, "lse", torch.float32, index)
         if not (lse.shape == (rows, n_heads) and lse.is_contiguous()):
             _need(False, f"lse is {tuple(lse.shape)}, ({rows}, {n_heads}) in one piece is wanted")
+        _no_gradient(lse, "lse")
         at_lse = lse.data_ptr()
     work = torch.empty(need, dtype=torch.uint8, device=kv.device) if need else None      # of this call alone; the allocator reuses it in stream order
     d = L.PagedAttnDesc(n_heads, scale, q.data_ptr(), ldq, out.data_ptr(), ldo, at_lse, split_keys, None if work is None else work.data_ptr(), need)

@@ -11,6 +11,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 pytestmark = pytest.mark.gpu
 
@@ -715,3 +716,47 @@ def test_8bit_rows_next_to_ties_at_small_scales():
     scale = (want.abs().amax(-1, keepdim=True) / 448).float().clamp_min(2.0 ** -126).double()
     off = got.cpu()[:, 0] != e4m3(want, scale).float()
     assert not off.any(), f"{int(off.sum())} of {off.numel()}, in rows {off.any(1).nonzero()[:, 0].tolist()[:8]}"
+
+
+def test_what_asks_for_gradients_is_refused_wherever_it_stands():
+    """Pools, scales, outputs and lse that require grad, and tangents of forward mode (which no_grad does not switch off): refused, nothing queued."""
+    H, KV, d = 4, 2, 64
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt, device=DEV)  # noqa: E731
+    b = paged.PagedBatch(i32(0, 2), i32(20), i32(1, 2)[None], max_q=2, max_ctx=32)
+    q, qkv, freq, gain = z(2, H, d), z(2, (H + 2 * KV) * d), z(32, dt=torch.float32), z(d, dt=torch.float32)
+    pool = lambda: (z(6, KV, 16, d), z(6, KV, 16, d))  # noqa: E731
+    pool8 = lambda: (z(6, KV, 16, d).to(E4M3), z(6, KV, 16, d).to(E4M3), z(6, KV, 16, dt=torch.float32), z(6, KV, 16, dt=torch.float32))  # noqa: E731
+    kv = paged.PagedKV(*pool())
+    uses = lambda c: (lambda: paged.attention(c, b, q), lambda: paged.append(c, b, qkv), lambda: paged.read(c, b, 2))  # noqa: E731
+    calls = []
+    for make, which in ((pool, 0), (pool, 1), (pool8, 2), (pool8, 3)):
+        t = make()
+        c = paged.PagedKV(*t)
+        t[which].requires_grad_()                                     # after the cache was made, too
+        calls += uses(c)
+    g = lambda t: t.requires_grad_()  # noqa: E731
+    calls += [lambda: paged.attention(kv, b, q, out=g(z(2, H, d))), lambda: paged.attention(kv, b, q, lse=g(z(2, H, dt=torch.float32))),
+              lambda: paged.append(kv, b, qkv, out=g(z(2, H, d))), lambda: paged.read(kv, b, out=(g(z(2, KV, d)), None)), lambda: paged.read(kv, b, out=(None, g(z(2, KV, d)))),
+              lambda: paged.qk_norm_rope(qkv, H, KV, i32(0, 1), freq, out=(g(z(2, H, d)), z(2, KV, d))),
+              lambda: paged.qk_norm_rope(qkv, H, KV, i32(0, 1), freq, out=(z(2, H, d), g(z(2, KV, d))))]
+    for call in calls:
+        with pytest.raises(ValueError, match="gradients"):
+            call()
+        with torch.no_grad():
+            call()
+    kv.check()
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        duals = [lambda: paged.attention(kv, b, dual(q)), lambda: paged.append(kv, b, dual(qkv)), lambda: paged.append(kv, b, qkv, dual(freq)),
+                 lambda: paged.append(kv, b, qkv, q_gain=dual(gain), k_gain=gain), lambda: paged.qk_norm_rope(dual(qkv), H, KV, i32(0, 1), freq),
+                 lambda: paged.attention(kv, b, q, out=dual(z(2, H, d))), lambda: paged.attention(kv, b, q, lse=dual(z(2, H, dt=torch.float32)))]
+        for c in (paged.PagedKV(dual(pool()[0]), pool()[1]), paged.PagedKV(pool()[0], dual(pool()[1])), paged.PagedKV(*pool8()[:2], dual(pool8()[2]), pool8()[3])):
+            duals += uses(c)
+        for call in duals:
+            with pytest.raises(ValueError, match="gradients"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="gradients"):
+                call()
+        for call in uses(kv):                                         # plain tensors inside a level are plain
+            call()
