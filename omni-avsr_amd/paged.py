@@ -74,6 +74,7 @@ _stream = torch._C._cuda_getCurrentRawStream      # of a device's index
 
 
 _device = torch._C._cuda_getDevice               # the current one's index
+_written = torch._C._increment_version           # tensors of the caller's that a call writes: a backward pass that has saved one is refused, as after torch's own writes
 
 
 class PagedKV:
@@ -254,6 +255,8 @@ def qk_norm_rope(qkv, n_heads, n_kv_heads, pos, inv_freq, *, q_gain=None, k_gain
     d = L.QkRopeDesc(_DT[dtype], rows, n_heads, n_kv_heads, head_dim, qkv.data_ptr(), ld, q.data_ptr(), ldq, k.data_ptr(), ldk, at_pos, at_freq, rot,
                      bool(interleaved), rot_scale, at_q, at_k, eps)
     _checked(_lib().oavsr_op_qk_norm_rope(C.byref(d), _stream(index)))
+    if out is not None:
+        _written((q, k))
     return q, k
 
 
@@ -280,14 +283,17 @@ def append(kv, batch, qkv, inv_freq=None, *, pos=None, q_gain=None, k_gain=None,
     at_q, at_k = _gains(q_gain, k_gain, index, head_dim)
     b = batch._for(rows, kv)
     ldq = n_heads * head_dim
+    written = kv._pools
     if out is None:
         out = qkv.new_empty((rows, n_heads, head_dim))
     else:
         ldq = _rows_of(out, "out", ldq, dtype, index, rows, True)
         _no_gradient(out, "out")
+        written += (out,)
     d = L.QkRopeDesc(_DT[dtype], rows, n_heads, heads, head_dim, qkv.data_ptr(), ld, out.data_ptr(), ldq, None, 0, at_pos, at_freq, rot, bool(interleaved), rot_scale,
                      at_q, at_k, eps)
     _checked(_lib().oavsr_op_paged_append(C.byref(desc), C.byref(b), C.byref(d), _stream(index)))
+    _written(written)
     return out
 
 
@@ -325,6 +331,8 @@ def read(kv, batch, rows=None, *, dtype=None, out=None):
             _no_gradient(v, "out[1]")
     b = batch._for(rows, kv)
     _checked(_lib().oavsr_op_paged_read(C.byref(desc), C.byref(b), at_k, ldk, at_v, ldv, _stream(index)))
+    if out is not None:
+        _written(given)
     return k, v
 
 
@@ -351,6 +359,7 @@ def attention(kv, batch, q, scale=None, *, out=None, lse=None, split_keys=0):
     b = batch._for(rows, kv)
     need = batch._workspace(b, kv, dtype, n_heads, split_keys)
     ldo = width
+    given = None if out is None and lse is None else [t for t in (out, lse) if t is not None]
     if out is None:
         out = torch.empty_like(q) if ldq == width else q.new_empty(shape)
     else:
@@ -366,4 +375,6 @@ def attention(kv, batch, q, scale=None, *, out=None, lse=None, split_keys=0):
     work = torch.empty(need, dtype=torch.uint8, device=kv.device) if need else None      # of this call alone; the allocator reuses it in stream order
     d = L.PagedAttnDesc(n_heads, scale, q.data_ptr(), ldq, out.data_ptr(), ldo, at_lse, split_keys, None if work is None else work.data_ptr(), need)
     _checked(_lib().oavsr_op_paged_attention(C.byref(desc), C.byref(b), C.byref(d), _stream(index)))
+    if given:
+        _written(given)
     return out

@@ -760,3 +760,29 @@ def test_what_asks_for_gradients_is_refused_wherever_it_stands():
                 call()
         for call in uses(kv):                                         # plain tensors inside a level are plain
             call()
+
+
+def test_what_is_written_is_known_to_autograd():
+    """A tensor that a backward pass has saved and a call then writes: the backward pass is refused, as after any write in place."""
+    H, KV, d = 4, 2, 64
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt, device=DEV)  # noqa: E731
+    b = paged.PagedBatch(i32(0, 2), i32(20), i32(1, 2)[None], max_q=2, max_ctx=32)
+    q, qkv, freq = z(2, H, d), z(2, (H + 2 * KV) * d), z(32, dt=torch.float32)
+    kv, kv8 = paged.PagedKV.empty(6, 16, KV, d), paged.PagedKV.empty(6, 16, KV, d, dtype=E4M3)
+    out, lse, keys, vals = z(2, H, d), z(2, H, dt=torch.float32), z(2, KV, d), z(2, KV, d)
+    fused = z(2, (H + 2 * KV) * d)
+    for call, written in ((lambda: paged.attention(kv, b, q, out=out, lse=lse), (out, lse)), (lambda: paged.append(kv, b, qkv), (kv.k, kv.v)),
+                          (lambda: paged.append(kv8, b, qkv, out=out), (out, kv8.k, kv8.v, kv8.k_scale, kv8.v_scale)), (lambda: paged.read(kv, b, out=(keys, vals)), (keys, vals)),
+                          (lambda: paged.read(kv, b, out=(keys, None)), (keys,)), (lambda: paged.qk_norm_rope(qkv, H, KV, i32(0, 1), freq, out=(out, keys)), (out, keys)),
+                          (lambda: paged.append(kv, b, fused, out=fused[:, :H * d]), (fused,))):
+        before = [t._version for t in written]
+        call()
+        assert all(t._version > n for t, n in zip(written, before))
+    w = torch.ones(2, H, d, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    loss = (w * out).sum()
+    paged.attention(kv, b, q, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():                                      # such tensors have no version
+        paged.append(kv, b, z(2, (H + 2 * KV) * d), out=z(2, H, d))
