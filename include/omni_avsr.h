@@ -342,8 +342,8 @@ typedef struct oavsr_paged_kv {
   int64_t page_stride;                              /* elements from one page to the next (>= n_kv_heads * page_size * head_dim, whole 16 bytes) */
   float *k_scale, *v_scale;                         /* E4M3: [n_pages][n_kv_heads][page_size], 16-byte aligned; else NULL */
   int64_t scale_stride;                             /* floats from one page's scales to the next (>= n_kv_heads * page_size, a multiple of 4) */
-  /* Optional device word.  The lengths and page numbers of a batch live on the device and are checked there: whatever they hold, nothing outside the
-     given buffers is touched.  A launch that meets a bad one ORs its bit into *status and goes on. */
+  /* Optional device word, zero at first.  The lengths and page numbers of a batch live on the device and are checked there: whatever they hold, nothing
+     outside the given buffers is touched.  A launch that meets a bad one ORs its bit into *status and goes on. */
   int32_t* status;
 } oavsr_paged_kv;
 #define OAVSR_PAGED_BAD_PAGE 1 /* a page number outside [0, n_pages) inside a context: its tokens are not written, and read and attend as zeros */
@@ -363,6 +363,9 @@ typedef struct oavsr_paged_batch {
 /* For a program that builds its tables on the host: the bits (OAVSR_PAGED_BAD_*) that a launch over this batch would set, 0 for a sound one.  cu_q, ctx_len
  * and table are HOST arrays here; no device is touched, and kv's pointers are not followed.  < 0: refused. */
 int oavsr_paged_check_host(const oavsr_paged_kv* kv, const oavsr_paged_batch* b);
+
+/* *taken (device) = *kv->status, *kv->status = 0, in one step: a bit that a launch running at the same time sets is in this word or stays for the next. */
+int oavsr_paged_take_status(const oavsr_paged_kv* kv, int32_t* taken, oavsr_stream stream);
 
 /* One pass over fused rows [n_heads q | n_kv_heads k | n_kv_heads v] x head_dim.  Per q and k head, in f32:  x = x * rsqrt(mean(x^2) + eps) * gain
  * (q_gain / k_gain; NULL: no norm);  then, with inv_freq, the pairs of the first rot_dim dimensions turn by pos * inv_freq[i]:

@@ -194,6 +194,7 @@ int launch_paged_read(const PagedKv& kv, const PagedBatch& b, void* k_out, int64
 int launch_paged_attention(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a, hipStream_t st);
 int64_t paged_attention_workspace(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a);      // < 0: refused
 int check_paged(const PagedKv& kv, const PagedBatch& b, const char* who);                              // what every paged launch asks of its cache and batch
+int launch_paged_take_status(const PagedKv& kv, int* taken, hipStream_t st);
 int check_paged_host(const PagedKv& kv, const PagedBatch& b);                                          // b's arrays on the host: the bits a launch would report
 
 // ---- normalisation / elementwise ----------------------------------------------------------------

@@ -2255,6 +2255,10 @@ int oavsr_paged_check_host(const oavsr_paged_kv* kv, const oavsr_paged_batch* b)
   OAVSR_REQUIRE(kv && b, "paged_check_host: null desc");
   return check_paged_host(paged_kv_of(kv), paged_batch_of(b));
 }
+int oavsr_paged_take_status(const oavsr_paged_kv* kv, int32_t* taken, oavsr_stream stream) {
+  OAVSR_REQUIRE(kv, "paged_take_status: null desc");
+  return launch_paged_take_status(paged_kv_of(kv), taken, (hipStream_t)stream);
+}
 int oavsr_op_paged_append(const oavsr_paged_kv* kv, const oavsr_paged_batch* b, const oavsr_qk_rope_desc* d, oavsr_stream stream) {
   OAVSR_REQUIRE(kv && b && d, "op_paged_append: null desc");
   return launch_paged_append(paged_kv_of(kv), paged_batch_of(b), qk_rope_of(d), (hipStream_t)stream);

@@ -265,6 +265,8 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(const PagedKv kv, 
   }
 }
 
+__global__ void take_status_kernel(int* status, int* taken) { *taken = atomicExch(status, 0); }
+
 int check_rope(const QkRopeArgs& a, const char* who) {
   OAVSR_REQUIRE(a.dtype == DT_F32 || a.dtype == DT_BF16, "%s: unknown dtype %d", who, a.dtype);
   OAVSR_REQUIRE(a.rows >= 0 && a.n_heads > 0 && a.n_kv_heads > 0, "%s: bad sizes (rows %d, heads %d / %d)", who, a.rows, a.n_heads, a.n_kv_heads);
@@ -340,6 +342,13 @@ int check_paged_host(const PagedKv& kv, const PagedBatch& b) {
       if (paged_page(kv, b, s, pos, page_shift_of(kv)) < 0) bits |= kBadPage;
   }
   return bits;
+}
+
+int launch_paged_take_status(const PagedKv& kv, int* taken, hipStream_t st) {
+  OAVSR_REQUIRE(kv.status && taken, "paged_take_status: null status");
+  hipLaunchKernelGGL(take_status_kernel, dim3(1), dim3(1), 0, st, kv.status, taken);
+  OAVSR_CHECK_HIP(hipGetLastError());
+  return 0;
 }
 
 int launch_qk_norm_rope(const QkRopeArgs& a, hipStream_t st) {

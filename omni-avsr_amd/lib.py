@@ -169,6 +169,7 @@ SYMBOLS = {
     "oavsr_op_attention": (C.c_int, [C.POINTER(AttnDesc), _P]),
     "oavsr_op_decode_attention": (C.c_int, [C.POINTER(DecodeAttnDesc), _P]),
     "oavsr_paged_check_host": (C.c_int, [C.POINTER(PagedKvDesc), C.POINTER(PagedBatchDesc)]),
+    "oavsr_paged_take_status": (C.c_int, [C.POINTER(PagedKvDesc), _P, _P]),
     "oavsr_op_qk_norm_rope": (C.c_int, [C.POINTER(QkRopeDesc), _P]),
     "oavsr_op_paged_append": (C.c_int, [C.POINTER(PagedKvDesc), C.POINTER(PagedBatchDesc), C.POINTER(QkRopeDesc), _P]),
     "oavsr_op_paged_read": (C.c_int, [C.POINTER(PagedKvDesc), C.POINTER(PagedBatchDesc), _P, _L, _P, _L, _P]),

@@ -140,10 +140,14 @@ class PagedKV:
         return d
 
     def check(self):
-        """Raises RuntimeError if a call has met a bad page number or length since the last check (waits for the device; clears the word)."""
-        bits = int(self.status.item())
+        """Raises RuntimeError if a call has met a bad page number or length since the last check.  Waits for the device, so that calls queued before, on any
+        stream, are covered, and takes the bits off the word in one step: what others set meanwhile is the next check's.  Not while a graph is captured."""
+        with torch.cuda.device(self.index):
+            torch.cuda.synchronize()
+            taken = torch.empty_like(self.status)
+            _checked(_lib().oavsr_paged_take_status(C.byref(self.desc), taken.data_ptr(), _stream(self.index)))
+            bits = int(taken.item())
         if bits:
-            self.status.zero_()
             what = [s for b, s in ((L.PAGED_BAD_PAGE, "a page number outside the pool"), (L.PAGED_BAD_LENGTH, "a length outside the batch's bounds")) if bits & b]
             raise RuntimeError("paged: " + " and ".join(what) + " was met")
 

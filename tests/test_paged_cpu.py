@@ -151,3 +151,10 @@ def test_tensors_of_the_host_are_refused():
                  lambda: paged.qk_norm_rope(torch.zeros(2, 512), 4, 2, i, torch.zeros(32))):
         with pytest.raises(ValueError, match="GPU"):
             call()
+
+
+def test_status_is_taken_from_one_word_into_another():
+    lib = L.load()
+    refused(lib.oavsr_paged_take_status(None, A, None), "null desc")
+    refused(lib.oavsr_paged_take_status(C.byref(kv_desc()), A, None), "null status")
+    refused(lib.oavsr_paged_take_status(C.byref(kv_desc(status=A)), None, None), "null status")

@@ -786,3 +786,22 @@ def test_what_is_written_is_known_to_autograd():
         loss.backward()
     with torch.inference_mode():                                      # such tensors have no version
         paged.append(kv, b, z(2, (H + 2 * KV) * d), out=z(2, H, d))
+
+
+def _one_token(page):
+    """One token in `page`."""
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    return paged.PagedBatch(i32([0, 1]), i32([1]), i32([[page]]), max_q=1, max_ctx=1)
+
+
+def test_check_sees_calls_on_every_stream():
+    """A call that waits on another stream is waited for; each report is given once."""
+    kv = paged.PagedKV.empty(6, 16, 2, 64)
+    bad, side = _one_token(6), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)
+        paged.read(kv, bad, 1)
+    with pytest.raises(RuntimeError, match="page number"):
+        kv.check()
+    kv.check()
