@@ -80,7 +80,7 @@ _written = torch._C._increment_version           # tensors of the caller's that 
 class PagedKV:
     """A layer's pool of pages: k and v [n_pages][n_kv_heads][page_size][head_dim] in float32, bfloat16, or float8_e4m3fn with k_scale and v_scale
     [n_pages][n_kv_heads][page_size] (float32).  Pages may be further apart than they are large (a view of a larger pool), k's and v's by the same stride.
-    Keeps the tensors; `status` is one int32 of device memory."""
+    Keeps the tensors; `status` is one int32 of device memory, cleared when the constructor returns (which waits for the current stream for that)."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         _need(isinstance(k, torch.Tensor) and k.is_cuda, "k has to be a tensor on a GPU")
@@ -98,6 +98,8 @@ class PagedKV:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self._pools = tuple(t for t in (k, v, k_scale, v_scale) if t is not None)
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        if not torch.cuda.is_current_stream_capturing():      # the word is clear for calls on any stream from here on
+            torch.cuda.current_stream(self.index).synchronize()
         d = self.desc = L.PagedKvDesc()
         d.format = L.KV_E4M3 if self.is_8bit else L.KV_SAME
         d.dtype = L.DT_BF16 if self.is_8bit else _DT[k.dtype]

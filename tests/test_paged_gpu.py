@@ -805,3 +805,17 @@ def test_check_sees_calls_on_every_stream():
     with pytest.raises(RuntimeError, match="page number"):
         kv.check()
     kv.check()
+
+
+def test_a_cache_made_behind_queued_work_reports_on_another_stream():
+    """The status word is clear when the constructor returns, whatever is still queued on the current stream."""
+    k, v = (torch.zeros(6, 2, 16, 64, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    bad, side = _one_token(6), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)
+    kv = paged.PagedKV(k, v)
+    with torch.cuda.stream(side):
+        paged.read(kv, bad, 1)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="page number"):
+        kv.check()
