@@ -77,10 +77,21 @@ _device = torch._C._cuda_getDevice               # the current one's index
 _written = torch._C._increment_version           # tensors of the caller's that a call writes: a backward pass that has saved one is refused, as after torch's own writes
 
 
-class PagedKV:
+class _Keeps:
+    """An object whose tensors' addresses were taken when it was made: others in their place would not be seen, so they are not accepted."""
+
+    def __setattr__(self, name, value):
+        if name in self._kept and self.__dict__.get(name, value) is not value:
+            _need(False, f"{name} is kept as it was given: write into it, or make another {type(self).__name__}")
+        self.__dict__[name] = value
+
+
+class PagedKV(_Keeps):
     """A layer's pool of pages: k and v [n_pages][n_kv_heads][page_size][head_dim] in float32, bfloat16, or float8_e4m3fn with k_scale and v_scale
     [n_pages][n_kv_heads][page_size] (float32).  Pages may be further apart than they are large (a view of a larger pool), k's and v's by the same stride.
     Keeps the tensors; `status` is one int32 of device memory, cleared when the constructor returns (which waits for the current stream for that)."""
+
+    _kept = ("k", "v", "k_scale", "v_scale", "status")
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         _need(isinstance(k, torch.Tensor) and k.is_cuda, "k has to be a tensor on a GPU")
@@ -154,10 +165,12 @@ class PagedKV:
             raise RuntimeError("paged: " + " and ".join(what) + " was met")
 
 
-class PagedBatch:
+class PagedBatch(_Keeps):
     """The sequences of a step: cu_q [n_seqs + 1] (row offsets of their new tokens), ctx_len [n_seqs] (tokens in the cache, the new ones among them), table
     [n_seqs][pages], all int32 on the device.  max_q and max_ctx bound a sequence's new tokens and context.  Keeps the tensors: refilled in place, the
     same batch serves the next step."""
+
+    _kept = ("cu_q", "ctx_len", "table")
 
     def __init__(self, cu_q, ctx_len, table, *, max_q, max_ctx):
         self.index = _on_gpu(cu_q, "cu_q", torch.int32)

@@ -819,3 +819,19 @@ def test_a_cache_made_behind_queued_work_reports_on_another_stream():
     torch.cuda.synchronize()
     with pytest.raises(RuntimeError, match="page number"):
         kv.check()
+
+
+def test_tensors_that_a_cache_or_a_batch_keeps_are_not_exchanged():
+    """Their addresses were taken: another tensor in their place would not be seen.  Writing into them is how they change."""
+    kv = paged.PagedKV.empty(6, 16, 2, 64, dtype=E4M3)
+    b = _one_token(1)
+    for owner, names in ((kv, ("k", "v", "k_scale", "v_scale", "status")), (b, ("cu_q", "ctx_len", "table"))):
+        for name in names:
+            old = getattr(owner, name)
+            with pytest.raises(ValueError, match=name):
+                setattr(owner, name, old.clone())
+            assert getattr(owner, name) is old
+    b.ctx_len += 0                                                    # the same tensor again
+    b.table[:] = 2
+    paged.read(kv, b, 1)
+    kv.check()
