@@ -360,8 +360,9 @@ typedef struct oavsr_paged_batch {
   int64_t ld_table;
 } oavsr_paged_batch;
 
-/* For a program that builds its tables on the host: the bits (OAVSR_PAGED_BAD_*) that a launch over this batch would set, 0 for a sound one.  cu_q, ctx_len
- * and table are HOST arrays here; no device is touched, and kv's pointers are not followed.  < 0: refused. */
+/* For a program that builds its tables on the host: the bits (OAVSR_PAGED_BAD_*) that append, read and attention over this batch would set between them,
+ * 0 for a sound one (append and read look up the new tokens' pages only, attention all of a context's; nothing those of a sequence that brings no rows).  cu_q,
+ * ctx_len and table are HOST arrays here; no device is touched, and kv's pointers are not followed.  < 0: refused. */
 int oavsr_paged_check_host(const oavsr_paged_kv* kv, const oavsr_paged_batch* b);
 
 /* *taken (device) = *kv->status, *kv->status = 0, in one step: a bit that a launch running at the same time sets is in this word or stays for the next. */

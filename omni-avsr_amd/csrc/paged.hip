@@ -337,7 +337,7 @@ int check_paged_host(const PagedKv& kv, const PagedBatch& b) {
   for (int s = 0; s < b.n_seqs; ++s) {
     const SeqInfo q = paged_seq(b, s);
     if (q.bad) bits |= kBadLength;
-    const int n = q.ctx < b.max_ctx ? q.ctx : b.max_ctx;
+    const int n = q.nq == 0 ? 0 : q.ctx < b.max_ctx ? q.ctx : b.max_ctx;      // no launch reads the pages of a sequence that brings no rows, or is skipped
     for (int pos = 0; pos < n; pos += kv.page_size)
       if (paged_page(kv, b, s, pos, page_shift_of(kv)) < 0) bits |= kBadPage;
   }

@@ -158,3 +158,14 @@ def test_status_is_taken_from_one_word_into_another():
     refused(lib.oavsr_paged_take_status(None, A, None), "null desc")
     refused(lib.oavsr_paged_take_status(C.byref(kv_desc()), A, None), "null status")
     refused(lib.oavsr_paged_take_status(C.byref(kv_desc(status=A)), None, None), "null status")
+
+
+@pytest.mark.parametrize("cu,ctx,table,bits", [
+    ([0, 0, 4], [33, 33], [[-1, -1, -1], [3, 4, 5]], 0),             # an idle slot: its old length, its pages given back
+    ([0, 4, 4], [33, 40], [[3, 4, 5], [1, 99, 99]], 0),
+    ([0, 0, 4], [41, 33], [[-1, -1, -1], [3, 4, 5]], LENGTH),        # its length is looked at
+    ([0, 5, 5], [33, 0], [[-1, -1, -1], [3, 4, 5]], LENGTH),         # skipped for its five new tokens
+    ([0, 6, 5], [33, 0], [[-1, -1, -1], [3, 4, 5]], LENGTH),
+    ([0, 1, 1], [33, 33], [[3, -1, 5], [3, 4, 5]], PAGE)])
+def test_pages_of_sequences_that_bring_no_rows_are_not_looked_at(cu, ctx, table, bits):
+    test_lengths_and_page_numbers(cu, ctx, table, bits)
