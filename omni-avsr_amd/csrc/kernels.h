@@ -195,6 +195,8 @@ int launch_paged_attention(const PagedKv& kv, const PagedBatch& b, const PagedAt
 int64_t paged_attention_workspace(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a);      // < 0: refused
 int check_paged(const PagedKv& kv, const PagedBatch& b, const char* who);                              // what every paged launch asks of its cache and batch
 int launch_paged_take_status(const PagedKv& kv, int* taken, hipStream_t st);
+// A batch without rows has nothing to do but the check of its lengths, where somebody asks for it.
+inline bool nothing_to_do(const PagedKv& kv, const PagedBatch& b) { return b.n_seqs == 0 || (b.rows == 0 && !kv.status); }
 int check_paged_host(const PagedKv& kv, const PagedBatch& b);                                          // b's arrays on the host: the bits a launch would report
 
 // ---- normalisation / elementwise ----------------------------------------------------------------

@@ -366,7 +366,7 @@ int launch_paged_append(const PagedKv& kv, const PagedBatch& b, const QkRopeArgs
   OAVSR_REQUIRE(a.rows == b.rows && a.dtype == kv.dtype && a.n_kv_heads == kv.n_kv_heads && a.head_dim == kv.head_dim,
                 "paged_append: rows (%d, dtype %d, %d kv heads of %d) are not the batch's and the cache's (%d, dtype %d, %d of %d)", a.rows, a.dtype, a.n_kv_heads,
                 a.head_dim, b.rows, kv.dtype, kv.n_kv_heads, kv.head_dim);
-  if (a.rows == 0 || b.n_seqs == 0) return 0;
+  if (nothing_to_do(kv, b)) return 0;
   if (kv.format == KV_E4M3) return a.dtype == DT_F32 ? launch_rope_t<float, true, true>(a, kv, b, st) : launch_rope_t<bf16_t, true, true>(a, kv, b, st);
   return a.dtype == DT_F32 ? launch_rope_t<float, true, false>(a, kv, b, st) : launch_rope_t<bf16_t, true, false>(a, kv, b, st);
 }
@@ -377,7 +377,7 @@ int launch_paged_read(const PagedKv& kv, const PagedBatch& b, void* k_out, int64
   const int64_t width = (int64_t)kv.n_kv_heads * kv.head_dim;
   OAVSR_REQUIRE((!k_out || (ldk >= width && ldk % vec == 0)) && (!v_out || (ldv >= width && ldv % vec == 0)), "paged_read: row strides %lld / %lld", (long long)ldk, (long long)ldv);
   OAVSR_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, "paged_read: pointers must be 16-byte aligned");
-  if (b.rows == 0 || b.n_seqs == 0 || (!k_out && !v_out)) return 0;
+  if (nothing_to_do(kv, b) || (b.rows && !k_out && !v_out)) return 0;      // (empty outputs have no address)
   if (kv.format == KV_E4M3) return kv.dtype == DT_F32 ? launch_read_t<float, true>(kv, b, k_out, ldk, v_out, ldv, st) : launch_read_t<bf16_t, true>(kv, b, k_out, ldk, v_out, ldv, st);
   return kv.dtype == DT_F32 ? launch_read_t<float, false>(kv, b, k_out, ldk, v_out, ldv, st) : launch_read_t<bf16_t, false>(kv, b, k_out, ldk, v_out, ldv, st);
 }

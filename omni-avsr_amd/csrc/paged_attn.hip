@@ -1275,7 +1275,7 @@ int launch_t(const PagedAttnKArgs& k, const Plan& pl, hipStream_t st) {
     if (pl.nw == 4) hipLaunchKernelGGL((paged_chunk_kernel<F8, HD, 4>), line, dim3(256), 0, st, k);
   }
   OAVSR_CHECK_HIP(hipGetLastError());
-  if (pl.split) {
+  if (pl.split && k.b.rows) {
     constexpr int ALL = kThreads / (HD / 4);
     static_assert(ALL >= kFewSplits, "groups");
     if (pl.splits > kFewSplits) hipLaunchKernelGGL((paged_merge_kernel<T, HD, ALL>), dim3((unsigned)((int64_t)k.b.rows * k.n_heads)), dim3(kThreads), 0, st, k);
@@ -1299,7 +1299,7 @@ int launch_paged_attention(const PagedKv& kv, const PagedBatch& b, const PagedAt
   OAVSR_REQUIRE(a.ldq >= width && a.ldo >= width && a.ldq % vec == 0 && a.ldo % vec == 0, "paged_attention: row strides %lld / %lld", (long long)a.ldq, (long long)a.ldo);
   OAVSR_REQUIRE(b.rows == 0 || (a.Q && a.O), "paged_attention: null rows");
   OAVSR_REQUIRE((((uintptr_t)a.Q | (uintptr_t)a.O | (uintptr_t)a.workspace) & 15) == 0, "paged_attention: pointers must be 16-byte aligned");
-  if (b.rows == 0 || b.n_seqs == 0) return 0;
+  if (nothing_to_do(kv, b)) return 0;
   const Plan pl = plan_of(kv, b, a);
   const uint64_t need = workspace_of(kv, b, a, pl);
   OAVSR_REQUIRE(need == 0 || (a.workspace && a.workspace_bytes >= need), "paged_attention: a workspace of %llu bytes is needed, %llu given", (unsigned long long)need,

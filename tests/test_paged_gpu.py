@@ -835,3 +835,21 @@ def test_tensors_that_a_cache_or_a_batch_keeps_are_not_exchanged():
     b.table[:] = 2
     paged.read(kv, b, 1)
     kv.check()
+
+
+@pytest.mark.parametrize("cu,ctx,bad", [([0, 5, 5], [5, 0], True), ([0, 0, 0], [3, 65], True), ([0, -1, 0], [3, 3], True), ([0, 0, 0], [3, 64], False)])
+@pytest.mark.parametrize("max_q", [5, 90])
+def test_lengths_are_checked_where_there_are_no_rows(cu, ctx, bad, max_q):
+    """Calls of no rows over sequences whose lengths say otherwise."""
+    kv = paged.PagedKV.empty(6, 16, 2, 64)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    b = paged.PagedBatch(i32(cu), i32(ctx), i32([[0, 1, 2, 3]] * 2), max_q=max_q, max_ctx=64)
+    for call in (lambda: paged.append(kv, b, torch.zeros(0, 512, dtype=torch.bfloat16, device=DEV)), lambda: paged.read(kv, b, 0),
+                 lambda: paged.attention(kv, b, torch.zeros(0, 4, 64, dtype=torch.bfloat16, device=DEV)),
+                 lambda: paged.attention(kv, b, torch.zeros(0, 4, 64, dtype=torch.bfloat16, device=DEV), split_keys=256)):
+        kv.check()
+        call()
+        if bad:
+            with pytest.raises(RuntimeError, match="length"):
+                kv.check()
+    kv.check()
