@@ -6,6 +6,8 @@ namespace oavsr {
 
 constexpr int kBadPage = 1, kBadLength = 2;      // bits of *status (include/omni_avsr.h: OAVSR_PAGED_BAD_*)
 
+constexpr int64_t kMaxThreads = (1ll << 32) - 1;      // of a launch, in one dimension
+
 __device__ __forceinline__ void paged_report(int* status, int bit) {
   if (status) atomicOr(status, bit);             // (the same word whoever comes first)
 }

@@ -290,7 +290,7 @@ int launch_rope_t(const QkRopeArgs& a, const PagedKv& kv, const PagedBatch& b, h
   const int hpw = 64 / (a.head_dim / 16), heads = a.n_heads + (CACHE ? 2 : 1) * a.n_kv_heads;
   const int parts = a.rows >= kManyRows ? 1 : ceil_div(heads, hpw);
   const int64_t blocks = ceil_div64((int64_t)a.rows * parts, kWaves) + (CACHE ? 1 : 0);
-  OAVSR_REQUIRE(blocks < (1ll << 31), "paged: %d rows are too many for one launch", a.rows);
+  OAVSR_REQUIRE(blocks * kThreads <= kMaxThreads, "paged: %d rows are too many for one launch", a.rows);
   std::conditional_t<CACHE, Pages, NoPages> pages;
   if constexpr (CACHE) { pages.kv = kv; pages.b = b; }
   if (a.head_dim == 64) hipLaunchKernelGGL((qk_rope_kernel<T, 64, CACHE, F8>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a, pages, parts);
@@ -301,7 +301,9 @@ int launch_rope_t(const QkRopeArgs& a, const PagedKv& kv, const PagedBatch& b, h
 
 template <typename T, bool F8>
 int launch_read_t(const PagedKv& kv, const PagedBatch& b, void* k_out, int64_t ldk, void* v_out, int64_t ldv, hipStream_t st) {
-  const dim3 grid(ceil_div(b.rows, kWaves) + 1);
+  const int64_t blocks = ceil_div64(b.rows, kWaves) + 1;
+  OAVSR_REQUIRE(blocks * kThreads <= kMaxThreads, "paged_read: %d rows are too many for one launch", b.rows);
+  const dim3 grid((unsigned)blocks);
   if (kv.head_dim == 64) hipLaunchKernelGGL((paged_read_kernel<T, 64, F8>), grid, dim3(kThreads), 0, st, kv, b, (T*)k_out, ldk, (T*)v_out, ldv);
   else hipLaunchKernelGGL((paged_read_kernel<T, 128, F8>), grid, dim3(kThreads), 0, st, kv, b, (T*)k_out, ldk, (T*)v_out, ldv);
   OAVSR_CHECK_HIP(hipGetLastError());

@@ -1242,7 +1242,7 @@ Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
     }
     pl.split = (int)std::max<int64_t>(least, ceil_div64(ceil_div64(10ll * b.max_ctx, tenths), 256) * 256);
   }
-  pl.splits = ceil_div(b.max_ctx, pl.split);
+  pl.splits = (int)ceil_div64(b.max_ctx, pl.split);
   if (pl.splits <= 1) pl.split = 0, pl.splits = 1;
   if (pl.decode) pl.nw = a.split_keys || wgs > cus ? 4 : 8;      // (a pinned split: the waves' shares too)
   return pl;
@@ -1304,7 +1304,9 @@ int launch_paged_attention(const PagedKv& kv, const PagedBatch& b, const PagedAt
   const uint64_t need = workspace_of(kv, b, a, pl);
   OAVSR_REQUIRE(need == 0 || (a.workspace && a.workspace_bytes >= need), "paged_attention: a workspace of %llu bytes is needed, %llu given", (unsigned long long)need,
                 (unsigned long long)(a.workspace ? a.workspace_bytes : 0));
-  OAVSR_REQUIRE(pl.tiles * kv.n_kv_heads * pl.splits < (1ll << 31) && pl.splits <= 65535, "paged_attention: too many workgroups (%lld tiles, %d splits)", (long long)pl.tiles, pl.splits);
+  const int64_t joins = pl.split ? (int64_t)b.rows * (pl.splits > kFewSplits ? a.n_heads : ceil_div(a.n_heads, kThreads / (kv.head_dim / 4))) : 0;
+  OAVSR_REQUIRE(pl.splits <= 65535 && pl.tiles * kv.n_kv_heads * pl.splits <= kMaxThreads / (pl.nw * 64) && joins <= kMaxThreads / kThreads,
+                "paged_attention: too many workgroups (%lld tiles, %d splits, %d rows)", (long long)pl.tiles, pl.splits, b.rows);
   PagedAttnKArgs k;
   k.kv = kv; k.b = b; k.Q = a.Q; k.ldq = a.ldq; k.O = a.O; k.ldo = a.ldo; k.lse = a.lse; k.scale2 = a.scale * 1.44269504088896340736f;
   k.n_heads = a.n_heads; k.group = a.n_heads / kv.n_kv_heads; k.split = pl.split; k.tiles = (int)pl.tiles;

@@ -169,3 +169,16 @@ def test_status_is_taken_from_one_word_into_another():
     ([0, 1, 1], [33, 33], [[3, -1, 5], [3, 4, 5]], PAGE)])
 def test_pages_of_sequences_that_bring_no_rows_are_not_looked_at(cu, ctx, table, bits):
     test_lengths_and_page_numbers(cu, ctx, table, bits)
+
+
+@pytest.mark.parametrize("call", [
+    lambda lib: lib.oavsr_op_qk_norm_rope(C.byref(rope_desc(rows=1 << 26)), None),                                                   # a wave per row: 2^32 threads
+    lambda lib: lib.oavsr_op_paged_append(C.byref(kv_desc()), C.byref(batch_desc(rows=1 << 26)), C.byref(rope_desc(rows=1 << 26)), None),
+    lambda lib: lib.oavsr_op_paged_read(C.byref(kv_desc()), C.byref(batch_desc(rows=1 << 26)), A, 128, A, 128, None),
+    lambda lib: lib.oavsr_op_paged_read(C.byref(kv_desc()), C.byref(batch_desc(rows=2 ** 31 - 1)), A, 128, A, 128, None),
+    lambda lib: lib.oavsr_op_paged_attention(C.byref(kv_desc()), C.byref(batch_desc(n_seqs=1 << 23)), C.byref(attn_desc()), None),     # single tokens: 256 threads a sequence and kv head
+    lambda lib: lib.oavsr_op_paged_attention(C.byref(kv_desc()), C.byref(batch_desc(rows=1 << 22, max_q=1 << 22, max_ctx=5000, ld_table=400)),
+                                             C.byref(attn_desc(split_keys=256, workspace=A, workspace_bytes=1 << 60)), None)])          # the join: 256 threads a row and head
+def test_launches_of_more_threads_than_a_grid_holds_are_refused(call):
+    """2^32 threads and more in one launch: refused before anything is queued."""
+    refused(call(L.load()), "too many")
