@@ -208,6 +208,7 @@ class PagedBatch(_Keeps):
         key = (d.rows, kv.shape, dtype, n_heads, split_keys)
         need = self._work.get(key)
         if need is None:
+            _need(0 <= split_keys < 2 ** 31, f"split_keys {split_keys} (a multiple of 256)")
             a = L.PagedAttnDesc(n_heads, 1.0)
             a.split_keys = split_keys
             need = _lib().oavsr_paged_attention_workspace(C.byref(kv._for(dtype)), C.byref(d), C.byref(a))

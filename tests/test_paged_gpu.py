@@ -853,3 +853,10 @@ def test_lengths_are_checked_where_there_are_no_rows(cu, ctx, bad, max_q):
             with pytest.raises(RuntimeError, match="length"):
                 kv.check()
     kv.check()
+
+
+@pytest.mark.parametrize("split", [2 ** 32, 2 ** 32 + 256, -2 ** 32, 2 ** 31])
+def test_split_keys_that_do_not_fit_are_refused(split):
+    kv = paged.PagedKV.empty(6, 16, 2, 64)
+    with pytest.raises(ValueError, match="split_keys"):
+        paged.attention(kv, _one_token(1), torch.zeros(1, 4, 64, dtype=torch.bfloat16, device=DEV), split_keys=split)
