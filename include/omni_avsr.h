@@ -375,8 +375,8 @@ int oavsr_paged_take_status(const oavsr_paged_kv* kv, int32_t* taken, oavsr_stre
 typedef struct oavsr_qk_rope_desc {
   int32_t dtype, rows, n_heads, n_kv_heads, head_dim;
   const void* qkv; int64_t ld;
-  void* q_out; int64_t ldq; /* [rows][n_heads * head_dim]; may be the q part of qkv itself */
-  void* k_out; int64_t ldk; /* [rows][n_kv_heads * head_dim]; may be the k part of qkv itself; append: unused */
+  void* q_out; int64_t ldq; /* [rows][n_heads * head_dim]; may be the q part of qkv itself, and share no other memory with it */
+  void* k_out; int64_t ldk; /* [rows][n_kv_heads * head_dim]; may be the k part of qkv itself, and share no other memory with it; append: unused */
   const int32_t* pos;       /* [rows]; append: NULL = the token's place in its sequence */
   const float* inv_freq;    /* [rot_dim / 2], with any long-context scaling in it; NULL: no rotation */
   int32_t rot_dim;          /* multiple of 16, <= head_dim */
@@ -401,7 +401,7 @@ typedef struct oavsr_paged_attn_desc {
   int32_t n_heads;
   float scale;         /* > 0 */
   const void* Q; int64_t ldq; /* [rows][n_heads * head_dim], kv->dtype */
-  void* O; int64_t ldo;
+  void* O; int64_t ldo; /* may be Q itself, and share no other memory with it */
   float* lse;          /* optional [rows][n_heads]: natural logarithm of the sum of exponentials of a row's scores */
   /* Long contexts of few rows are split: workgroups take split_keys keys each and a second launch joins their partial results.  0: the launcher's rule,
      which follows the batch's bounds (so the last bits of a row may follow them); a multiple of 256: this split, the same bits for a row in any batch of

@@ -69,6 +69,14 @@ def _rows_of(t, name, width, dtype, index, rows=None, written=False):
     return stride[0]
 
 
+def _apart(a, lda, wa, b, ldb, wb, rows, names):
+    """Rows of a (lda apart, wa long, from that byte on) and of b share no memory: behind each other, or columns of the same rows.  All in bytes."""
+    if rows == 0 or a + (rows - 1) * lda + wa <= b or b + (rows - 1) * ldb + wb <= a:
+        return
+    off = (b - a) % lda
+    _need(lda == ldb and wa <= off and off + wb <= lda, f"{names} overlap")
+
+
 _lib = functools.lru_cache(None)(L.load)
 _stream = torch._C._cuda_getCurrentRawStream      # of a device's index
 
@@ -246,8 +254,8 @@ def _checked(rc):
 
 def qk_norm_rope(qkv, n_heads, n_kv_heads, pos, inv_freq, *, q_gain=None, k_gain=None, eps=1e-6, interleaved=False, rot_scale=1.0, out=None):
     """Norm (with q_gain, k_gain) and rotation (by pos * inv_freq; None: none) of the query and key heads of fused rows [rows][(n_heads + 2 n_kv_heads) *
-    head_dim].  Returns q [rows][n_heads][head_dim] and k [rows][n_kv_heads][head_dim]; `out` = (q, k) to write into, which may be qkv's own parts.
-    inv_freq [rot_dim / 2]: the first rot_dim dimensions of a head turn, halves against each other, or neighbours when interleaved."""
+    head_dim].  Returns q [rows][n_heads][head_dim] and k [rows][n_kv_heads][head_dim]; `out` = (q, k) to write into: qkv's own parts, or memory apart from
+    it.  inv_freq [rot_dim / 2]: the first rot_dim dimensions of a head turn, halves against each other, or neighbours when interleaved."""
     if not (isinstance(qkv, torch.Tensor) and qkv.dim() == 2 and qkv.dtype in _DT and qkv.is_cuda):
         _need(False, "qkv has to be rows of float32 or bfloat16 on a GPU")
     if qkv.requires_grad or _forward_ad._current_level >= 0:
@@ -272,6 +280,12 @@ def qk_norm_rope(qkv, n_heads, n_kv_heads, pos, inv_freq, *, q_gain=None, k_gain
         ldq, ldk = _rows_of(q, "out[0]", ldq, dtype, index, rows, True), _rows_of(k, "out[1]", ldk, dtype, index, rows, True)
         _no_gradient(q, "out[0]")
         _no_gradient(k, "out[1]")
+        e, at, to_q, to_k, q_wide, k_wide = qkv.element_size(), qkv.data_ptr(), q.data_ptr(), k.data_ptr(), n_heads * head_dim, n_kv_heads * head_dim
+        if to_q != at or (ldq != ld and rows > 1):                      # else: the rows' own queries
+            _apart(at, ld * e, width * e, to_q, ldq * e, q_wide * e, rows, "qkv and out[0]")
+        if to_k != at + q_wide * e or (ldk != ld and rows > 1):         # else: their own keys
+            _apart(at, ld * e, width * e, to_k, ldk * e, k_wide * e, rows, "qkv and out[1]")
+        _apart(to_q, ldq * e, q_wide * e, to_k, ldk * e, k_wide * e, rows, "out[0] and out[1]")
     d = L.QkRopeDesc(_DT[dtype], rows, n_heads, n_kv_heads, head_dim, qkv.data_ptr(), ld, q.data_ptr(), ldq, k.data_ptr(), ldk, at_pos, at_freq, rot,
                      bool(interleaved), rot_scale, at_q, at_k, eps)
     _checked(_lib().oavsr_op_qk_norm_rope(C.byref(d), _stream(index)))
@@ -281,8 +295,9 @@ def qk_norm_rope(qkv, n_heads, n_kv_heads, pos, inv_freq, *, q_gain=None, k_gain
 
 
 def append(kv, batch, qkv, inv_freq=None, *, pos=None, q_gain=None, k_gain=None, eps=1e-6, interleaved=False, rot_scale=1.0, out=None):
-    """qk_norm_rope of the batch's rows, the keys and values going into their sequences' pages.  Returns q [rows][n_heads][head_dim] (`out`: where to, which
-    may be qkv's own part).  pos [rows]: positions to turn by where they are not the tokens' places in their sequences.  Rows of no sequence are left."""
+    """qk_norm_rope of the batch's rows, the keys and values going into their sequences' pages.  Returns q [rows][n_heads][head_dim] (`out`: where to, qkv's own
+    part or memory apart from it).  pos [rows]: positions to turn by where they are not the tokens' places in their sequences.  Rows of no sequence, and those
+    before their sequence's first place (where ctx_len counts fewer tokens than are new), are left as they were: in a q made here, undefined."""
     if not (isinstance(qkv, torch.Tensor) and qkv.dim() == 2 and qkv.is_cuda):
         _need(False, "qkv has to be rows on a GPU")
     heads, head_dim, index = kv.heads, kv.head_dim, kv.index
@@ -309,6 +324,9 @@ def append(kv, batch, qkv, inv_freq=None, *, pos=None, q_gain=None, k_gain=None,
     else:
         ldq = _rows_of(out, "out", ldq, dtype, index, rows, True)
         _no_gradient(out, "out")
+        if out.data_ptr() != qkv.data_ptr() or (ldq != ld and rows > 1):      # else: the rows' own queries
+            e = qkv.element_size()
+            _apart(qkv.data_ptr(), ld * e, width * e, out.data_ptr(), ldq * e, n_heads * head_dim * e, rows, "qkv and out")
         written += (out,)
     d = L.QkRopeDesc(_DT[dtype], rows, n_heads, heads, head_dim, qkv.data_ptr(), ld, out.data_ptr(), ldq, None, 0, at_pos, at_freq, rot, bool(interleaved), rot_scale,
                      at_q, at_k, eps)
@@ -349,6 +367,9 @@ def read(kv, batch, rows=None, *, dtype=None, out=None):
         if v is not None:
             ldv, at_v = _rows_of(v, "out[1]", width, dtype, index, rows, True), v.data_ptr()
             _no_gradient(v, "out[1]")
+        if len(given) == 2:
+            e = k.element_size()
+            _apart(at_k, ldk * e, width * e, at_v, ldv * e, width * e, rows, "out[0] and out[1]")
     b = batch._for(rows, kv)
     _checked(_lib().oavsr_op_paged_read(C.byref(desc), C.byref(b), at_k, ldk, at_v, ldv, _stream(index)))
     if out is not None:
@@ -385,6 +406,9 @@ def attention(kv, batch, q, scale=None, *, out=None, lse=None, split_keys=0):
     else:
         ldo = _rows_of(out, "out", width, dtype, index, rows, True)
         _no_gradient(out, "out")
+        if out.data_ptr() != q.data_ptr() or (ldo != ldq and rows > 1):
+            e = q.element_size()
+            _apart(q.data_ptr(), ldq * e, width * e, out.data_ptr(), ldo * e, width * e, rows, "q and out")
     at_lse = None
     if lse is not None:
         _on_gpu(lse, "lse", torch.float32, index)

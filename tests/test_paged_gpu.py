@@ -860,3 +860,33 @@ def test_split_keys_that_do_not_fit_are_refused(split):
     kv = paged.PagedKV.empty(6, 16, 2, 64)
     with pytest.raises(ValueError, match="split_keys"):
         paged.attention(kv, _one_token(1), torch.zeros(1, 4, 64, dtype=torch.bfloat16, device=DEV), split_keys=split)
+
+
+def test_outputs_that_overlap_what_is_read_are_refused():
+    """An output may be the part it replaces; any other share of memory is refused, columns beside each other are not."""
+    H, KV, d = 4, 2, 64
+    kv = paged.PagedKV.empty(6, 16, KV, d)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    b = paged.PagedBatch(i32(0, 3), i32(20), i32(1, 2)[None], max_q=3, max_ctx=32)
+    wide = torch.zeros(4, (2 * H + 2 * KV) * d, dtype=torch.bfloat16, device=DEV)
+    qkv, q, k, rest = wide[:3, :(H + 2 * KV) * d], wide[:3, :H * d], wide[:3, H * d:(H + KV) * d], wide[:3, (H + 2 * KV) * d:]
+    flat = wide.view(-1)
+    pos = i32(0, 1, 2)
+    rope = lambda out: paged.qk_norm_rope(qkv, H, KV, pos, None, out=out)  # noqa: E731
+    apart = torch.zeros(3, H, d, dtype=torch.bfloat16, device=DEV)
+    bad = [lambda: rope((k.new_zeros(3, H * d), q[:, :KV * d])), lambda: rope((wide[1:, :H * d], k)), lambda: rope((flat[:3 * H * d].view(3, H, d), apart[:, :KV])),
+           lambda: rope((apart, apart[:, :KV])), lambda: rope((rest, wide[:3, (H + 2 * KV) * d + d:(2 * KV + H) * d + d + KV * d])),
+           lambda: paged.append(kv, b, qkv, out=wide[:3, d:H * d + d]), lambda: paged.append(kv, b, qkv, out=flat[:3 * H * d].view(3, H, d)),
+           lambda: paged.attention(kv, b, q, out=wide[1:, :H * d]), lambda: paged.attention(kv, b, q, out=wide[:3, d:H * d + d]),
+           lambda: paged.read(kv, b, out=(k, k)), lambda: paged.read(kv, b, out=(k, wide[:3, H * d + d:(H + KV) * d + d]))]
+    for call in bad:
+        with pytest.raises(ValueError, match="overlap|row of out"):
+            call()
+    rope((q, k))
+    rope((rest, k))
+    paged.append(kv, b, qkv, out=rest)
+    paged.append(kv, b, qkv, out=q)
+    paged.attention(kv, b, q, out=q)
+    paged.attention(kv, b, q, out=rest)
+    paged.read(kv, b, out=(k, wide[:3, (H + KV) * d:(H + 2 * KV) * d]))
+    paged.attention(kv, b, q, split_keys=256)
