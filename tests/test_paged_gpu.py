@@ -890,3 +890,41 @@ def test_outputs_that_overlap_what_is_read_are_refused():
     paged.attention(kv, b, q, out=rest)
     paged.read(kv, b, out=(k, wide[:3, (H + KV) * d:(H + 2 * KV) * d]))
     paged.attention(kv, b, q, split_keys=256)
+
+
+SMALL_F32 = [("f32", "e4m3", 4, 2, 64, 16, [1, 3, 0, 8], [300, 5, 9, 8]), ("f32", "e4m3", 8, 1, 128, 32, [1, 2], [700, 64]), ("f32", "e4m3", 14, 2, 64, 64, [1] * 3, [1, 64, 1500]),
+             ("f32", "e4m3", 16, 1, 128, 256, [1, 1], [257, 1]), ("f32", "e4m3", 2, 1, 64, 16, [1] * 300, [1 + 3 * i for i in range(300)]),
+             ("f32", "e4m3", 8, 2, 128, 16, [1, 2] * 80, [2 + 5 * i for i in range(160)])]
+
+
+@pytest.mark.parametrize("split", [0, 256])
+@pytest.mark.parametrize("case", SMALL_F32, ids=lambda c: f"{c[2]}-{c[3]}-{c[4]}-{len(c[6])}")
+def test_attention_of_few_f32_rows_over_8_bits(case, split):
+    """Up to 16 rows per kv head and sequence, exact f32 over e4m3 bytes: workgroups of eight waves, and of four (more sequences than CUs, or a pinned split)."""
+    test_attention(*case, split)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [3, 80])
+def test_attention_f32_over_8_bits_keys_a_row_does_not_see_do_not_count(d, new):
+    test_attention_keys_a_row_does_not_see_do_not_count("f32", "e4m3", 4, 2, d, new)
+
+
+@pytest.mark.parametrize("fmt,H,KV,d,ctx", [("same", 32, 8, 64, 313), ("same", 28, 4, 128, 700), ("e4m3", 32, 8, 128, 600), ("e4m3", 14, 2, 64, 500)])
+def test_attention_single_tokens_weigh_values_by_two_numbers(fmt, H, KV, d, ctx):
+    """bf16, up to 16 rows: a weight is the sum of two bf16 numbers, cut off at 2^-7 of it and rounded at 2^-8 of the rest, so 2^-15 stands where one number's 2^-8 would:
+    a bound that weights of one number break."""
+    n = 6
+    pool = Pool(KV, d, 16, "bf16", fmt, [ctx] * n)
+    k, v = pool.fill([ctx] * n)
+    q = rnd(n, H, d, seed=8, dtype=torch.bfloat16)
+    out = paged.attention(pool.kv, pool.batch([1] * n, [ctx] * n), q.to(DEV))
+    y, err, _ = attended(q, k, v, [1] * n, [ctx] * n, d ** -0.5, False)
+    G = H // KV
+    P = [torch.softmax(torch.einsum("hd,chd->hc", q[s].double(), k[s].repeat_interleave(G, 1)) * d ** -0.5, -1) for s in range(n)]
+    size = torch.stack([torch.einsum("hc,chd->hd", p, x.abs().repeat_interleave(G, 1)) for p, x in zip(P, v)])
+    tol = err + 2.0 ** -15 * size
+    tol = tol + U[torch.bfloat16] * (y.abs() + tol)
+    within(out, y, tol, "two numbers")
+    one = torch.stack([torch.einsum("hc,chd->hd", p.bfloat16().double(), x.repeat_interleave(G, 1)) for p, x in zip(P, v)]).bfloat16().double()
+    assert ((one - y).abs() > tol).any()
