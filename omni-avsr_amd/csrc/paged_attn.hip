@@ -554,7 +554,8 @@ template <bool F8, int HD, int NW>
 __global__ __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) void paged_chunk_kernel(const PagedAttnKArgs p) {
   constexpr int ROWS = NW * 32, RB = HD * 2, IMG = KT * RB, NSTAGE = 2, STAGE = 2 * IMG + (F8 ? 2 * KT * 4 : 0);
   constexpr int NDS = HD / 16, NDT = HD / 32;
-  constexpr int CB = F8 ? HD : RB, FB = CB / NW, RW = KT / NW, NC = FB < 16 ? 1 : FB / 16;      // bytes of a cached row, of them per thread; rows per wave; 16-byte loads
+  constexpr int CB = F8 ? HD : RB, FB = CB / NW, RW = KT / NW, NC = FB / 16;      // bytes of a cached row, of them per thread; rows per wave; 16-byte loads
+  static_assert(FB >= 16, "a thread loads whole 16-byte pieces");
   __shared__ __attribute__((aligned(1024))) char smem[NSTAGE * STAGE];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ql = lane & 31, h = lane >> 5;
@@ -599,18 +600,12 @@ __global__ __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) void paged_chunk_kernel(
   auto fetch = [&](int kt0, Raw& x) __attribute__((always_inline)) {
     const int key = kt0 + wave * RW + lane / NW;
     const bool ok = page >= 0 && key < kend;
-    const int64_t at = (int64_t)page * page_bytes + ((int64_t)kvh * p.kv.page_size + (key & pmask)) * CB + (lane % NW) * (FB < 16 ? FB : 16);
+    const int64_t at = (int64_t)page * page_bytes + ((int64_t)kvh * p.kv.page_size + (key & pmask)) * CB + (lane % NW) * 16;
     const char *k = ok ? Kb + at : zero, *v = ok ? Vb + at : zero;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      if constexpr (FB < 16) {
-        const uint2 a = *reinterpret_cast<const uint2*>(k), b = *reinterpret_cast<const uint2*>(v);
-        x.k[c] = u32x4{a.x, a.y, 0u, 0u};
-        x.v[c] = u32x4{b.x, b.y, 0u, 0u};
-      } else {
-        x.k[c] = *reinterpret_cast<const u32x4*>(k + c * NW * 16);
-        x.v[c] = *reinterpret_cast<const u32x4*>(v + c * NW * 16);
-      }
+      x.k[c] = *reinterpret_cast<const u32x4*>(k + c * NW * 16);
+      x.v[c] = *reinterpret_cast<const u32x4*>(v + c * NW * 16);
     }
     if constexpr (F8) {
       const int skey = kt0 + wave * RW + lane % RW;
@@ -628,10 +623,9 @@ __global__ __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) void paged_chunk_kernel(
       const int at = lane % NW + c * NW;
       if constexpr (F8) {
 #pragma unroll
-        for (int w = 0; w < (FB < 16 ? 1 : 2); ++w) {
-          const int to = FB < 16 ? at : 2 * at + w;
-          put(dst, to, __builtin_bit_cast(u32x4, join(e4m3_to_bf16(x.k[c][2 * w]), e4m3_to_bf16(x.k[c][2 * w + 1]))));
-          put(dst + IMG, to, __builtin_bit_cast(u32x4, join(e4m3_to_bf16(x.v[c][2 * w]), e4m3_to_bf16(x.v[c][2 * w + 1]))));
+        for (int w = 0; w < 2; ++w) {
+          put(dst, 2 * at + w, __builtin_bit_cast(u32x4, join(e4m3_to_bf16(x.k[c][2 * w]), e4m3_to_bf16(x.k[c][2 * w + 1]))));
+          put(dst + IMG, 2 * at + w, __builtin_bit_cast(u32x4, join(e4m3_to_bf16(x.v[c][2 * w]), e4m3_to_bf16(x.v[c][2 * w + 1]))));
         }
       } else {
         put(dst, at, x.k[c]);
