@@ -129,12 +129,13 @@ __device__ __forceinline__ float max_xor16_32(float x) {
 }
 
 // The running maximum need not be the maximum: any number near it keeps the exponentials in range and cancels in O / l.  It is raised, and O and l rescaled,
-// only when some row's scores pass it by kSlack, so that probabilities stay below 2^8 at the same relative precision.  (With the exact maximum some
-// row of a wave finds a new one in nearly every of the first dozens of tiles, and each time all of O is multiplied.)
+// only when some row's scores pass it, and then by kSlack more than they do, so that this is rare (with the exact maximum some row of a wave finds a new one in
+// nearly every of the first dozens of tiles, and each time all of O is multiplied).  Weights stay between 2^-8, at the largest score, and 1: none
+// takes a sum out of range that the values themselves do not.
 constexpr float kSlack = 8.f;
 __device__ __forceinline__ float raise_max(float& m_run, float mt) {
-  const bool up = mt > m_run + kSlack;                 // of this row alone: a row's bits do not follow the wave's other rows
-  const float m_new = up ? mt : m_run, alpha = up ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.f;
+  const bool up = mt > m_run;                          // of this row alone: a row's bits do not follow the wave's other rows
+  const float m_new = up ? mt + kSlack : m_run, alpha = up ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.f;
   m_run = m_new;
   return alpha;
 }
@@ -367,7 +368,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
       }
     }
     mt = max_xor16_32(mt);
-    if (__builtin_amdgcn_ballot_w64(mt > m_run + kSlack) != 0ull) {
+    if (__builtin_amdgcn_ballot_w64(mt > m_run) != 0ull) {
       const float alpha = raise_max(m_run, mt);
       l_run *= alpha;
 #pragma unroll
@@ -712,7 +713,7 @@ __global__ __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) void paged_chunk_kernel(
       for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[t2][e]);
     mt = max_xor32(mt);
     if constexpr (!F8) mt *= p.scale2;                 // scale > 0
-    if (__builtin_amdgcn_ballot_w64(mt > m_run + kSlack) != 0ull) {
+    if (__builtin_amdgcn_ballot_w64(mt > m_run) != 0ull) {
       const float alpha = raise_max(m_run, mt);
       l_run *= alpha;
 #pragma unroll
@@ -998,7 +999,7 @@ __global__ __launch_bounds__(256, 3) void paged_rows_f32_kernel(const PagedAttnK
       }
     }
     mt = max_xor16_32(mt);
-    if (__builtin_amdgcn_ballot_w64(mt > m_run + kSlack) != 0ull) {
+    if (__builtin_amdgcn_ballot_w64(mt > m_run) != 0ull) {
       const float alpha = raise_max(m_run, mt);
       l_run *= alpha;
 #pragma unroll

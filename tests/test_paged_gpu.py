@@ -928,3 +928,23 @@ def test_attention_single_tokens_weigh_values_by_two_numbers(fmt, H, KV, d, ctx)
     within(out, y, tol, "two numbers")
     one = torch.stack([torch.einsum("hc,chd->hd", p.bfloat16().double(), x.repeat_interleave(G, 1)) for p, x in zip(P, v)]).bfloat16().double()
     assert ((one - y).abs() > tol).any()
+
+
+@pytest.mark.parametrize("dtype,fmt", [("bf16", "same"), ("f32", "same"), ("bf16", "e4m3"), ("f32", "e4m3")])
+@pytest.mark.parametrize("new,split", [(1, 0), (1, 256), (40, 0), (40, 256)])
+def test_attention_of_large_values(dtype, fmt, new, split):
+    """Values of 2^126 whose largest weight comes late and is about 2^7 times the first tile's: a mean of equal numbers is that number, and no weight above 1 may
+    carry the sum out of range."""
+    ctx, d, dt = 300, 64, tdt(dtype)
+    pool = Pool(1, d, 16, dtype, fmt, [ctx])
+    rows = torch.zeros(ctx, 3 * d)
+    rows[:, d] = -200.0                                              # q . k / 8 of all keys but two
+    rows[0, d], rows[256, d] = 0.0, 4.84375
+    rows[:, 2 * d:] = 2.0 ** 126
+    paged.append(pool.kv, pool.batch([ctx], [ctx]), rows.to(dt).to(DEV))
+    _, v = paged.read(pool.kv, pool.batch([ctx], [ctx]), ctx, dtype=torch.float32 if fmt == "e4m3" else dt)
+    q = torch.zeros(new, 4, d, dtype=dt, device=DEV)
+    q[..., 0] = 8.0
+    out = paged.attention(pool.kv, pool.batch([new], [ctx]), q, split_keys=split)
+    want = v[:1].double().cpu().expand(new, 4, d)
+    within(out, want, (U[dt] + (U[torch.bfloat16] if dtype == "bf16" else 0) + 16 * U32) * want, "a mean of equal numbers")
