@@ -396,7 +396,9 @@ int oavsr_op_paged_read(const oavsr_paged_kv* kv, const oavsr_paged_batch* b, vo
 
 /* O[row][h] = softmax over the keys j <= p of the row's sequence of (scale q . k_j), times v_j;  kv head h / (n_heads / n_kv_heads).  Scores and softmax
  * statistics in f32; keys a row does not see do not count, whatever their bytes hold.  A row that sees no key (p < 0): zeros, lse = -infinity.  A row of which
- * every visible key scores -infinity: NaN, as its softmax is, lse = -infinity. */
+ * every visible key scores -infinity: NaN, as its softmax is, lse = -infinity.  With bf16 rows the weights of the values are sums of two bf16 numbers where
+ * max_q * n_heads / n_kv_heads <= 16, single ones (2^-8 of each weight, relative) where it is more.  Weights, 1 at most, are multiplied with values (8 bits:
+ * with their scales, before the bytes) and summed before the division by their sum: sums that pass 2^128, and scales below about 2^-100, lose their accuracy. */
 typedef struct oavsr_paged_attn_desc {
   int32_t n_heads;
   float scale;         /* > 0 */

@@ -210,8 +210,9 @@ __device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) { return bf16x8{a[0],
 
 // ---- few rows per sequence: single tokens ------------------------------------------------------------------------------------------------------
 //
-// A workgroup per (sequence, kv head, split of its keys) whose packed rows are the <= 16 columns of the matrix instructions.  HBM bound: 2 G flop per byte
-// of a bf16 cache.  Each wave streams its own tiles of KT keys (wave, wave + NW, ...) through a private ring of NS tiles in LDS, fetched by LDS-DMA and
+// A workgroup per (sequence, kv head, split of its keys) whose packed rows are the <= 16 columns of the matrix instructions.  HBM bound: G flop per byte of
+// a bf16 cache, 2 G of an 8-bit one.  (Not f32 rows over 8 bits: the instructions work on 16 columns whatever G, 32 flop per byte, which the f32 pipe does
+// at 4 TB/s, and the bytes are widened beside it: 97 sequences of up to 6000, 28 / 4 heads x 128: 167 us, 2.1 TB/s; f32 bytes, up to 3000: 130 us, 5.0.)  Each wave streams its own tiles of KT keys (wave, wave + NW, ...) through a private ring of NS tiles in LDS, fetched by LDS-DMA and
 // awaited by counted vmcnt, so there is no barrier in the loop.  The 8 waves of a CU share its LDS: two tiles each where they are small, one where they are
 // 16 KB (f32 or bf16 at head_dim 128), other waves' tiles being on their way while one is computed.  16 keys lie in one page, so an instruction's page is
 // uniform: scalar loads, one page base per 16 keys.  The waves' (m, l, O) meet in LDS in wave order.  The cache is read once and the loads say so
@@ -551,6 +552,9 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_decode_kernel(const PagedAtt
 // of 8192, 32 / 8 heads: 642 us in rising order, 576 so, 549 with 256 rows; one level of all sequences at a time: the same there, but 4 chunks over
 // 12000 keys 704 us against 447, since the L2 no longer sees a sequence's keys once).  2048 new tokens over 16384: 500 us, 1030 TFLOP/s.
 // A wave skips the tiles none of its rows sees, and masks only those that some row sees in part, in a loop of its own.
+// A weight is one bf16 number (in 8 bits behind its product with the value's scale): a rounding of 2^-8 of each weight, relative, that the kernel of
+// single tokens does not make, and the result's error against 64 bits is 0.0023 where its own rounding alone makes 0.0017.  Two numbers, as there, are half again
+// as many products and cost a third: 2048 over 16384 683 us against 514, in 8 bits 743 against 574, 4 prompts of 4096 at 32 / 8 heads x 64 463 against 357.
 template <bool F8, int HD, int NW>
 __global__ __launch_bounds__(NW * 64, HD == 64 ? 3 : 2) void paged_chunk_kernel(const PagedAttnKArgs p) {
   constexpr int ROWS = NW * 32, RB = HD * 2, IMG = KT * RB, NSTAGE = 2, STAGE = 2 * IMG + (F8 ? 2 * KT * 4 : 0);
@@ -1198,8 +1202,12 @@ int cu_count() {
 //           heads: unsplit 484, 3 splits 561; 2 prompts of 6000: unsplit 539, 5 splits 743).  The others: two rounds, since a ragged batch's longest
 //           sequence else runs on alone (24 sequences, 5 of them chunks of up to 701: 76 us, unsplit 131); in bf16 with a last split that is short, so that
 //           only the longest sequences have one and the short work comes last (2.6 % over 15 ragged batches, 0 .. 13 %; the 256 keys' grain already does
-//           that to f32's many short ones).  Ragged prompts that fill the chip are not split, as even ones are not (3 of up to 2000, 28 / 4 heads: 104
-//           us, in two 134).
+//           that to f32's many short ones).  Ragged prompts that fill the chip are not split, as even ones are not (3 of up to 2000, 28 / 4 heads: 117
+//           us, in two 141; 4 of up to 1000 56 against 65; 12 of up to 700, 16 / 16 heads x 64: 24 against 33; 8 of up to 1500, 14 / 2 heads x 64: 44
+//           against 45; 5 of up to 2000 in 8 bits 157 against 155).  Over far longer contexts they are, for the longest one's sake (4 chunks of up to
+//           1000 over 6000: 214 us, unsplit 240; over 3000, where the two rules meet, 118 and 115).
+//           At head_dim 64 three workgroups fit side by side, and two are counted: three would take a chunk of 1024 over 32768 at 14 / 2 heads from 226
+//           us to 216 in 8 bits, but one of 512 over 8000 at 32 / 8 from 59 to 62, and 24 sequences with 5 chunks in 8 bits from 75 to 82.
 struct Plan { int64_t tiles; int split, splits, nw; bool decode; };
 Plan plan_of(const PagedKv& kv, const PagedBatch& b, const PagedAttnArgs& a) {
   Plan pl;

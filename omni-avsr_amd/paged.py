@@ -379,8 +379,9 @@ def read(kv, batch, rows=None, *, dtype=None, out=None):
 
 def attention(kv, batch, q, scale=None, *, out=None, lse=None, split_keys=0):
     """Causal attention of the batch's new tokens q [rows][n_heads][head_dim] (or [rows][n_heads * head_dim]) over their sequences' cached context.  Returns
-    out, shaped like q (which it may be).  scale: default head_dim ** -0.5.  lse: float32 [rows][n_heads] to fill.  split_keys: keys per workgroup (a multiple of 256; 0: the
-    library's rule), for results whose last bits do not follow the batch a row is in."""
+    out, shaped like q (which it may be).  scale: default head_dim ** -0.5.  lse: float32 [rows][n_heads] to fill.  split_keys: keys per workgroup
+    (a multiple of 256; 0: the library's rule): a row then has the same bits in any batch of the same max_q.  max_q chooses the kernel: up to 16 rows per kv
+    head (max_q * n_heads / n_kv_heads) weigh bf16 values by two bf16 numbers each, more by one, a rounding more."""
     index, head_dim = kv.index, kv.head_dim
     if not (isinstance(q, torch.Tensor) and q.dim() in (2, 3) and q.is_cuda):
         _need(False, "q has to be rows on a GPU")
