@@ -398,7 +398,8 @@ int oavsr_op_paged_read(const oavsr_paged_kv* kv, const oavsr_paged_batch* b, vo
  * statistics in f32; keys a row does not see do not count, whatever their bytes hold.  A row that sees no key (p < 0): zeros, lse = -infinity.  A row of which
  * every visible key scores -infinity: NaN, as its softmax is, lse = -infinity.  With bf16 rows the weights of the values are sums of two bf16 numbers where
  * max_q * n_heads / n_kv_heads <= 16, single ones (2^-8 of each weight, relative) where it is more.  Weights, 1 at most, are multiplied with values (8 bits:
- * with their scales, before the bytes) and summed before the division by their sum: sums that pass 2^128, and scales below about 2^-100, lose their accuracy. */
+ * with their scales, before the bytes) and summed before the division by their sum: where such a sum passes 2^128, or values or scales lie below about 2^-100,
+ * the result loses its accuracy. */
 typedef struct oavsr_paged_attn_desc {
   int32_t n_heads;
   float scale;         /* > 0 */
