@@ -30,11 +30,13 @@ def _need(ok, what):
 
 
 def _no_gradient(t, name):
-    """Refuses a tensor whose gradient, or whose tangent in forward mode (which no_grad leaves on), a pass of torch's would form."""
-    if t.requires_grad:
-        _need(not torch.is_grad_enabled(), f"{name} asks for gradients, and none are formed here: call under torch.no_grad(), or detach it")
-    if _forward_ad._current_level >= 0:
-        _need(_forward_ad.unpack_dual(t).tangent is None, f"{name} carries a tangent, and no gradients are formed here: detach it")
+    _need(not (t.requires_grad and torch.is_grad_enabled()), f"{name} asks for gradients, and none are formed here: call under torch.no_grad(), or detach it")
+
+
+def _no_tangents(*tensors):
+    """For calls inside a level of forward mode, which no_grad leaves on."""
+    for t in tensors:
+        _need(not isinstance(t, torch.Tensor) or _forward_ad.unpack_dual(t).tangent is None, "a tensor carries a tangent, and no gradients are formed here: detach it")
 
 
 def _on_gpu(t, name, dtype, index=None):
@@ -150,9 +152,8 @@ class PagedKV(_Keeps):
 
     def _for(self, dtype):
         """The description for rows of `dtype`, of pools that ask for no gradients."""
-        dual = _forward_ad._current_level >= 0
         for t in self._pools:
-            if t.requires_grad or dual:
+            if t.requires_grad:
                 _no_gradient(t, "a pool of the cache")
         d = self.descs.get(dtype)
         if d is None:
@@ -233,7 +234,7 @@ def _vector(t, name, dtype, index, n=None):
     if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index and t.dim() == 1 and (n is None or t.numel() == n) and t.is_contiguous()):
         _on_gpu(t, name, dtype, index)
         _need(False, f"{name} is {tuple(t.shape)} (strides {t.stride()}), a vector{'' if n is None else f' of {n}'} in one piece is wanted")
-    if t.requires_grad or _forward_ad._current_level >= 0:
+    if t.requires_grad:
         _no_gradient(t, name)
     return t.data_ptr()
 
@@ -258,7 +259,9 @@ def qk_norm_rope(qkv, n_heads, n_kv_heads, pos, inv_freq, *, q_gain=None, k_gain
     it.  inv_freq [rot_dim / 2]: the first rot_dim dimensions of a head turn, halves against each other, or neighbours when interleaved."""
     if not (isinstance(qkv, torch.Tensor) and qkv.dim() == 2 and qkv.dtype in _DT and qkv.is_cuda):
         _need(False, "qkv has to be rows of float32 or bfloat16 on a GPU")
-    if qkv.requires_grad or _forward_ad._current_level >= 0:
+    if _forward_ad._current_level >= 0:
+        _no_tangents(qkv, inv_freq, q_gain, k_gain, *(out or ()))
+    if qkv.requires_grad:
         _no_gradient(qkv, "qkv")
     rows, width = qkv.shape
     dtype, index, all_heads = qkv.dtype, qkv.get_device(), n_heads + 2 * n_kv_heads
@@ -304,7 +307,9 @@ def append(kv, batch, qkv, inv_freq=None, *, pos=None, q_gain=None, k_gain=None,
     if _device() != index:
         with torch.cuda.device(index):
             return append(kv, batch, qkv, inv_freq, pos=pos, q_gain=q_gain, k_gain=k_gain, eps=eps, interleaved=interleaved, rot_scale=rot_scale, out=out)
-    if qkv.requires_grad or _forward_ad._current_level >= 0:
+    if _forward_ad._current_level >= 0:
+        _no_tangents(qkv, inv_freq, q_gain, k_gain, out, *kv._pools)
+    if qkv.requires_grad:
         _no_gradient(qkv, "qkv")
     rows, width = qkv.shape
     dtype = qkv.dtype
@@ -342,6 +347,8 @@ def read(kv, batch, rows=None, *, dtype=None, out=None):
     if _device() != index:
         with torch.cuda.device(index):
             return read(kv, batch, rows, dtype=dtype, out=out)
+    if _forward_ad._current_level >= 0:
+        _no_tangents(*(out or ()), *kv._pools)
     ldk = ldv = width = heads * head_dim
     if out is None:
         if not (rows is not None):
@@ -388,7 +395,9 @@ def attention(kv, batch, q, scale=None, *, out=None, lse=None, split_keys=0):
     if _device() != index:
         with torch.cuda.device(index):
             return attention(kv, batch, q, scale, out=out, lse=lse, split_keys=split_keys)
-    if q.requires_grad or _forward_ad._current_level >= 0:
+    if _forward_ad._current_level >= 0:
+        _no_tangents(q, out, lse, *kv._pools)
+    if q.requires_grad:
         _no_gradient(q, "q")
     dtype, shape = q.dtype, q.shape
     desc, rows = kv._for(dtype), shape[0]
